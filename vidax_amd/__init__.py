@@ -9,10 +9,14 @@ and the q/k prologue in front of them:
                                           (src/vidax/core/attention.py, rope3d.py)
   default_rope_dim_split, create_abs_rope3d_freqs, create_abs_rope3d_axis_freqs,
   apply_abs_rope3d, na3d_qk_norm_rope     (src/vidax/models/ltx2_5/diffusion_vae.py)
-all backed by libvx_attn.so (C ABI: include/vx_attn.h).
+and an 8-bit key/value cache with the attention over it:
+  KVCache, create_kv_cache, kv_cache_write, kv_cache_read, cached_attention, shared_prefix_attention
+all backed by libvx_attn.so (C ABI: include/vx_attn.h, include/vx_cache.h).
 """
 from .attention import (dot_product_attention, flash_attention, flash_supported, local_attention,
                         masked_self_attention)
+from .kv_cache import (KVCache, cached_attention, create_kv_cache, kv_cache_read, kv_cache_write,
+                       shared_prefix_attention)
 from .natten import na3d_block_attention, neighborhood_attention_3d
 from .prologue import (AbsRope3dAxes, apply_abs_rope3d, apply_rope3d, create_abs_rope3d_axis_freqs,
                        create_abs_rope3d_freqs, create_rope3d_freqs, default_rope_dim_split, na3d_qk_norm_rope,
@@ -36,4 +40,10 @@ __all__ = [
     "AbsRope3dAxes",
     "apply_abs_rope3d",
     "na3d_qk_norm_rope",
+    "KVCache",
+    "create_kv_cache",
+    "kv_cache_write",
+    "kv_cache_read",
+    "cached_attention",
+    "shared_prefix_attention",
 ]

@@ -1,4 +1,5 @@
-"""ctypes binding of libvx_attn.so (the C ABI in include/vx_attn.h).
+"""ctypes binding of libvx_attn.so (the C ABI in include/vx_attn.h and
+include/vx_cache.h).
 
 torch is imported before the library is opened so that the library binds to
 the HIP runtime torch already loaded (both resolve `libamdhip64.so.7`): device
@@ -51,6 +52,16 @@ EXPORTED_SYMBOLS = (
     "vx_flash_attn_device_plan",
 )
 
+CACHE_SYMBOLS = (  # include/vx_cache.h
+    "vx_kv_write_fwd",
+    "vx_kv_write_check",
+    "vx_kv_read_fwd",
+    "vx_kv_read_check",
+    "vx_cached_attn_fwd",
+    "vx_cached_attn_check",
+    "vx_cached_attn_workspace_size",
+)
+
 _lock = threading.Lock()
 _lib = None
 
@@ -69,6 +80,9 @@ _FLASH_BIAS_ARGS = [_p, _p, _p, _p, _p, _p, _p, _i64, _p, _i64p, _i32, _i32, _i3
 _NA3D_QPREP_ARGS = [_p, _p, _p, _p] + [_i32] * 9 + [_p, _f32, _f32, _p, _p, _i64]
 _NA3D_QPREP_AXES_ARGS = [_p, _p, _p, _p] + [_i32] * 9 + [_p, _f32, _f32, _p, _p, _i64, _i32p]
 _PROLOGUE_ARGS = [_p, _p, _p, _f32, _i32, _p, _p, _i64, _i32, _i32, _i32, _i32, _i64p, _i64p]
+_KV_WRITE_ARGS = [_p, _p, _i64p, _i64p] + [_p] * 4 + [_i32, _i32, _p, _p, _p] + [_i32] * 4
+_KV_READ_ARGS = [_p] * 4 + [_i32, _i32, _p, _p] + [_i32] * 4 + [_p, _p]
+_CACHED_ATTN_ARGS = [_p, _p, _i64p, _i64p] + ([_p] * 4 + [_i32, _i32]) * 2 + [_p] * 4 + [_i32] * 6 + [_f32]
 _SCALED_PROLOGUE_ARGS = _PROLOGUE_ARGS[:5] + [_f32] + _PROLOGUE_ARGS[5:]
 
 
@@ -149,6 +163,20 @@ def lib() -> ctypes.CDLL:
             h.vx_key_masks_fwd.argtypes = [_p, _i64p, _p, _i64p, _i32, _i32, _p, _p, _p, _i64, _p]
             h.vx_full_bias_fwd.restype = _i32
             h.vx_full_bias_fwd.argtypes = [_p, _i64p, _p, _i64p, _i32, _i32, _i32, _i32, _p, _p]
+            h.vx_kv_write_fwd.restype = _i32
+            h.vx_kv_write_fwd.argtypes = _KV_WRITE_ARGS + [_p]
+            h.vx_kv_write_check.restype = _i32
+            h.vx_kv_write_check.argtypes = _KV_WRITE_ARGS
+            h.vx_kv_read_fwd.restype = _i32
+            h.vx_kv_read_fwd.argtypes = _KV_READ_ARGS + [_p]
+            h.vx_kv_read_check.restype = _i32
+            h.vx_kv_read_check.argtypes = _KV_READ_ARGS
+            h.vx_cached_attn_fwd.restype = _i32
+            h.vx_cached_attn_fwd.argtypes = _CACHED_ATTN_ARGS + [_p, _i64, _p]
+            h.vx_cached_attn_check.restype = _i32
+            h.vx_cached_attn_check.argtypes = _CACHED_ATTN_ARGS
+            h.vx_cached_attn_workspace_size.restype = _i64
+            h.vx_cached_attn_workspace_size.argtypes = [_i32] * 8
             h.vx_last_launch.restype = ctypes.c_char_p
             h.vx_last_launch.argtypes = []
             _lib = h

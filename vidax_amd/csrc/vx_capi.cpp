@@ -1,8 +1,10 @@
-// C ABI of the attention kernels (declared in include/vx_attn.h).
+// C ABI of the attention kernels (declared in include/vx_attn.h) and of the 8-bit
+// cache (include/vx_cache.h).
 //
 // Plain C++ with no HIP dependency: argument checks, error reporting and the
 // failure-injection hook run on a host without a GPU. The kernels are reached
-// through vx::launch_* (flash_fwd.hip, na3d_fwd.hip, qk_prologue.hip).
+// through vx::launch_* (flash_fwd.hip, na3d_fwd.hip, qk_prologue.hip, kv_cache.hip,
+// cached_attn.hip).
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -15,6 +17,7 @@
 #include <string>
 
 #include "../../include/vx_attn.h"
+#include "../../include/vx_cache.h"
 #include "vx_kernels.h"
 
 namespace {
@@ -634,6 +637,139 @@ int32_t injected() {
   return VX_OK;
 }
 
+// ---- the 8-bit key/value cache
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+int32_t cache_check(const char* what, const void* k, const void* v, const uint8_t* ks, const uint8_t* vs,
+                    int32_t slots, int32_t cap, int32_t Hk, int32_t D, vx::KvCache* c) {
+  if (k == nullptr || v == nullptr || ks == nullptr || vs == nullptr)
+    return fail(VX_ERR_INVALID_ARGUMENT, "%s arrays must be non-NULL", what);
+  if (!aligned16(k) || !aligned16(v) || !aligned16(ks) || !aligned16(vs))
+    return fail(VX_ERR_INVALID_ARGUMENT, "%s arrays must be 16-byte aligned", what);
+  if (slots < 1 || Hk < 1)
+    return fail(VX_ERR_INVALID_ARGUMENT, "%s: slots (%d) and num_kv_heads (%d) must be >= 1", what, slots, Hk);
+  if (Hk > 65535) return fail(VX_ERR_INVALID_ARGUMENT, "num_kv_heads (%d) must be <= 65535", Hk);
+  if (cap < 64 || cap % 64 != 0)
+    return fail(VX_ERR_INVALID_ARGUMENT, "%s: capacity (%d) must be a multiple of 64 and >= 64", what, cap);
+  if (D != 64 && D != 128)
+    return fail(VX_ERR_UNSUPPORTED, "head_dim %d is not supported (this build handles 64 and 128)", D);
+  *c = vx::KvCache{static_cast<uint8_t*>(const_cast<void*>(k)), static_cast<uint8_t*>(const_cast<void*>(v)),
+                   const_cast<uint8_t*>(ks), const_cast<uint8_t*>(vs), slots, cap, Hk, D};
+  return VX_OK;
+}
+
+// Batch, sequence and index arrays of a cache call.
+int32_t cache_batch_check(const int32_t* i0, const int32_t* i1, const int32_t* slots, int32_t num_slots, int32_t B,
+                          int32_t S) {
+  if (B < 1 || B > 65535) return fail(VX_ERR_INVALID_ARGUMENT, "batch (%d) must be in 1..65535", B);
+  if (S < 1) return fail(VX_ERR_INVALID_ARGUMENT, "seq (%d) must be >= 1", S);
+  if (!aligned4(i0) || !aligned4(i1) || !aligned4(slots))
+    return fail(VX_ERR_INVALID_ARGUMENT, "index arrays must be 4-byte aligned");
+  if (slots == nullptr && B > num_slots)
+    return fail(VX_ERR_INVALID_ARGUMENT, "batch (%d) exceeds the cache's %d slots and no slots are given", B,
+                num_slots);
+  return VX_OK;
+}
+
+int32_t kv_grid_check(int32_t S, int32_t Hk) {
+  if (((int64_t)S + vx::kKvTokensPerWave - 1) / vx::kKvTokensPerWave * Hk > INT32_MAX)
+    return fail(VX_ERR_UNSUPPORTED, "seq (%d) times num_kv_heads (%d) is too large", S, Hk);
+  return ok();
+}
+
+int32_t kv_write_check(const void* k, const void* v, const int64_t* ks, const int64_t* vs, const void* ck,
+                       const void* cv, const uint8_t* cks, const uint8_t* cvs, int32_t slots, int32_t cap,
+                       const int32_t* start, const int32_t* num, const int32_t* slot_of, int32_t B, int32_t S,
+                       int32_t Hk, int32_t D, vx::KvWriteArgs* a) {
+  if (k == nullptr || v == nullptr) return fail(VX_ERR_INVALID_ARGUMENT, "k and v must be non-NULL");
+  if (!aligned16(k) || !aligned16(v)) return fail(VX_ERR_INVALID_ARGUMENT, "k and v must be 16-byte aligned");
+  int32_t rc;
+  if ((rc = cache_check("cache", ck, cv, cks, cvs, slots, cap, Hk, D, &a->c)) != VX_OK) return rc;
+  if ((rc = cache_batch_check(start, num, slot_of, slots, B, S)) != VX_OK) return rc;
+  a->k = k;
+  a->v = v;
+  strides_or_default(ks, S, Hk, D, a->ks);
+  strides_or_default(vs, S, Hk, D, a->vs);
+  if ((rc = check_strides("k", a->ks, S)) != VX_OK || (rc = check_strides("v", a->vs, S)) != VX_OK) return rc;
+  a->start = start;
+  a->num = num;
+  a->slots = slot_of;
+  a->B = B;
+  a->S = S;
+  return kv_grid_check(S, Hk);
+}
+
+int32_t kv_read_check(const void* ck, const void* cv, const uint8_t* cks, const uint8_t* cvs, int32_t slots,
+                      int32_t cap, const int32_t* start, const int32_t* slot_of, int32_t B, int32_t S, int32_t Hk,
+                      int32_t D, const void* k_out, const void* v_out, vx::KvReadArgs* a) {
+  if (k_out == nullptr || v_out == nullptr) return fail(VX_ERR_INVALID_ARGUMENT, "k_out and v_out must be non-NULL");
+  if (!aligned16(k_out) || !aligned16(v_out))
+    return fail(VX_ERR_INVALID_ARGUMENT, "k_out and v_out must be 16-byte aligned");
+  int32_t rc;
+  if ((rc = cache_check("cache", ck, cv, cks, cvs, slots, cap, Hk, D, &a->c)) != VX_OK) return rc;
+  if ((rc = cache_batch_check(start, nullptr, slot_of, slots, B, S)) != VX_OK) return rc;
+  a->start = start;
+  a->slots = slot_of;
+  a->B = B;
+  a->S = S;
+  a->k_out = const_cast<void*>(k_out);
+  a->v_out = const_cast<void*>(v_out);
+  return kv_grid_check(S, Hk);
+}
+
+// Query rows that share a cached head are held in 31 bits.
+constexpr int64_t kMaxSharedRows = 1 << 30;
+
+int32_t cached_attn_check(const void* q, const void* out, const int64_t* qs, const int64_t* os, const void* ck,
+                          const void* cv, const uint8_t* cks, const uint8_t* cvs, int32_t slots, int32_t cap,
+                          const void* pk, const void* pv, const uint8_t* pks, const uint8_t* pvs, int32_t n_prefix,
+                          int32_t p_cap, const int32_t* kv_len, const int32_t* q_len, const int32_t* slot_of,
+                          const int32_t* prefix_len, int32_t B, int32_t Sq, int32_t H, int32_t Hk, int32_t D,
+                          int32_t causal, float scale, vx::CachedAttnArgs* a) {
+  if (q == nullptr || out == nullptr) return fail(VX_ERR_INVALID_ARGUMENT, "q and out must be non-NULL");
+  if (!aligned16(q) || !aligned16(out)) return fail(VX_ERR_INVALID_ARGUMENT, "q and out must be 16-byte aligned");
+  int32_t rc;
+  if ((rc = cache_check("cache", ck, cv, cks, cvs, slots, cap, Hk, D, &a->c)) != VX_OK) return rc;
+  if ((rc = cache_batch_check(kv_len, q_len, slot_of, slots, B, Sq)) != VX_OK) return rc;
+  if (H < 1 || H > 65535 || H % Hk != 0)
+    return fail(VX_ERR_INVALID_ARGUMENT, "num_heads (%d) must be a multiple of num_kv_heads (%d), at most 65535", H,
+                Hk);
+  if (causal != 0 && causal != 1) return fail(VX_ERR_INVALID_ARGUMENT, "causal must be 0 or 1");
+  if (!(scale > 0.f) || !std::isfinite(scale))
+    return fail(VX_ERR_INVALID_ARGUMENT, "scale must be positive and finite (got %g)", (double)scale);
+  int64_t sharers = 1;
+  a->prefix = vx::KvCache{};
+  a->prefix_len = nullptr;
+  if (pk != nullptr || pv != nullptr || pks != nullptr || pvs != nullptr) {
+    if ((rc = cache_check("prefix", pk, pv, pks, pvs, n_prefix, p_cap, Hk, D, &a->prefix)) != VX_OK) return rc;
+    if (B % n_prefix != 0)
+      return fail(VX_ERR_INVALID_ARGUMENT, "batch (%d) must be a multiple of num_prefixes (%d)", B, n_prefix);
+    if (!aligned4(prefix_len)) return fail(VX_ERR_INVALID_ARGUMENT, "index arrays must be 4-byte aligned");
+    a->prefix_len = prefix_len;
+    sharers = B / n_prefix;
+  } else if (n_prefix != 0 || prefix_len != nullptr) {
+    return fail(VX_ERR_INVALID_ARGUMENT, "num_prefixes and prefix_len need the prefix arrays");
+  }
+  if (sharers * Sq > kMaxSharedRows / (H / Hk))
+    return fail(VX_ERR_UNSUPPORTED, "%lld queries of %d heads on one cached head are too many",
+                (long long)(sharers * Sq), H / Hk);
+  a->q = q;
+  a->o = const_cast<void*>(out);
+  strides_or_default(qs, Sq, H, D, a->qs);
+  strides_or_default(os, Sq, H, D, a->os);
+  if ((rc = check_strides("q", a->qs, Sq)) != VX_OK || (rc = check_strides("out", a->os, Sq)) != VX_OK) return rc;
+  a->kv_len = kv_len;
+  a->q_len = q_len;
+  a->slots = slot_of;
+  a->B = B;
+  a->Sq = Sq;
+  a->H = H;
+  a->causal = causal;
+  a->scale = scale;
+  a->ws = nullptr;
+  return ok();
+}
+
 }  // namespace
 
 extern "C" {
@@ -1063,6 +1199,101 @@ int32_t vx_rmsnorm_scale_rope_fwd(const void* x, void* out, const float* weight,
   if (err != 0) return fail(VX_ERR_LAUNCH, "rmsnorm/rope launch failed (hipError_t %d)", err);
   g_last_launch = launched;
   return ok();
+}
+
+int32_t vx_kv_write_check(const void* k, const void* v, const int64_t* k_strides, const int64_t* v_strides,
+                          const void* cache_k, const void* cache_v, const uint8_t* k_scale, const uint8_t* v_scale,
+                          int32_t num_slots, int32_t capacity, const int32_t* start, const int32_t* num,
+                          const int32_t* slots, int32_t batch, int32_t seq, int32_t num_kv_heads, int32_t head_dim) {
+  vx::KvWriteArgs a;
+  return kv_write_check(k, v, k_strides, v_strides, cache_k, cache_v, k_scale, v_scale, num_slots, capacity, start,
+                        num, slots, batch, seq, num_kv_heads, head_dim, &a);
+}
+
+int32_t vx_kv_write_fwd(const void* k, const void* v, const int64_t* k_strides, const int64_t* v_strides,
+                        void* cache_k, void* cache_v, uint8_t* k_scale, uint8_t* v_scale, int32_t num_slots,
+                        int32_t capacity, const int32_t* start, const int32_t* num, const int32_t* slots,
+                        int32_t batch, int32_t seq, int32_t num_kv_heads, int32_t head_dim, void* stream) {
+  vx::KvWriteArgs a;
+  int32_t rc = kv_write_check(k, v, k_strides, v_strides, cache_k, cache_v, k_scale, v_scale, num_slots, capacity,
+                              start, num, slots, batch, seq, num_kv_heads, head_dim, &a);
+  if (rc != VX_OK) return rc;
+  if ((rc = injected()) != VX_OK) return rc;
+  const char* launched = "";
+  const int err = vx::launch_kv_write(a, stream, &launched);
+  if (err != 0) return fail(VX_ERR_LAUNCH, "cache write launch failed (hipError_t %d)", err);
+  g_last_launch = launched;
+  return ok();
+}
+
+int32_t vx_kv_read_check(const void* cache_k, const void* cache_v, const uint8_t* k_scale, const uint8_t* v_scale,
+                         int32_t num_slots, int32_t capacity, const int32_t* start, const int32_t* slots,
+                         int32_t batch, int32_t seq, int32_t num_kv_heads, int32_t head_dim, const void* k_out,
+                         const void* v_out) {
+  vx::KvReadArgs a;
+  return kv_read_check(cache_k, cache_v, k_scale, v_scale, num_slots, capacity, start, slots, batch, seq,
+                       num_kv_heads, head_dim, k_out, v_out, &a);
+}
+
+int32_t vx_kv_read_fwd(const void* cache_k, const void* cache_v, const uint8_t* k_scale, const uint8_t* v_scale,
+                       int32_t num_slots, int32_t capacity, const int32_t* start, const int32_t* slots,
+                       int32_t batch, int32_t seq, int32_t num_kv_heads, int32_t head_dim, void* k_out, void* v_out,
+                       void* stream) {
+  vx::KvReadArgs a;
+  int32_t rc = kv_read_check(cache_k, cache_v, k_scale, v_scale, num_slots, capacity, start, slots, batch, seq,
+                             num_kv_heads, head_dim, k_out, v_out, &a);
+  if (rc != VX_OK) return rc;
+  if ((rc = injected()) != VX_OK) return rc;
+  const char* launched = "";
+  const int err = vx::launch_kv_read(a, stream, &launched);
+  if (err != 0) return fail(VX_ERR_LAUNCH, "cache read launch failed (hipError_t %d)", err);
+  g_last_launch = launched;
+  return ok();
+}
+
+int32_t vx_cached_attn_check(const void* q, const void* out, const int64_t* q_strides, const int64_t* out_strides,
+                             const void* cache_k, const void* cache_v, const uint8_t* k_scale, const uint8_t* v_scale,
+                             int32_t num_slots, int32_t capacity, const void* prefix_k, const void* prefix_v,
+                             const uint8_t* prefix_k_scale, const uint8_t* prefix_v_scale, int32_t num_prefixes,
+                             int32_t prefix_capacity, const int32_t* kv_len, const int32_t* q_len,
+                             const int32_t* slots, const int32_t* prefix_len, int32_t batch, int32_t seq_q,
+                             int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t causal, float scale) {
+  vx::CachedAttnArgs a;
+  return cached_attn_check(q, out, q_strides, out_strides, cache_k, cache_v, k_scale, v_scale, num_slots, capacity,
+                           prefix_k, prefix_v, prefix_k_scale, prefix_v_scale, num_prefixes, prefix_capacity, kv_len,
+                           q_len, slots, prefix_len, batch, seq_q, num_heads, num_kv_heads, head_dim, causal, scale,
+                           &a);
+}
+
+int32_t vx_cached_attn_fwd(const void* q, void* out, const int64_t* q_strides, const int64_t* out_strides,
+                           const void* cache_k, const void* cache_v, const uint8_t* k_scale, const uint8_t* v_scale,
+                           int32_t num_slots, int32_t capacity, const void* prefix_k, const void* prefix_v,
+                           const uint8_t* prefix_k_scale, const uint8_t* prefix_v_scale, int32_t num_prefixes,
+                           int32_t prefix_capacity, const int32_t* kv_len, const int32_t* q_len, const int32_t* slots,
+                           const int32_t* prefix_len, int32_t batch, int32_t seq_q, int32_t num_heads,
+                           int32_t num_kv_heads, int32_t head_dim, int32_t causal, float scale, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+  vx::CachedAttnArgs a;
+  int32_t rc = cached_attn_check(q, out, q_strides, out_strides, cache_k, cache_v, k_scale, v_scale, num_slots,
+                                 capacity, prefix_k, prefix_v, prefix_k_scale, prefix_v_scale, num_prefixes,
+                                 prefix_capacity, kv_len, q_len, slots, prefix_len, batch, seq_q, num_heads,
+                                 num_kv_heads, head_dim, causal, scale, &a);
+  if (rc != VX_OK) return rc;
+  if ((rc = injected()) != VX_OK) return rc;
+  (void)workspace;
+  (void)workspace_bytes;
+  const char* launched = "";
+  const int err = vx::launch_cached_attn(a, stream, &launched);
+  if (err != 0) return fail(VX_ERR_LAUNCH, "cached attention launch failed (hipError_t %d)", err);
+  g_last_launch = launched;
+  return ok();
+}
+
+int64_t vx_cached_attn_workspace_size(int32_t capacity, int32_t num_prefixes, int32_t prefix_capacity, int32_t batch,
+                                      int32_t seq_q, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim) {
+  (void)capacity, (void)num_prefixes, (void)prefix_capacity, (void)batch, (void)seq_q, (void)num_heads;
+  (void)num_kv_heads, (void)head_dim;
+  return 0;
 }
 
 }  // extern "C"

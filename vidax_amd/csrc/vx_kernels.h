@@ -164,6 +164,59 @@ struct FullBiasArgs {
   float* out;
 };
 
+// An 8-bit key/value cache: rows of D e4m3 bytes in (slot, kv head, position)
+// order, a scale byte (e8m0) each; cap is a multiple of 64.
+struct KvCache {
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* ks;
+  uint8_t* vs;
+  int32_t slots, cap, Hk, D;
+};
+
+// Positions per wave of the cache's write and read kernels.
+constexpr int kKvTokensPerWave = 16;
+
+// New rows (B, S, Hk, D) to positions start[b] + t of slot slots[b], t < num[b].
+struct KvWriteArgs {
+  const void* k;
+  const void* v;
+  int64_t ks[3], vs[3];  // elements: {batch, seq, head}
+  KvCache c;
+  const int32_t* start;  // [B] or nullptr (0), as num (S) and slots (b)
+  const int32_t* num;
+  const int32_t* slots;
+  int32_t B, S;
+};
+
+// Positions start[b] + t, t < S, of slot slots[b] to contiguous (B, S, Hk, D).
+struct KvReadArgs {
+  KvCache c;
+  const int32_t* start;
+  const int32_t* slots;
+  int32_t B, S;
+  void* k_out;
+  void* v_out;
+};
+
+// Attention of q (B, Sq, H, D) over the first kv_len[b] positions of slot
+// slots[b] of `c` and, with a prefix (prefix.k not null), the first
+// prefix_len[g] positions of slot g = b / (B / prefix.slots) of `prefix`.
+struct CachedAttnArgs {
+  const void* q;
+  void* o;
+  int64_t qs[3], os[3];  // elements: {batch, seq, head}
+  KvCache c, prefix;
+  const int32_t* kv_len;  // [B] or nullptr (cap), as q_len (Sq) and slots (b)
+  const int32_t* q_len;
+  const int32_t* slots;
+  const int32_t* prefix_len;  // [prefix.slots] or nullptr (prefix.cap)
+  int32_t B, Sq, H;
+  int32_t causal;
+  float scale;
+  float* ws;
+};
+
 // Compute units of the current device (0 if unknown), cached per device.
 int device_cu_count();
 
@@ -179,6 +232,9 @@ int launch_na3d_fwd(const Na3dArgs& a, void* stream, const char** launched);
 int launch_qk_prologue(const PrologueArgs& a, void* stream, const char** launched);
 int launch_key_masks(const KeyMaskArgs& a, void* stream, const char** launched);
 int launch_full_bias(const FullBiasArgs& a, void* stream, const char** launched);
+int launch_kv_write(const KvWriteArgs& a, void* stream, const char** launched);
+int launch_kv_read(const KvReadArgs& a, void* stream, const char** launched);
+int launch_cached_attn(const CachedAttnArgs& a, void* stream, const char** launched);
 
 // Measurement only: n_groups one-wave workgroups each store (XCD id, HW_ID,
 // shader clock counter, real-time counter) as four uint64 at out + 4 * group;
