@@ -717,8 +717,24 @@ int32_t kv_read_check(const void* ck, const void* cv, const uint8_t* cks, const 
   return kv_grid_check(S, Hk);
 }
 
-// Query rows that share a cached head are held in 31 bits.
+// Query rows that share a cached head, tiles of them and an item's rows are
+// held in 31 bits by the kernels and their grids.
 constexpr int64_t kMaxSharedRows = 1 << 30;
+
+int32_t cached_sizes_check(int32_t n_prefix, int32_t B, int32_t Sq, int32_t H, int32_t Hk) {
+  if (B < 1 || B > 65535) return fail(VX_ERR_INVALID_ARGUMENT, "batch (%d) must be in 1..65535", B);
+  if (Sq < 1) return fail(VX_ERR_INVALID_ARGUMENT, "seq (%d) must be >= 1", Sq);
+  if (Hk < 1 || H < 1 || H > 65535 || H % Hk != 0)
+    return fail(VX_ERR_INVALID_ARGUMENT, "num_heads (%d) must be a multiple of num_kv_heads (%d), at most 65535", H,
+                Hk);
+  if (n_prefix < 0 || (n_prefix > 0 && B % n_prefix != 0))
+    return fail(VX_ERR_INVALID_ARGUMENT, "batch (%d) must be a multiple of num_prefixes (%d)", B, n_prefix);
+  const int64_t rows = (int64_t)Sq * (H / Hk), sharers = n_prefix > 0 ? B / n_prefix : 1;
+  if (rows > kMaxSharedRows || sharers * rows > kMaxSharedRows || (rows + 127) / 128 * B > kMaxSharedRows ||
+      (int64_t)H * Sq > 4 * kMaxSharedRows)
+    return fail(VX_ERR_UNSUPPORTED, "%d queries of %d heads for %d items are too many", Sq, H, B);
+  return VX_OK;
+}
 
 int32_t cached_attn_check(const void* q, const void* out, const int64_t* qs, const int64_t* os, const void* ck,
                           const void* cv, const uint8_t* cks, const uint8_t* cvs, int32_t slots, int32_t cap,
@@ -731,28 +747,20 @@ int32_t cached_attn_check(const void* q, const void* out, const int64_t* qs, con
   int32_t rc;
   if ((rc = cache_check("cache", ck, cv, cks, cvs, slots, cap, Hk, D, &a->c)) != VX_OK) return rc;
   if ((rc = cache_batch_check(kv_len, q_len, slot_of, slots, B, Sq)) != VX_OK) return rc;
-  if (H < 1 || H > 65535 || H % Hk != 0)
-    return fail(VX_ERR_INVALID_ARGUMENT, "num_heads (%d) must be a multiple of num_kv_heads (%d), at most 65535", H,
-                Hk);
+  if ((rc = cached_sizes_check(0, B, Sq, H, Hk)) != VX_OK) return rc;
   if (causal != 0 && causal != 1) return fail(VX_ERR_INVALID_ARGUMENT, "causal must be 0 or 1");
   if (!(scale > 0.f) || !std::isfinite(scale))
     return fail(VX_ERR_INVALID_ARGUMENT, "scale must be positive and finite (got %g)", (double)scale);
-  int64_t sharers = 1;
   a->prefix = vx::KvCache{};
   a->prefix_len = nullptr;
   if (pk != nullptr || pv != nullptr || pks != nullptr || pvs != nullptr) {
     if ((rc = cache_check("prefix", pk, pv, pks, pvs, n_prefix, p_cap, Hk, D, &a->prefix)) != VX_OK) return rc;
-    if (B % n_prefix != 0)
-      return fail(VX_ERR_INVALID_ARGUMENT, "batch (%d) must be a multiple of num_prefixes (%d)", B, n_prefix);
+    if ((rc = cached_sizes_check(n_prefix, B, Sq, H, Hk)) != VX_OK) return rc;
     if (!aligned4(prefix_len)) return fail(VX_ERR_INVALID_ARGUMENT, "index arrays must be 4-byte aligned");
     a->prefix_len = prefix_len;
-    sharers = B / n_prefix;
   } else if (n_prefix != 0 || prefix_len != nullptr) {
     return fail(VX_ERR_INVALID_ARGUMENT, "num_prefixes and prefix_len need the prefix arrays");
   }
-  if (sharers * Sq > kMaxSharedRows / (H / Hk))
-    return fail(VX_ERR_UNSUPPORTED, "%lld queries of %d heads on one cached head are too many",
-                (long long)(sharers * Sq), H / Hk);
   a->q = q;
   a->o = const_cast<void*>(out);
   strides_or_default(qs, Sq, H, D, a->qs);
@@ -1280,8 +1288,12 @@ int32_t vx_cached_attn_fwd(const void* q, void* out, const int64_t* q_strides, c
                                  num_kv_heads, head_dim, causal, scale, &a);
   if (rc != VX_OK) return rc;
   if ((rc = injected()) != VX_OK) return rc;
-  (void)workspace;
-  (void)workspace_bytes;
+  const int64_t need = vx::cached_attn_workspace(a.c.cap, a.prefix.slots, a.prefix.cap, batch, seq_q, num_heads,
+                                                 num_kv_heads, head_dim);
+  if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need))
+    return fail(VX_ERR_INVALID_ARGUMENT, "a 16-byte aligned workspace of %lld bytes is needed (%lld given)",
+                (long long)need, (long long)(workspace != nullptr ? workspace_bytes : 0));
+  a.ws = static_cast<float*>(workspace);
   const char* launched = "";
   const int err = vx::launch_cached_attn(a, stream, &launched);
   if (err != 0) return fail(VX_ERR_LAUNCH, "cached attention launch failed (hipError_t %d)", err);
@@ -1291,9 +1303,19 @@ int32_t vx_cached_attn_fwd(const void* q, void* out, const int64_t* q_strides, c
 
 int64_t vx_cached_attn_workspace_size(int32_t capacity, int32_t num_prefixes, int32_t prefix_capacity, int32_t batch,
                                       int32_t seq_q, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim) {
-  (void)capacity, (void)num_prefixes, (void)prefix_capacity, (void)batch, (void)seq_q, (void)num_heads;
-  (void)num_kv_heads, (void)head_dim;
-  return 0;
+  vx::KvCache c;
+  int32_t rc;
+  const void* some = reinterpret_cast<const void*>(uintptr_t(1) << 20);  // (an aligned address, not looked at)
+  const uint8_t* scales = static_cast<const uint8_t*>(some);
+  if ((rc = cache_check("cache", some, some, scales, scales, 1, capacity, num_kv_heads, head_dim, &c)) != VX_OK ||
+      (rc = cached_sizes_check(num_prefixes, batch, seq_q, num_heads, num_kv_heads)) != VX_OK)
+    return -1;
+  if (num_prefixes > 0 && cache_check("prefix", some, some, scales, scales, num_prefixes, prefix_capacity,
+                                      num_kv_heads, head_dim, &c) != VX_OK)
+    return -1;
+  ok();
+  return vx::cached_attn_workspace(capacity, num_prefixes, prefix_capacity, batch, seq_q, num_heads, num_kv_heads,
+                                   head_dim);
 }
 
 }  // extern "C"

@@ -224,6 +224,10 @@ int device_cu_count();
 // (used by vx_flash_attn_noalloc_fwd); returns a hipError_t value.
 int noalloc_scratch(void** ptr, int64_t* bytes);
 
+// Bytes of partial results that launch_cached_attn needs for these sizes on the current device.
+int64_t cached_attn_workspace(int32_t cap, int32_t n_prefix, int32_t p_cap, int32_t B, int32_t Sq, int32_t H,
+                              int32_t Hk, int32_t D);
+
 // All return a hipError_t value (0 on success) and store the name of the kernel they launched in *launched (a string with
 // static storage, built from the launched instantiation's template
 // arguments).
