@@ -26,6 +26,7 @@
 #include "vx_kernels.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace vx {
 namespace {
@@ -36,6 +37,10 @@ constexpr float kNegBig = -1.0e30f;  // finite "no key seen yet" reference point
 constexpr float kSlack = 8.0f;       // weights up to 2^kSlack before the reference point moves
 
 typedef VX_LDS unsigned char lds_u8;
+// (a pointer made from an integer is a flat one unless its type says more, and a
+// flat load holds up the LDS counter that every barrier waits for)
+#define VX_GLOBAL __attribute__((address_space(1)))
+typedef VX_GLOBAL const uint8_t global_u8;
 
 template <int N>
 __device__ __forceinline__ void wait_copies() {
@@ -171,6 +176,19 @@ __device__ __forceinline__ int own_bound(const CachedAttnArgs& a, int b, int i, 
   return a.causal ? min(max(len - m + i + 1, 0), len) : len;
 }
 
+// One launch's work on one kind of streams.
+struct Part {
+  Streams s;
+  int32_t rows, per;          // rows of a stream per kv head; batch items that share it
+  int32_t budget, min_chunk;  // of its cut (budget 0: one item per stream)
+  int32_t items;              // items to launch, per kv head and row tile: some may have nothing to do
+  int32_t prefix;             // 1: every row sees every key
+  int32_t one_round;          // 1: all workgroups find a place at once (many_part)
+  int32_t direct;             // 1: a stream of one item writes its output itself
+  int32_t few;                // few_part, else many_part
+  float* ws;                  // partial results
+};
+
 // Partial results in the workspace, one block per (item, kv head): rows x D
 // unnormalised fp32 outputs, then (reference point, sum) per row.
 __device__ __forceinline__ int64_t part_floats(int64_t rows, int D) { return (rows * (D + 2) + 3) & ~(int64_t)3; }
@@ -199,7 +217,8 @@ struct FewCfg {
   static constexpr int kRing = 2;
   static constexpr int kOutRow = D + 4;                  // fp32 values between rows of the exchange
   static constexpr int kExchange = 32 * kOutRow * 4;
-  static constexpr int kSmem = (kRing * kBuf > kExchange ? kRing * kBuf : kExchange) * kWaves;
+  static constexpr int kTiles = (kRing * kBuf > kExchange ? kRing * kBuf : kExchange) * kWaves;
+  static constexpr int kSmem = kTiles + kWaves * 32 * 8;  // then (reference point, sum) of the waves' rows
 };
 
 // One wave's softmax state and the step over 32 keys.
@@ -211,28 +230,28 @@ struct FewState {
 };
 
 template <int D>
-__global__ __launch_bounds__(kThreads, 2) void few_kernel(const CachedAttnArgs a, const Streams s, const int rows,
-                                                        const int per, const int prefix, const int budget,
-                                                        const int min_chunk, const int direct, float* ws) {
+__device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt, const int block,
+                                         unsigned char* smem) {
   using C = FewCfg<D>;
   using T = Fp8Tile<D>;
-  __shared__ __attribute__((aligned(256))) unsigned char smem[C::kSmem];
-  __shared__ float ml[kWaves][32][2];
+  const Streams& s = pt.s;
+  const int rows = pt.rows;
+  float(*const ml)[32][2] = (float(*)[32][2])(smem + C::kTiles);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hf = lane >> 5, col = lane & 31;
-  const int kvh = blockIdx.y, Hk = s.c.Hk;
+  const int Hk = s.c.Hk, kvh = block % Hk, item = block / Hk;
   Cut cut;
-  const int stream = __builtin_amdgcn_readfirstlane(stream_of<kFewTile>(s, budget, min_chunk, blockIdx.x, cut));
+  const int stream = __builtin_amdgcn_readfirstlane(stream_of<kFewTile>(s, pt.budget, pt.min_chunk, item, cut));
   if (stream < 0) return;  // (the whole workgroup)
   const int len = __builtin_amdgcn_readfirstlane(keys_of(s, stream));
   const int tiles = (len + kFewTile - 1) / kFewTile;
-  const int chunk_no = blockIdx.x - __builtin_amdgcn_readfirstlane(cut.first);
+  const int chunk_no = item - __builtin_amdgcn_readfirstlane(cut.first);
   const int chunk = __builtin_amdgcn_readfirstlane(cut.chunk);
-  const int t0 = min((int64_t)chunk_no * chunk, (int64_t)tiles);
-  const int t1 = min((int64_t)t0 + chunk, (int64_t)tiles);
+  const int t0 = __builtin_amdgcn_readfirstlane((int)min((int64_t)chunk_no * chunk, (int64_t)tiles));
+  const int t1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)t0 + chunk, (int64_t)tiles));
 
-  const RowMap map{a, stream, kvh, a.H / Hk, per};
+  const RowMap map{a, stream, kvh, a.H / Hk, pt.per};
   int rb, ri, rh;
   map.place(min(col, rows - 1), rb, ri, rh);
   FewState<D> st;
@@ -245,7 +264,7 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const CachedAttnArgs a
     }
   }
   // keys this lane's row sees, and those that every row sees
-  const int bound = prefix ? len : own_bound(a, rb, ri, len);
+  const int bound = pt.prefix ? len : own_bound(a, rb, ri, len);
   int all = bound;
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) all = min(all, __shfl_xor(all, off, 64));
@@ -380,8 +399,8 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const CachedAttnArgs a
     }
   }
   __syncthreads();
-  const bool final_rows = direct && cut.count == 1;
-  float* const part = final_rows ? nullptr : ws + ((int64_t)blockIdx.x * Hk + kvh) * part_floats(rows, D);
+  const bool final_rows = pt.direct && cut.count == 1;
+  float* const part = final_rows ? nullptr : pt.ws + ((int64_t)item * Hk + kvh) * part_floats(rows, D);
   for (int x = threadIdx.x; x < rows * (D / 4); x += kThreads) {
     const int r = x / (D / 4), d = (x % (D / 4)) * 4;
     float M = ml[0][r][0];
@@ -414,122 +433,141 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const CachedAttnArgs a
 }
 
 // ------------------------------------------------------------------ many rows
-constexpr int kManyTile = 64;             // keys per tile of many_kernel
-constexpr int kManyRows = 32 * kWaves;    // rows per workgroup
+constexpr int kManyTile = 64;  // keys per tile of many_part
 
-template <int D>
+// A workgroup of W waves of 32 rows. LDS: two K tiles, two V tiles of bf16; a
+// tile is D / 64 half planes of 64 keys x 128 bytes, a row's 16-byte chunks XOR
+// half_swizzle (as in flash_fwd.hip).
+template <int D, int W>
 struct ManyCfg {
-  static constexpr int kHalf = kManyTile * 128;          // 64 keys x 64 dims of bf16
-  static constexpr int kTileBytes = kManyTile * D * 2;   // of K, and of V
-  static constexpr int kBuf = 2 * kTileBytes;
-  static constexpr int kLoads = kManyTile * (D / 16) / kThreads;  // 16-byte chunks of K, and of V, per thread
-  static constexpr int kSmem = 2 * kBuf;
+  static constexpr int kRows = 32 * W;
+  static constexpr int kHalf = kManyTile * 128;         // 64 keys x 64 dims
+  static constexpr int kTileBytes = kManyTile * D * 2;  // of K, and of V
+  static constexpr int kVBuf = 0, kKBuf = 2 * kTileBytes;
+  static constexpr int kLoads = kManyTile * (D / 16) / (W * 64);  // 16-byte chunks of K, and of V, per thread
+  static constexpr int kSmem = 4 * kTileBytes;
+  static constexpr int kDB = D / 32, kDS = D / 16;
+  static constexpr int kPV = 4 * kDB, kQK = 2 * kDS, kSlots = kPV + kQK;
+  static constexpr int kAhead = 2;  // fragments read ahead of their MFMA
 };
 
-template <int D>
-__global__ __launch_bounds__(kThreads, 2) void many_kernel(const CachedAttnArgs a, const Streams s, const int rows,
-                                                         const int per, const int prefix, const int budget,
-                                                         const int min_chunk, const int direct, float* ws) {
-  using C = ManyCfg<D>;
-  __shared__ __attribute__((aligned(256))) unsigned char smem[C::kSmem];
+template <int D, int W>
+__device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& pt, const int block,
+                                          unsigned char* smem) {
+  using C = ManyCfg<D, W>;
+  const Streams& s = pt.s;
+  const int rows = pt.rows;
+  constexpr int kDB = C::kDB, kDS = C::kDS, kPV = C::kPV, kSlots = C::kSlots, kAhead = C::kAhead;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hf = lane >> 5, col = lane & 31;
-  const int kvh = blockIdx.y, Hk = s.c.Hk;
-  const int n_rt = (rows + kManyRows - 1) / kManyRows;
-  const int item = blockIdx.x / n_rt;
-  // (a prompt's last row tiles see the most keys: they start first)
-  const int rt = n_rt - 1 - (int)(blockIdx.x - item * n_rt);
+  const int Hk = s.c.Hk;
+  const int n_rt = (rows + C::kRows - 1) / C::kRows;
+  // Order: a prompt's last row tiles, which see the most keys, first; kv heads
+  // side by side, so that with 8 of them each XCD keeps one head's keys in its L2.
+  // Where all workgroups find a place at once (two per CU), the second half runs
+  // the other way, so that a long one shares its CU with a short one.
+  const int kvh = block % Hk;
+  int place = block / Hk;
+  if (pt.one_round) {
+    const int all_places = pt.items * n_rt, half = all_places / 2;
+    if (place >= half) place = half + all_places - 1 - place;
+  }
+  const int rt = n_rt - 1 - place / pt.items, item = place % pt.items;
   Cut cut;
-  const int stream = __builtin_amdgcn_readfirstlane(stream_of<kManyTile>(s, budget, min_chunk, item, cut));
-  if (stream < 0) return;
+  const int stream = __builtin_amdgcn_readfirstlane(stream_of<kManyTile>(s, pt.budget, pt.min_chunk, item, cut));
+  if (stream < 0) return;  // (the whole workgroup)
   const int len = __builtin_amdgcn_readfirstlane(keys_of(s, stream));
-  const RowMap map{a, stream, kvh, a.H / Hk, per};
-  const int r = rt * kManyRows + wave * 32 + col;
-  int rb, ri, rh;
-  map.place(min(r, rows - 1), rb, ri, rh);
-  bf16x8 q[D / 16];
+  const RowMap map{a, stream, kvh, a.H / Hk, pt.per};
+  bf16x8 q[kDS];
+  int bound;  // keys that this lane's row sees
   {
+    int rb, ri, rh;
+    map.place(min(rt * C::kRows + wave * 32 + col, rows - 1), rb, ri, rh);
+    bound = pt.prefix ? len : own_bound(a, rb, ri, len);
     const bf16* p = (const bf16*)a.q + rb * a.qs[0] + ri * a.qs[1] + rh * a.qs[2] + hf * 8;
 #pragma unroll
-    for (int ds = 0; ds < D / 16; ++ds) q[ds] = *(const bf16x8*)(p + ds * 16);
+    for (int ds = 0; ds < kDS; ++ds) q[ds] = *(const bf16x8*)(p + ds * 16);
   }
-  const int bound = prefix ? len : own_bound(a, rb, ri, len);
-  int all = bound, any = bound;  // keys that every row of the wave sees, and that any does
+  int all = bound;  // keys that every row of the wave sees
 #pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) {
-    all = min(all, __shfl_xor(all, off, 64));
-    any = max(any, __shfl_xor(any, off, 64));
-  }
+  for (int off = 16; off >= 1; off >>= 1) all = min(all, __shfl_xor(all, off, 64));
   all = __builtin_amdgcn_readfirstlane(all);
-  any = __builtin_amdgcn_readfirstlane(any);
   // keys that any row of the workgroup sees
   int end = len;
-  if (!prefix) {
+  if (!pt.prefix) {
     const int m = clamp_len(a.q_len, stream, a.Sq);
-    const int i0 = rt * kManyRows / map.G, i1 = min(rt * kManyRows + kManyRows - 1, rows - 1) / map.G;
+    const int i0 = rt * C::kRows / map.G, i1 = min(rt * C::kRows + C::kRows - 1, rows - 1) / map.G;
     end = i0 < m ? own_bound(a, stream, min(i1, m - 1), len) : 0;
     end = __builtin_amdgcn_readfirstlane(end);
   }
   const int tiles = (end + kManyTile - 1) / kManyTile;
   const int chunk = __builtin_amdgcn_readfirstlane(cut.chunk);
   const int chunk_no = item - __builtin_amdgcn_readfirstlane(cut.first);
-  const int t0 = min((int64_t)chunk_no * chunk, (int64_t)tiles);
-  const int t1 = min((int64_t)t0 + chunk, (int64_t)tiles);
+  // (64-bit minima are vector instructions: back to scalar registers)
+  const int t0 = __builtin_amdgcn_readfirstlane((int)min((int64_t)chunk_no * chunk, (int64_t)tiles));
+  const int n = __builtin_amdgcn_readfirstlane((int)min((int64_t)chunk, (int64_t)tiles - t0));
 
-  f32x16 O[D / 32];
+  f32x16 O[kDB];
 #pragma unroll
-  for (int db = 0; db < D / 32; ++db) O[db] = f32x16{};
+  for (int db = 0; db < kDB; ++db) O[db] = f32x16{};
   float m_run = kNegBig, l_run = 0.f;
   const float c = a.scale * kLog2e;
 
   // ---- staging: a thread takes 16-byte chunks (16 values of one key) of K and
-  // of V to registers, and converts them with the key's scale on the way to LDS:
-  // once per workgroup, not once per wave.
+  // of V to registers, an iteration ahead, and converts them with the key's scale
+  // on the way to LDS: once per workgroup, not once per wave. 8 lanes take four
+  // chunks of keys k and k + 8, whose even (then odd) 16-byte halves the swizzle
+  // sends to eight different bank groups of a cycle's 128 bytes.
   const int64_t row0 = ((int64_t)slot_of(s, stream) * Hk + kvh) * s.c.cap;
-  const uint8_t* const kg = s.c.k + row0 * D;
-  const uint8_t* const vg = s.c.v + row0 * D;
-  constexpr int kPerRow = D / 16, kRowsPerPass = kThreads / kPerRow;
-  const int srow = threadIdx.x / kPerRow, sch = threadIdx.x % kPerRow;
-  u32x4 rk[C::kLoads], rv[C::kLoads];
-  uint32_t sk[C::kLoads], sv[C::kLoads];
-  auto load = [&](int t) {
+  // (uniform bases and 32-bit offsets per lane)
+  const uint64_t kg = uniform_u64((uint64_t)(uintptr_t)(s.c.k + row0 * D));
+  const uint64_t vg = uniform_u64((uint64_t)(uintptr_t)(s.c.v + row0 * D));
+  const uint64_t ksg = uniform_u64((uint64_t)(uintptr_t)(s.c.ks + row0));
+  const uint64_t vsg = uniform_u64((uint64_t)(uintptr_t)(s.c.vs + row0));
+  constexpr int kPlanes = D / 64;
+  const int tid = threadIdx.x;
+  // thread bits: chunk (2), key bits 3, 0, 1 and 2, plane, the key's other bits
+  const int plane = kPlanes == 2 ? (tid >> 6) & 1 : 0;
+  const int skey = ((tid >> 3) & 1) | (((tid >> 4) & 3) << 1) | (((tid >> 2) & 1) << 3) |
+                   ((tid >> (kPlanes == 2 ? 7 : 6)) << 4);
+  const int ssrc = plane * 64 + (tid & 3) * 16;                          // byte of the row
+  const int sdst = plane * C::kHalf + skey * 128;
+  const int sat = ((2 * (tid & 3)) ^ half_swizzle(skey)) * 16;           // its first half (the second: ^ 16)
+  constexpr int kKeysPerPass = kManyTile / C::kLoads;
+  struct Raw {
+    u32x4 x[C::kLoads];
+    uint32_t ks[C::kLoads], vs[C::kLoads];
+  };
+  auto load = [&](uint64_t base, int u, Raw& w) {
+    const uint64_t key0 = (uint64_t)(t0 + u) * kManyTile;
+    global_u8* const rows_at = (global_u8*)(uintptr_t)(base + key0 * D);
+    global_u8* const ks_at = (global_u8*)(uintptr_t)(ksg + key0);
+    global_u8* const vs_at = (global_u8*)(uintptr_t)(vsg + key0);
+    const uint32_t last = (uint32_t)(end - 1 - (t0 + u) * kManyTile);
 #pragma unroll
     for (int p = 0; p < C::kLoads; ++p) {
-      const int64_t key = min(t * (int64_t)kManyTile + p * kRowsPerPass + srow, (int64_t)end - 1);
-      rk[p] = *(const u32x4*)(kg + key * D + sch * 16);
-      rv[p] = *(const u32x4*)(vg + key * D + sch * 16);
-      sk[p] = s.c.ks[row0 + key];
-      sv[p] = s.c.vs[row0 + key];
+      const uint32_t key = min((uint32_t)(p * kKeysPerPass + skey), last);  // (past the last key: it again)
+      w.x[p] = *(VX_GLOBAL const u32x4*)(rows_at + (key * D + ssrc));
+      w.ks[p] = ks_at[key];
+      w.vs[p] = vs_at[key];
     }
   };
-  // Tile layout in LDS: K, then V; D / 64 half planes of 64 keys x 128 bytes, a
-  // row's 16-byte chunks XOR half_swizzle. Lanes with chunks of the second
-  // plane write their two halves in the other order: no two of a cycle's 16 lanes
-  // meet in a bank.
-  auto store = [&](int buf) {
-    lds_u8* const kb = (lds_u8*)smem + buf * C::kBuf;
+  auto store = [&](const Raw& w, bool is_k, int buf) {
+    lds_u8* const tile = (lds_u8*)smem + buf;
 #pragma unroll
     for (int p = 0; p < C::kLoads; ++p) {
-      const int key = p * kRowsPerPass + srow;
-      const float kf = __uint_as_float(max(sk[p], sv[p]) == 255u ? 0x7fc00000u : sk[p] << 23);
-      const float vf = __uint_as_float(min(sv[p], 254u) << 23);  // (such a row's bytes are zeros)
-      lds_u8* const row = kb + (sch >> 2) * C::kHalf + key * 128;
-      const int flip = (sch >> 2) & 1;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int h = x ^ flip;
-        const u32x2 k2 = h ? u32x2{rk[p][2], rk[p][3]} : u32x2{rk[p][0], rk[p][1]};
-        const u32x2 v2 = h ? u32x2{rv[p][2], rv[p][3]} : u32x2{rv[p][0], rv[p][1]};
-        const int at = ((2 * (sch & 3) + h) ^ half_swizzle(key)) * 16;
-        *(VX_LDS bf16x8*)(row + at) = e4m3x8_bf16(k2, kf);
-        *(VX_LDS bf16x8*)(row + C::kTileBytes + at) = e4m3x8_bf16(v2, vf);
-      }
+      // (a row whose key or value has scale NaN: a NaN key; its value bytes are zeros)
+      const float f = is_k ? __uint_as_float(max(w.ks[p], w.vs[p]) == 255u ? 0x7fc00000u : w.ks[p] << 23)
+                           : __uint_as_float(min(w.vs[p], 254u) << 23);
+      lds_u8* const row = tile + p * kKeysPerPass * 128 + sdst;
+      *(VX_LDS bf16x8*)(row + sat) = e4m3x8_bf16(u32x2{w.x[p][0], w.x[p][1]}, f);
+      *(VX_LDS bf16x8*)(row + (sat ^ 16)) = e4m3x8_bf16(u32x2{w.x[p][2], w.x[p][3]}, f);
     }
   };
+  static_assert(kKeysPerPass % 16 == 0, "a pass's keys keep their swizzle");
 
-  // ---- per-lane LDS offsets of the fragments (see flash_fwd.hip: the same
-  // tile layout)
+  // ---- per-lane LDS offsets of the fragments
   const int ksw = half_swizzle(col);
   int koff[4];
 #pragma unroll
@@ -541,95 +579,195 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const CachedAttnArgs 
     const int key = hf * 4 + vr;
     voff[db1] = key * 128 + (((4 * db1 + 2 * dh + (vc >> 1)) ^ half_swizzle(key)) * 16) + (vc & 1) * 8;
   }
+  auto frag_k = [&](const lds_u8* kb, int ds, int k2) -> bf16x8 {
+    return *(const VX_LDS bf16x8*)(kb + koff[ds & 3] + k2 * 32 * 128 + (ds >> 2) * C::kHalf);
+  };
+  auto frag_v = [&](const lds_u8* vb, int k2, int j, int db) -> bf16x8 {
+    const lds_u8* p = vb + (k2 * 32 + 16 * j) * 128 + (db >> 1) * C::kHalf;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((VX_LDS s16x4*)(p + voff[db & 1]));
+    const s16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((VX_LDS s16x4*)(p + 8 * 128 + (voff[db & 1] ^ 16)));
+    return concat(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi4));
+  };
 
-  auto step = [&](int t, int buf) {
-    const lds_u8* kb = (const lds_u8*)smem + buf * C::kBuf;
-    const lds_u8* vb = kb + C::kTileBytes;
+  if (n > 0) {
+    // Tile u's keys in K buffer u % 2, its values in V buffer u % 2. Iteration u
+    // issues the MFMAs of PV(u - 1) and of QK^T(u + 1) in one block and the
+    // softmax of tile u as a VALU block, writes K(u + 2) and V(u) (loaded in the
+    // last iteration) to the buffers that iteration u - 1 read, and loads the
+    // next two tiles. "V(-1)" is zeros, its weights are zeros.
+    Raw wk, wv;
+    Raw w0;
+    load(kg, 0, w0);
+    load(kg, min(1, n - 1), wk);
+    load(vg, 0, wv);
+    const int kZero = W * 64 * 16;
+#pragma unroll
+    for (int p = 0; p < C::kTileBytes / (W * 64 * 16); ++p)
+      *(VX_LDS u32x4*)((lds_u8*)smem + C::kVBuf + C::kTileBytes + p * kZero + tid * 16) = u32x4{0, 0, 0, 0};
+    store(w0, true, C::kKBuf);
+    store(wk, true, C::kKBuf + C::kTileBytes);
+    load(kg, min(2, n - 1), wk);
+    __syncthreads();
     f32x16 S[2] = {f32x16{}, f32x16{}};
 #pragma unroll
-    for (int ds = 0; ds < D / 16; ++ds)
+    for (int ds = 0; ds < kDS; ++ds)
 #pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2) {
-        const bf16x8 kf = *(const VX_LDS bf16x8*)(kb + koff[ds & 3] + k2 * 32 * 128 + (ds >> 2) * C::kHalf);
-        S[k2] = mfma32x32x16(kf, q[ds], S[k2]);
+      for (int k2 = 0; k2 < 2; ++k2) S[k2] = mfma32x32x16(frag_k((lds_u8*)smem + C::kKBuf, ds, k2), q[ds], S[k2]);
+    bf16x8 Pp[2][2];
+#pragma unroll
+    for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) Pp[k2][j] = bf16x8{};
+
+    auto iteration = [&](auto late_tag, auto odd_tag, const int u, f32x16 (&S)[2], f32x16 (&Sn)[2], const bf16x8 (&Pp)[2][2],
+                         bf16x8 (&P)[2][2]) __attribute__((always_inline)) {
+      constexpr bool LATE = decltype(late_tag)::value;
+      constexpr int kOdd = decltype(odd_tag)::value;  // u % 2
+      __syncthreads();
+      store(wk, true, C::kKBuf + kOdd * C::kTileBytes);
+      store(wv, false, C::kVBuf + kOdd * C::kTileBytes);
+      load(kg, min(u + 3, n - 1), wk);
+      load(vg, min(u + 1, n - 1), wv);
+      // scores of a tile with a key that some row does not see: to log2 units
+      // here, the unseen ones to -inf
+      const int key0 = (t0 + u) * kManyTile;
+      float cc = c;
+      if (key0 + kManyTile > all) {
+        cc = 1.0f;
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            S[k2][i] = key0 + k2 * 32 + (i >> 2) * 8 + hf * 4 + (i & 3) < bound ? S[k2][i] * c : -__builtin_inff();
       }
-    // a lane's score i of block k2: key k2 32 + (i / 4) 8 + hf 4 + i % 4
-    const int key0 = t * kManyTile;
-    float cc = c;
-    if (key0 + kManyTile > all) {
-      cc = 1.0f;
+      const lds_u8* kb = (const lds_u8*)smem + C::kKBuf + (1 - kOdd) * C::kTileBytes;
+      const lds_u8* vb = (const lds_u8*)smem + C::kVBuf + (1 - kOdd) * C::kTileBytes;
+      auto frag = [&](int x) -> bf16x8 {
+        if (x < kPV) return frag_v(vb, x / (2 * kDB), (x / kDB) & 1, x % kDB);
+        return frag_k(kb, (x - kPV) >> 1, (x - kPV) & 1);
+      };
+      // weights against the reference point, which moves up when a tile's maximum
+      // is 2^kSlack above it; their sum is that of the rounded weights, so that the
+      // ones that multiply V sum to one
+      const bf16x2 one2 = {(bf16)1.0f, (bf16)1.0f};
+      bf16x2 pk[16];
+      // (O takes alpha after PV(u - 1), whose weights are against the old point)
+      bool moved = false;
+      float alpha = 1.0f;
+      auto weights = [&]() {
+        float mx = fmaxf(S[0][0], S[1][0]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(fmaxf(mx, S[0][i]), S[1][i]);
+        mx = halves_max(mx) * cc;
+        if (__builtin_amdgcn_ballot_w64(mx > m_run + kSlack) != 0) {
+          const float mn = fmaxf(m_run, mx);
+          alpha = fast_exp2(m_run - mn);
+          m_run = mn;
+          l_run *= alpha;
+          moved = true;
+        }
+        const float mneg = -m_run;
+        float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float pf[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pf[i] = fast_exp2(__builtin_fmaf(S[g >> 1][8 * (g & 1) + i], cc, mneg));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            pk[4 * g + i] = bf16x2{(bf16)pf[2 * i], (bf16)pf[2 * i + 1]};
+            l4[i] = __builtin_amdgcn_fdot2_f32_bf16(pk[4 * g + i], one2, l4[i], false);
+          }
+        }
+        l_run += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        // (here, not where the next iteration uses them)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(pk[i]));
+      };
+      bf16x8 fr[kSlots];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) fr[x] = frag(x);
+      if (!LATE) weights();
+      __builtin_amdgcn_sched_barrier(0);
+      Sn[0] = f32x16{};
+      Sn[1] = f32x16{};
+#pragma unroll
+      for (int x = 0; x < kSlots; ++x) {
+        if (x + kAhead < kSlots) fr[x + kAhead] = frag(x + kAhead);
+        if (x < kPV) {
+          O[x % kDB] = mfma32x32x16(fr[x], Pp[x / (2 * kDB)][(x / kDB) & 1], O[x % kDB]);
+        } else {
+          const int ds = (x - kPV) >> 1, k2 = (x - kPV) & 1;
+          Sn[k2] = mfma32x32x16(fr[x], q[ds], Sn[k2]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (LATE) weights();
+      if (moved) {
+#pragma unroll
+        for (int db = 0; db < kDB; ++db) O[db] *= alpha;
+      }
 #pragma unroll
       for (int k2 = 0; k2 < 2; ++k2)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          S[k2][i] = key0 + k2 * 32 + (i >> 2) * 8 + hf * 4 + (i & 3) < bound ? S[k2][i] * c : -__builtin_inff();
-    }
-    float mx = fmaxf(S[0][0], S[1][0]);
-#pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(fmaxf(mx, S[0][i]), S[1][i]);
-    mx = halves_max(mx) * cc;
-    if (__builtin_amdgcn_ballot_w64(mx > m_run + kSlack) != 0) {
-      const float mn = fmaxf(m_run, mx), alpha = fast_exp2(m_run - mn);
-      m_run = mn;
-      l_run *= alpha;
-#pragma unroll
-      for (int db = 0; db < D / 32; ++db) O[db] *= alpha;
-    }
-    const float mneg = -m_run;
-    bf16x8 P[2][2];
-#pragma unroll
-    for (int k2 = 0; k2 < 2; ++k2)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p = fast_exp2(__builtin_fmaf(S[k2][8 * j + e], cc, mneg));
-          l_run += p;
-          P[k2][j][e] = (bf16)p;
+        for (int j = 0; j < 2; ++j) {
+          const int x = k2 * 8 + j * 4;
+          P[k2][j] = __builtin_shufflevector(__builtin_shufflevector(pk[x], pk[x + 1], 0, 1, 2, 3),
+                                             __builtin_shufflevector(pk[x + 2], pk[x + 3], 0, 1, 2, 3), 0, 1, 2, 3, 4,
+                                             5, 6, 7);
         }
-#pragma unroll
-    for (int k2 = 0; k2 < 2; ++k2)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int db = 0; db < D / 32; ++db) {
-          const lds_u8* p = vb + (k2 * 32 + 16 * j) * 128 + (db >> 1) * C::kHalf;
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((VX_LDS s16x4*)(p + voff[db & 1]));
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((VX_LDS s16x4*)(p + 8 * 128 + (voff[db & 1] ^ 16)));
-          const bf16x8 vf = concat(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi));
-          O[db] = mfma32x32x16(vf, P[k2][j], O[db]);
-        }
-  };
-
-  if (t0 < t1) {
-    load(t0);
-    store(0);
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-      const int buf = (t - t0) & 1;
-      if (t + 1 < t1) load(t + 1);
-      if (t * kManyTile < any) step(t, buf);
-      if (t + 1 < t1) store(buf ^ 1);
+    };
+    f32x16 S2[2];
+    bf16x8 P2[2][2];
+    using Even = std::integral_constant<int, 0>;
+    using Odd = std::integral_constant<int, 1>;
+    auto last_pv = [&](auto odd_tag, const bf16x8 (&P)[2][2]) __attribute__((always_inline)) {
       __syncthreads();
-    }
+      const lds_u8* vb = (const lds_u8*)smem + C::kVBuf + decltype(odd_tag)::value * C::kTileBytes;
+#pragma unroll
+      for (int x = 0; x < kPV; ++x)
+        O[x % kDB] =
+            mfma32x32x16(frag_v(vb, x / (2 * kDB), (x / kDB) & 1, x % kDB), P[x / (2 * kDB)][(x / kDB) & 1], O[x % kDB]);
+    };
+    auto key_loop = [&](auto late_tag) __attribute__((always_inline)) {
+      int u = 0;
+      for (; u + 1 < n; u += 2) {
+        iteration(late_tag, Even{}, u, S, S2, Pp, P2);
+        iteration(late_tag, Odd{}, u + 1, S2, S, P2, Pp);
+      }
+      // the last tile's PV
+      if (u < n) {
+        iteration(late_tag, Even{}, u, S, S2, Pp, P2);
+        last_pv(Even{}, P2);
+      } else {
+        last_pv(Odd{}, Pp);
+      }
+    };
+    if (W == 4 || wave < 4)
+      key_loop(std::integral_constant<bool, false>{});
+    else
+      key_loop(std::integral_constant<bool, true>{});
   }
 
   const float L = halves_sum(l_run);
-  if (direct && cut.count == 1) {
+  const int r = rt * C::kRows + wave * 32 + col;
+  if (pt.direct && cut.count == 1) {
+    int rb, ri, rh;
+    map.place(min(r, rows - 1), rb, ri, rh);
     const float inv = is_zero(L) ? 0.f : 1.0f / L;
-    u32x4 chunk[D / 32][2];
-    pack_out_rows<D / 32>(O, inv, chunk);
+    u32x4 out[kDB][2];
+    pack_out_rows<kDB>(O, inv, out);
     if (r < rows) {
       bf16* const o = (bf16*)a.o + rb * a.os[0] + ri * a.os[1] + rh * a.os[2];
 #pragma unroll
-      for (int db = 0; db < D / 32; ++db)
+      for (int db = 0; db < kDB; ++db)
 #pragma unroll
-        for (int pr = 0; pr < 2; ++pr) *(u32x4*)(o + db * 32 + 8 * (2 * pr + hf)) = chunk[db][pr];
+        for (int pr = 0; pr < 2; ++pr) *(u32x4*)(o + db * 32 + 8 * (2 * pr + hf)) = out[db][pr];
     }
   } else if (r < rows) {
-    float* const part = ws + ((int64_t)item * Hk + kvh) * part_floats(rows, D);
+    float* const part = pt.ws + ((int64_t)item * Hk + kvh) * part_floats(rows, D);
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db)
+    for (int db = 0; db < kDB; ++db)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *(f32x4*)(part + (int64_t)r * D + db * 32 + 8 * g + 4 * hf) =
@@ -641,51 +779,101 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const CachedAttnArgs 
   }
 }
 
-// ------------------------------------------------------------------ merge
-// Output rows of item blockIdx.y: D / 4 lanes per row over the parts of the
-// item's own chunks and of its group's prefix chunks, in order.
-struct Parts {
-  Streams s;
-  int32_t budget, min_chunk, few;
-  int32_t rows;  // per stream and kv head
-  float* ws;
-};
+template <int D>
+__global__ __launch_bounds__(kThreads, 2) void few_kernel(const CachedAttnArgs a, const Part own) {
+  __shared__ __attribute__((aligned(256))) unsigned char smem[FewCfg<D>::kSmem];
+  few_part<D>(a, own, blockIdx.x, smem);
+}
 
 template <int D>
-__global__ __launch_bounds__(kThreads) void merge_kernel(const CachedAttnArgs a, const Parts own, const Parts pre) {
+__global__ __launch_bounds__(kThreads, 2) void many_kernel(const CachedAttnArgs a, const Part own) {
+  __shared__ __attribute__((aligned(256))) unsigned char smem[ManyCfg<D, kWaves>::kSmem];
+  many_part<D, kWaves>(a, own, blockIdx.x, smem);
+}
+
+// A prefix's chunks (the first pre_blocks workgroups) and the items' own, side by
+// side: the prefix alone would leave most of the chip idle, and so would they.
+template <int D, bool PRE_FEW, bool OWN_FEW>
+__global__ __launch_bounds__(kThreads, 2) void prefix_kernel(const CachedAttnArgs a, const Part pre, const Part own,
+                                                           const int pre_blocks) {
+  constexpr int kFew = FewCfg<D>::kSmem, kMany = ManyCfg<D, kWaves>::kSmem;
+  constexpr int kPre = PRE_FEW ? kFew : kMany, kOwn = OWN_FEW ? kFew : kMany;
+  __shared__ __attribute__((aligned(256))) unsigned char smem[kPre > kOwn ? kPre : kOwn];
+  const int block = blockIdx.x;
+  if (block < pre_blocks) {
+    if constexpr (PRE_FEW)
+      few_part<D>(a, pre, block, smem);
+    else
+      many_part<D, kWaves>(a, pre, block, smem);
+  } else {
+    if constexpr (OWN_FEW)
+      few_part<D>(a, own, block - pre_blocks, smem);
+    else
+      many_part<D, kWaves>(a, own, block - pre_blocks, smem);
+  }
+}
+
+// ------------------------------------------------------------------ merge
+// Output rows of item blockIdx.y from the parts of the item's own chunks and of
+// its group's prefix chunks. D / 4 lanes take a row; `split` such groups share
+// the parts of a row, and join in LDS, in a fixed order.
+template <int D>
+__global__ __launch_bounds__(kThreads) void merge_kernel(const CachedAttnArgs a, const Part own, const Part pre,
+                                                       const int split) {
+  constexpr int kLanes = D / 4, kGroups = kThreads / kLanes;
+  __shared__ f32x4 xo[kGroups][kLanes];
+  __shared__ float xml[kGroups][2];
   const int b = blockIdx.y, Hk = a.c.Hk, G = a.H / Hk;
   const Cut oc = own.few ? cut_of<kFewTile>(own.s, own.budget, own.min_chunk, b)
                          : cut_of<kManyTile>(own.s, own.budget, own.min_chunk, b);
   const bool with_prefix = pre.s.n > 0;
   if (!with_prefix && oc.count == 1) return;  // (written by its only chunk)
   Cut pc{0, 0, 0};
-  const int per = with_prefix ? a.B / pre.s.n : 1;
   if (with_prefix)
-    pc = pre.few ? cut_of<kFewTile>(pre.s, pre.budget, pre.min_chunk, b / per)
-                 : cut_of<kManyTile>(pre.s, pre.budget, pre.min_chunk, b / per);
-  const int64_t x = (int64_t)blockIdx.x * (kThreads / (D / 4)) + threadIdx.x / (D / 4);
-  if (x >= (int64_t)Hk * own.rows) return;
-  const int d = (threadIdx.x % (D / 4)) * 4;
-  const int kvh = (int)(x / own.rows), r = (int)(x - (int64_t)kvh * own.rows);
-  const int i = r / G, h = kvh * G + r % G;
+    pc = pre.few ? cut_of<kFewTile>(pre.s, pre.budget, pre.min_chunk, b / pre.per)
+                 : cut_of<kManyTile>(pre.s, pre.budget, pre.min_chunk, b / pre.per);
+  const int group = threadIdx.x / kLanes, d = (threadIdx.x % kLanes) * 4;
+  const int part0 = group % split;
+  const int64_t x = (int64_t)blockIdx.x * (kGroups / split) + group / split;
+  const bool real = x < (int64_t)Hk * own.rows;
+  const int kvh = real ? (int)(x / own.rows) : 0, r = real ? (int)(x - (int64_t)kvh * own.rows) : 0;
   float M = kNegBig, L = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  auto add = [&](const Parts& p, const Cut& cut, int row) {
-    const int64_t block = part_floats(p.rows, D);
-    const float* base = p.ws + ((int64_t)cut.first * Hk + kvh) * block;
+  const int total = real ? pc.count + oc.count : 0;
+  const int64_t pre_block = part_floats(pre.rows, D), own_block = part_floats(own.rows, D);
+  const int pre_row = with_prefix ? (b % pre.per) * own.rows + r : 0;
 #pragma unroll 4
-    for (int n = 0; n < cut.count; ++n) {
-      const float* part = base + (int64_t)n * Hk * block;
-      const f32x4 po = *(const f32x4*)(part + (int64_t)row * D + d);
-      const float pm = part[(int64_t)p.rows * D + 2 * row], pl = part[(int64_t)p.rows * D + 2 * row + 1];
+  for (int n = part0; n < total; n += split) {
+    const bool p = n < pc.count;
+    const int64_t block = p ? pre_block : own_block, rows = p ? pre.rows : own.rows;
+    const int64_t at = (int64_t)(p ? pc.first + n : oc.first + n - pc.count) * Hk + kvh;
+    const float* part = (p ? pre.ws : own.ws) + at * block;
+    const int row = p ? pre_row : r;
+    const f32x4 po = *(const f32x4*)(part + (int64_t)row * D + d);
+    const float pm = part[rows * D + 2 * row], pl = part[rows * D + 2 * row + 1];
+    const float mn = fmaxf(M, pm), a0 = fast_exp2(M - mn), a1 = fast_exp2(pm - mn);
+    o = o * a0 + po * a1;
+    L = L * a0 + pl * a1;
+    M = mn;
+  }
+  if (split > 1) {
+    xo[group][threadIdx.x % kLanes] = o;
+    if (d == 0) {
+      xml[group][0] = M;
+      xml[group][1] = L;
+    }
+    __syncthreads();
+    if (part0 != 0) return;
+    for (int g = 1; g < split; ++g) {
+      const float pm = xml[group + g][0], pl = xml[group + g][1];
       const float mn = fmaxf(M, pm), a0 = fast_exp2(M - mn), a1 = fast_exp2(pm - mn);
-      o = o * a0 + po * a1;
+      o = o * a0 + xo[group + g][threadIdx.x % kLanes] * a1;
       L = L * a0 + pl * a1;
       M = mn;
     }
-  };
-  if (with_prefix) add(pre, pc, (b % per) * own.rows + r);
-  add(own, oc, r);
+  }
+  if (!real) return;
+  const int i = r / G, h = kvh * G + r % G;
   const bool none = is_zero(L) || i >= clamp_len(a.q_len, b, a.Sq);
   const float inv = 1.0f / L;
   bf16x4 y;
@@ -695,81 +883,101 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const CachedAttnArgs a,
 }
 
 // ------------------------------------------------------------------ launch plan
-struct Half {
-  int streams = 0, rows = 0, per = 1;
-  bool few = false;
-  int budget = 0, min_chunk = 1;
-  int64_t items = 0;  // workgroups per kv head and row tile
+constexpr int kManyRows = 32 * kWaves;
+
+// Fills a part's plan; returns its workgroups.
+struct Planned {
+  Part p{};
+  int64_t blocks = 0;
   int64_t floats = 0;  // of partial results
+  int most_parts = 1;  // of a stream
 };
 
-Half plan_half(int streams, int64_t rows, int per, int cap, int Hk, int D, int cus, bool parts) {
-  Half h;
-  h.streams = streams;
-  h.rows = (int)rows;
-  h.per = per;
-  h.few = rows <= 32;
-  const int64_t slots = 2 * (int64_t)cus;
-  const int64_t row_tiles = h.few ? 1 : (rows + kManyRows - 1) / kManyRows;
-  const int64_t groups = streams * row_tiles * Hk;
-  const int64_t tiles = (cap + (h.few ? kFewTile : kManyTile) - 1) / (h.few ? kFewTile : kManyTile);
-  h.min_chunk = 4;
-  if (tiles > h.min_chunk && (h.few || groups < slots))
-    h.budget = (int)std::min<int64_t>((slots * (h.few ? 2 : 1) + Hk * row_tiles - 1) / (Hk * row_tiles),
-                                      streams * ((tiles + h.min_chunk - 1) / h.min_chunk));
-  h.items = h.budget + (int64_t)streams;
-  if (h.budget == 0) h.items = streams;
-  if (parts || h.budget > 0) h.floats = h.items * Hk * ((rows * (D + 2) + 3) & ~(int64_t)3);
+Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, int D, int64_t slots, bool prefix,
+                  bool with_prefix) {
+  Planned h;
+  Part& p = h.p;
+  p.rows = (int)rows;
+  p.per = per;
+  p.few = rows <= 32;
+  p.prefix = prefix;
+  p.direct = !with_prefix;
+  const int64_t row_tiles = p.few ? 1 : (rows + kManyRows - 1) / kManyRows;
+  const int64_t tile = p.few ? kFewTile : kManyTile;
+  const int64_t tiles = (cap + tile - 1) / tile;
+  const int64_t per_head = std::max<int64_t>(slots / (Hk * row_tiles), 1);
+  p.min_chunk = 4;
+  if (tiles > p.min_chunk && (p.few || streams * row_tiles * Hk < slots)) {
+    // As many items as find a place at once, where that leaves two and more per
+    // stream; else several rounds of them.
+    int64_t budget = per_head >= 2 * streams ? per_head - streams : std::max(3 * per_head, (int64_t)2 * streams);
+    p.budget = (int)std::min(budget, streams * ((tiles + p.min_chunk - 1) / p.min_chunk));
+  }
+  p.items = p.budget + streams;
+  if (p.budget == 0) p.items = streams;
+  h.most_parts = (int)std::min<int64_t>(p.budget == 0 ? 1 : p.budget, (tiles + p.min_chunk - 1) / p.min_chunk);
+  h.blocks = p.items * row_tiles * Hk;
+  p.one_round = h.blocks <= slots;
+  if (with_prefix || p.budget > 0) h.floats = (int64_t)p.items * Hk * ((rows * (D + 2) + 3) & ~(int64_t)3);
   return h;
 }
 
 struct Plan {
-  Half own, pre;
+  Planned own, pre;
 };
 
 Plan plan_of(int cap, int n_prefix, int p_cap, int B, int Sq, int H, int Hk, int D) {
-  const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
+  // workgroups that the device holds at once (256 if it is not known)
+  const int64_t slots = 2 * (int64_t)(device_cu_count() > 0 ? device_cu_count() : 256);
   const int64_t rows = (int64_t)Sq * (H / Hk);
   Plan p;
-  p.own = plan_half(B, rows, 1, cap, Hk, D, cus, n_prefix > 0);
-  if (n_prefix > 0) p.pre = plan_half(n_prefix, rows * (B / n_prefix), B / n_prefix, p_cap, Hk, D, cus, true);
-  return p;
-}
-
-template <int D>
-int launch_half(const CachedAttnArgs& a, const Streams& s, const Half& h, bool prefix, float* ws, hipStream_t st) {
-  const int direct = !prefix && a.prefix.k == nullptr;
-  if (h.few) {
-    hipLaunchKernelGGL(few_kernel<D>, dim3((unsigned)h.items, s.c.Hk), dim3(kThreads), 0, st, a, s, h.rows, h.per,
-                       (int)prefix, h.budget, h.min_chunk, direct, ws);
-  } else {
-    const int64_t n = h.items * ((h.rows + (int64_t)kManyRows - 1) / kManyRows);
-    hipLaunchKernelGGL(many_kernel<D>, dim3((unsigned)n, s.c.Hk), dim3(kThreads), 0, st, a, s, h.rows, h.per,
-                       (int)prefix, h.budget, h.min_chunk, direct, ws);
+  p.own = plan_part(B, rows, 1, cap, Hk, D, slots, false, n_prefix > 0);
+  if (n_prefix > 0) {
+    const int per = B / n_prefix;
+    p.pre = plan_part(n_prefix, rows * per, per, p_cap, Hk, D, std::max(slots - p.own.blocks, slots / 2), true, true);
   }
-  return (int)hipGetLastError();
+  return p;
 }
 
 template <int D>
 int launch(const CachedAttnArgs& a, hipStream_t st, const char** launched) {
   const int n_prefix = a.prefix.k != nullptr ? a.prefix.slots : 0;
-  const Plan p = plan_of(a.c.cap, n_prefix, a.prefix.cap, a.B, a.Sq, a.H, a.c.Hk, D);
-  const Streams own{a.c, a.kv_len, a.slots, a.B};
-  const Streams pre{a.prefix, a.prefix_len, nullptr, n_prefix};
-  float* const ws_pre = a.ws + p.own.floats;
-  int err = 0;
-  if (n_prefix > 0 && (err = launch_half<D>(a, pre, p.pre, true, ws_pre, st)) != 0) return err;
-  if ((err = launch_half<D>(a, own, p.own, false, a.ws, st)) != 0) return err;
-  if (n_prefix > 0 || p.own.budget > 0) {
-    const Parts po{own, p.own.budget, p.own.min_chunk, p.own.few, p.own.rows, a.ws};
-    const Parts pp{pre, p.pre.budget, p.pre.min_chunk, p.pre.few, p.pre.rows, ws_pre};
-    const int64_t per_wg = kThreads / (D / 4);
-    hipLaunchKernelGGL(merge_kernel<D>, dim3((unsigned)(((int64_t)a.c.Hk * p.own.rows + per_wg - 1) / per_wg), a.B),
-                       dim3(kThreads), 0, st, a, po, pp);
+  Plan pl = plan_of(a.c.cap, n_prefix, a.prefix.cap, a.B, a.Sq, a.H, a.c.Hk, D);
+  Part& own = pl.own.p;
+  Part& pre = pl.pre.p;
+  own.s = Streams{a.c, a.kv_len, a.slots, a.B};
+  own.ws = a.ws;
+  pre.s = Streams{a.prefix, a.prefix_len, nullptr, n_prefix};
+  pre.ws = a.ws + pl.own.floats;
+  const dim3 grid((unsigned)(pl.pre.blocks + pl.own.blocks)), threads(kThreads);
+  const int pre_blocks = (int)pl.pre.blocks;
+  if (n_prefix == 0) {
+    if (own.few)
+      hipLaunchKernelGGL(few_kernel<D>, grid, threads, 0, st, a, own);
+    else
+      hipLaunchKernelGGL(many_kernel<D>, grid, threads, 0, st, a, own);
+    *launched = own.few ? (D == 128 ? "few_kernel<128>" : "few_kernel<64>")
+                        : (D == 128 ? "many_kernel<128>" : "many_kernel<64>");
+  } else if (pre.few) {  // (a prefix's streams have no fewer rows than the items')
+    hipLaunchKernelGGL((prefix_kernel<D, true, true>), grid, threads, 0, st, a, pre, own, pre_blocks);
+    *launched = D == 128 ? "prefix_kernel<128, true, true>" : "prefix_kernel<64, true, true>";
+  } else if (own.few) {
+    hipLaunchKernelGGL((prefix_kernel<D, false, true>), grid, threads, 0, st, a, pre, own, pre_blocks);
+    *launched = D == 128 ? "prefix_kernel<128, false, true>" : "prefix_kernel<64, false, true>";
+  } else {
+    hipLaunchKernelGGL((prefix_kernel<D, false, false>), grid, threads, 0, st, a, pre, own, pre_blocks);
+    *launched = D == 128 ? "prefix_kernel<128, false, false>" : "prefix_kernel<64, false, false>";
+  }
+  int err = (int)hipGetLastError();
+  if (err == 0 && (n_prefix > 0 || own.budget > 0)) {
+    constexpr int kGroups = kThreads / (D / 4);
+    int split = 1;  // about four parts in turn per group of lanes
+    while (split < kGroups && 4 * split < pl.own.most_parts + (n_prefix > 0 ? pl.pre.most_parts : 0)) split *= 2;
+    const int64_t per_wg = kGroups / split;
+    hipLaunchKernelGGL(merge_kernel<D>, dim3((unsigned)(((int64_t)a.c.Hk * own.rows + per_wg - 1) / per_wg), a.B),
+                       threads, 0, st, a, own, pre, split);
     err = (int)hipGetLastError();
   }
-  *launched = p.own.few ? (D == 128 ? "few_kernel<128>" : "few_kernel<64>")
-                        : (D == 128 ? "many_kernel<128>" : "many_kernel<64>");
   return err;
 }
 

@@ -730,7 +730,7 @@ int32_t cached_sizes_check(int32_t n_prefix, int32_t B, int32_t Sq, int32_t H, i
   if (n_prefix < 0 || (n_prefix > 0 && B % n_prefix != 0))
     return fail(VX_ERR_INVALID_ARGUMENT, "batch (%d) must be a multiple of num_prefixes (%d)", B, n_prefix);
   const int64_t rows = (int64_t)Sq * (H / Hk), sharers = n_prefix > 0 ? B / n_prefix : 1;
-  if (rows > kMaxSharedRows || sharers * rows > kMaxSharedRows || (rows + 127) / 128 * B > kMaxSharedRows ||
+  if (rows > kMaxSharedRows || sharers * rows > kMaxSharedRows || (rows + 127) / 128 * B > kMaxSharedRows / 4 / Hk ||
       (int64_t)H * Sq > 4 * kMaxSharedRows)
     return fail(VX_ERR_UNSUPPORTED, "%d queries of %d heads for %d items are too many", Sq, H, B);
   return VX_OK;
