@@ -539,31 +539,37 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
     u32x4 x[C::kLoads];
     uint32_t ks[C::kLoads], vs[C::kLoads];
   };
+  // (through a buffer resource that ends with the last key: what lies behind
+  // reads as zeros)
+  const uint32_t sofs = skey * D + ssrc;
   auto load = [&](uint64_t base, int u, Raw& w) {
-    const uint64_t key0 = (uint64_t)(t0 + u) * kManyTile;
-    global_u8* const rows_at = (global_u8*)(uintptr_t)(base + key0 * D);
-    global_u8* const ks_at = (global_u8*)(uintptr_t)(ksg + key0);
-    global_u8* const vs_at = (global_u8*)(uintptr_t)(vsg + key0);
-    const uint32_t last = (uint32_t)(end - 1 - (t0 + u) * kManyTile);
+    const int tile = t0 + u, keys = min(end - tile * kManyTile, kManyTile);
+    auto rsrc = [&](uint64_t p, int bytes) {
+      return __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)p, 0, bytes, 0x00020000);
+    };
+    const auto rows_r = rsrc(base + (uint64_t)tile * (kManyTile * D), keys * D);
+    const auto ks_r = rsrc(ksg + (uint64_t)tile * kManyTile, keys);
+    const auto vs_r = rsrc(vsg + (uint64_t)tile * kManyTile, keys);
 #pragma unroll
     for (int p = 0; p < C::kLoads; ++p) {
-      const uint32_t key = min((uint32_t)(p * kKeysPerPass + skey), last);  // (past the last key: it again)
-      w.x[p] = *(VX_GLOBAL const u32x4*)(rows_at + (key * D + ssrc));
-      w.ks[p] = ks_at[key];
-      w.vs[p] = vs_at[key];
+      w.x[p] = __builtin_amdgcn_raw_buffer_load_b128(rows_r, sofs, p * kKeysPerPass * D, 0);
+      w.ks[p] = __builtin_amdgcn_raw_buffer_load_b8(ks_r, skey, p * kKeysPerPass, 0);
+      w.vs[p] = __builtin_amdgcn_raw_buffer_load_b8(vs_r, skey, p * kKeysPerPass, 0);
     }
   };
-  auto store = [&](const Raw& w, bool is_k, int buf) {
-    lds_u8* const tile = (lds_u8*)smem + buf;
+  // piece j of 2 kLoads: half of a chunk to the tile at `buf`
+  auto store = [&](const Raw& w, bool is_k, int buf, int j) {
+    const int p = j / 2, half = j % 2;
+    // (a row whose key or value has scale NaN: a NaN key; its value bytes are zeros)
+    const float f = is_k ? __uint_as_float(max(w.ks[p], w.vs[p]) == 255u ? 0x7fc00000u : w.ks[p] << 23)
+                         : __uint_as_float(min(w.vs[p], 254u) << 23);
+    lds_u8* const row = (lds_u8*)smem + buf + p * kKeysPerPass * 128 + sdst;
+    *(VX_LDS bf16x8*)(row + (half ? sat ^ 16 : sat)) =
+        e4m3x8_bf16(u32x2{w.x[p][2 * half], w.x[p][2 * half + 1]}, f);
+  };
+  auto store_all = [&](const Raw& w, bool is_k, int buf) {
 #pragma unroll
-    for (int p = 0; p < C::kLoads; ++p) {
-      // (a row whose key or value has scale NaN: a NaN key; its value bytes are zeros)
-      const float f = is_k ? __uint_as_float(max(w.ks[p], w.vs[p]) == 255u ? 0x7fc00000u : w.ks[p] << 23)
-                           : __uint_as_float(min(w.vs[p], 254u) << 23);
-      lds_u8* const row = tile + p * kKeysPerPass * 128 + sdst;
-      *(VX_LDS bf16x8*)(row + sat) = e4m3x8_bf16(u32x2{w.x[p][0], w.x[p][1]}, f);
-      *(VX_LDS bf16x8*)(row + (sat ^ 16)) = e4m3x8_bf16(u32x2{w.x[p][2], w.x[p][3]}, f);
-    }
+    for (int j = 0; j < 2 * C::kLoads; ++j) store(w, is_k, buf, j);
   };
   static_assert(kKeysPerPass % 16 == 0, "a pass's keys keep their swizzle");
 
@@ -599,14 +605,14 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
     Raw w0;
     load(kg, 0, w0);
     load(kg, min(1, n - 1), wk);
-    load(vg, 0, wv);
     const int kZero = W * 64 * 16;
 #pragma unroll
     for (int p = 0; p < C::kTileBytes / (W * 64 * 16); ++p)
       *(VX_LDS u32x4*)((lds_u8*)smem + C::kVBuf + C::kTileBytes + p * kZero + tid * 16) = u32x4{0, 0, 0, 0};
-    store(w0, true, C::kKBuf);
-    store(wk, true, C::kKBuf + C::kTileBytes);
-    load(kg, min(2, n - 1), wk);
+    store_all(w0, true, C::kKBuf);
+    store_all(wk, true, C::kKBuf + C::kTileBytes);
+    load(kg, min(2, n - 1), wk);  // (in the loop's order)
+    load(vg, 0, wv);
     __syncthreads();
     f32x16 S[2] = {f32x16{}, f32x16{}};
 #pragma unroll
@@ -619,15 +625,9 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
 #pragma unroll
       for (int j = 0; j < 2; ++j) Pp[k2][j] = bf16x8{};
 
-    auto iteration = [&](auto late_tag, auto odd_tag, const int u, f32x16 (&S)[2], f32x16 (&Sn)[2], const bf16x8 (&Pp)[2][2],
+    auto iteration = [&](auto odd_tag, const int u, f32x16 (&S)[2], f32x16 (&Sn)[2], const bf16x8 (&Pp)[2][2],
                          bf16x8 (&P)[2][2]) __attribute__((always_inline)) {
-      constexpr bool LATE = decltype(late_tag)::value;
       constexpr int kOdd = decltype(odd_tag)::value;  // u % 2
-      __syncthreads();
-      store(wk, true, C::kKBuf + kOdd * C::kTileBytes);
-      store(wv, false, C::kVBuf + kOdd * C::kTileBytes);
-      load(kg, min(u + 3, n - 1), wk);
-      load(vg, min(u + 1, n - 1), wv);
       // scores of a tile with a key that some row does not see: to log2 units
       // here, the unseen ones to -inf
       const int key0 = (t0 + u) * kManyTile;
@@ -640,69 +640,73 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
           for (int i = 0; i < 16; ++i)
             S[k2][i] = key0 + k2 * 32 + (i >> 2) * 8 + hf * 4 + (i & 3) < bound ? S[k2][i] * c : -__builtin_inff();
       }
+      // The reference point of the weights moves up when a tile's maximum is
+      // 2^kSlack above it. (O takes alpha after PV(u - 1), whose weights are against
+      // the old point.)
+      float mx = fmaxf(S[0][0], S[1][0]);
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(fmaxf(mx, S[0][i]), S[1][i]);
+      mx = halves_max(mx) * cc;
+      float alpha = 1.0f;
+      const bool moved = __builtin_amdgcn_ballot_w64(mx > m_run + kSlack) != 0;
+      if (moved) {
+        const float mn = fmaxf(m_run, mx);
+        alpha = fast_exp2(m_run - mn);
+        m_run = mn;
+        l_run *= alpha;
+      }
+      __syncthreads();
       const lds_u8* kb = (const lds_u8*)smem + C::kKBuf + (1 - kOdd) * C::kTileBytes;
       const lds_u8* vb = (const lds_u8*)smem + C::kVBuf + (1 - kOdd) * C::kTileBytes;
       auto frag = [&](int x) -> bf16x8 {
         if (x < kPV) return frag_v(vb, x / (2 * kDB), (x / kDB) & 1, x % kDB);
         return frag_k(kb, (x - kPV) >> 1, (x - kPV) & 1);
       };
-      // weights against the reference point, which moves up when a tile's maximum
-      // is 2^kSlack above it; their sum is that of the rounded weights, so that the
-      // ones that multiply V sum to one
+      // One block of kSlots MFMAs, each with the fragment kAhead MFMAs on, and
+      // behind it what does not depend on it, in the cycles that the matrix core
+      // takes: behind PV's the tile's weights (two exponentials and four other
+      // instructions fill an MFMA's 32 cycles), behind QK^T's the conversion of the
+      // next tiles, then their successors' loads. l is the sum of the rounded
+      // weights, so that the ones that multiply V sum to one.
       const bf16x2 one2 = {(bf16)1.0f, (bf16)1.0f};
+      const float mneg = -m_run;
       bf16x2 pk[16];
-      // (O takes alpha after PV(u - 1), whose weights are against the old point)
-      bool moved = false;
-      float alpha = 1.0f;
-      auto weights = [&]() {
-        float mx = fmaxf(S[0][0], S[1][0]);
-#pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(fmaxf(mx, S[0][i]), S[1][i]);
-        mx = halves_max(mx) * cc;
-        if (__builtin_amdgcn_ballot_w64(mx > m_run + kSlack) != 0) {
-          const float mn = fmaxf(m_run, mx);
-          alpha = fast_exp2(m_run - mn);
-          m_run = mn;
-          l_run *= alpha;
-          moved = true;
-        }
-        const float mneg = -m_run;
-        float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float pf[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pf[i] = fast_exp2(__builtin_fmaf(S[g >> 1][8 * (g & 1) + i], cc, mneg));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            pk[4 * g + i] = bf16x2{(bf16)pf[2 * i], (bf16)pf[2 * i + 1]};
-            l4[i] = __builtin_amdgcn_fdot2_f32_bf16(pk[4 * g + i], one2, l4[i], false);
-          }
-        }
-        l_run += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-        // (here, not where the next iteration uses them)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(pk[i]));
+      float l2[2] = {0.f, 0.f};
+      auto weights = [&](int i) {
+        const float p0 = fast_exp2(__builtin_fmaf(S[i >> 3][2 * (i & 7)], cc, mneg));
+        const float p1 = fast_exp2(__builtin_fmaf(S[i >> 3][2 * (i & 7) + 1], cc, mneg));
+        pk[i] = bf16x2{(bf16)p0, (bf16)p1};
+        l2[i & 1] = __builtin_amdgcn_fdot2_f32_bf16(pk[i], one2, l2[i & 1], false);
+        asm volatile("" : "+v"(pk[i]));  // (here, not where the next iteration uses it)
       };
       bf16x8 fr[kSlots];
 #pragma unroll
       for (int x = 0; x < kAhead; ++x) fr[x] = frag(x);
-      if (!LATE) weights();
-      __builtin_amdgcn_sched_barrier(0);
-      Sn[0] = f32x16{};
-      Sn[1] = f32x16{};
 #pragma unroll
       for (int x = 0; x < kSlots; ++x) {
         if (x + kAhead < kSlots) fr[x + kAhead] = frag(x + kAhead);
         if (x < kPV) {
           O[x % kDB] = mfma32x32x16(fr[x], Pp[x / (2 * kDB)][(x / kDB) & 1], O[x % kDB]);
+#pragma unroll
+          for (int i = 0; i < 16 / kPV; ++i) weights(x * (16 / kPV) + i);
         } else {
-          const int ds = (x - kPV) >> 1, k2 = (x - kPV) & 1;
-          Sn[k2] = mfma32x32x16(fr[x], q[ds], Sn[k2]);
+          const int y = x - kPV;
+          if (y < 2) Sn[y] = f32x16{};
+          Sn[y & 1] = mfma32x32x16(fr[x], q[y >> 1], Sn[y & 1]);
+          constexpr int kPieces = 4 * C::kLoads, kEvery = C::kQK / kPieces;
+          if (y % kEvery == 0) {
+            const int j = y / kEvery;
+            if (j < kPieces / 2)
+              store(wk, true, C::kKBuf + kOdd * C::kTileBytes, j);
+            else
+              store(wv, false, C::kVBuf + kOdd * C::kTileBytes, j - kPieces / 2);
+            if (j == kPieces / 2 - 1) load(kg, min(u + 3, n - 1), wk);
+            if (j == kPieces - 1) load(vg, min(u + 1, n - 1), wv);
+          }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (LATE) weights();
+      l_run += l2[0] + l2[1];
       if (moved) {
 #pragma unroll
         for (int db = 0; db < kDB; ++db) O[db] *= alpha;
@@ -729,24 +733,17 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
         O[x % kDB] =
             mfma32x32x16(frag_v(vb, x / (2 * kDB), (x / kDB) & 1, x % kDB), P[x / (2 * kDB)][(x / kDB) & 1], O[x % kDB]);
     };
-    auto key_loop = [&](auto late_tag) __attribute__((always_inline)) {
-      int u = 0;
-      for (; u + 1 < n; u += 2) {
-        iteration(late_tag, Even{}, u, S, S2, Pp, P2);
-        iteration(late_tag, Odd{}, u + 1, S2, S, P2, Pp);
-      }
-      // the last tile's PV
-      if (u < n) {
-        iteration(late_tag, Even{}, u, S, S2, Pp, P2);
-        last_pv(Even{}, P2);
-      } else {
-        last_pv(Odd{}, Pp);
-      }
-    };
-    if (W == 4 || wave < 4)
-      key_loop(std::integral_constant<bool, false>{});
-    else
-      key_loop(std::integral_constant<bool, true>{});
+    int u = 0;
+    for (; u + 1 < n; u += 2) {
+      iteration(Even{}, u, S, S2, Pp, P2);
+      iteration(Odd{}, u + 1, S2, S, P2, Pp);
+    }
+    if (u < n) {
+      iteration(Even{}, u, S, S2, Pp, P2);
+      last_pv(Even{}, P2);
+    } else {
+      last_pv(Odd{}, Pp);
+    }
   }
 
   const float L = halves_sum(l_run);
