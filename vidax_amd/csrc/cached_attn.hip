@@ -881,6 +881,10 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const CachedAttnArgs a,
 
 // ------------------------------------------------------------------ launch plan
 constexpr int kManyRows = 32 * kWaves;
+// Caches of up to this many 32-key tiles are one item per stream of few rows: at
+// 1024 positions (eight tiles a wave) the launch that would merge costs more than
+// the parts save (12 heads, 700 keys: 11.5 us a call, with parts 15.5).
+constexpr int kFewWhole = 32;
 
 // Fills a part's plan; returns its workgroups.
 struct Planned {
@@ -904,7 +908,7 @@ Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, int D, in
   const int64_t tiles = (cap + tile - 1) / tile;
   const int64_t per_head = std::max<int64_t>(slots / (Hk * row_tiles), 1);
   p.min_chunk = 4;
-  if (tiles > p.min_chunk && (p.few || streams * row_tiles * Hk < slots)) {
+  if (tiles > (p.few ? kFewWhole : p.min_chunk) && (p.few || streams * row_tiles * Hk < slots)) {
     // As many items as find a place at once, where that leaves two and more per
     // stream; else several rounds of them.
     int64_t budget = per_head >= 2 * streams ? per_head - streams : std::max(3 * per_head, (int64_t)2 * streams);

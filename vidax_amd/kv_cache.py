@@ -60,74 +60,87 @@ def create_kv_cache(num_slots: int, capacity: int, num_kv_heads: int, head_dim: 
     return KVCache(k, v, ks, vs)
 
 
-def _check_cache(cache: KVCache, name: str) -> None:
-    k, v, ks, vs = cache
-    if (k.dtype == v.dtype == _E4M3 and ks.dtype == vs.dtype == _E8M0 and k.dim() == 4 and k.shape == v.shape and
-            ks.shape == vs.shape == k.shape[:3] and k.is_cuda and k.device == v.device == ks.device == vs.device and
-            k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
-        return  # (the checks below say what is wrong; the C ABI checks sizes and alignment)
-    parts = (("k", k, _E4M3, 4), ("v", v, _E4M3, 4), ("k_scale", ks, _E8M0, 3), ("v_scale", vs, _E8M0, 3))
-    for n, t, dtype, dims in parts:
+def _check_cache(cache: KVCache, name: str) -> Tuple[int, int, int, int, int]:
+    """(slots, num_kv_heads, capacity, head_dim, device index) of a cache whose
+    tensors go together (the C ABI checks sizes and alignment)."""
+    try:
+        k, v, ks, vs = cache
+        shape = k.shape
+        n, h, c, d = shape
+        index = k.get_device()
+        if (k.dtype is _E4M3 and v.dtype is _E4M3 and ks.dtype is _E8M0 and vs.dtype is _E8M0 and v.shape == shape and
+                ks.shape == (n, h, c) and vs.shape == (n, h, c) and index >= 0 and v.get_device() == index and
+                ks.get_device() == index and vs.get_device() == index and k.is_contiguous() and v.is_contiguous() and
+                ks.is_contiguous() and vs.is_contiguous()):
+            return n, h, c, d, index
+    except (AttributeError, TypeError, ValueError):
+        pass
+    # what is wrong
+    if not isinstance(cache, tuple) or len(cache) != 4 or not all(isinstance(t, torch.Tensor) for t in cache):
+        raise TypeError(f"{name} must be a KVCache")
+    parts = tuple(zip(("k", "v", "k_scale", "v_scale"), cache, (_E4M3, _E4M3, _E8M0, _E8M0), (4, 4, 3, 3)))
+    k = cache[0]
+    for part, t, dtype, dims in parts:
         if t.dtype != dtype:
-            raise TypeError(f"{name}.{n} must be {dtype}; got {t.dtype}")
+            raise TypeError(f"{name}.{part} must be {dtype}; got {t.dtype}")
         if t.dim() != dims or t.shape != k.shape[:dims]:
-            raise ValueError(f"{name}.{n} of shape {tuple(t.shape)} does not go with {name}.k {tuple(k.shape)}: k and "
-                             "v are (slots, num_kv_heads, capacity, head_dim), the scales the first three")
-    for n, t, _, _ in parts:
+            raise ValueError(f"{name}.{part} of shape {tuple(t.shape)} does not go with {name}.k {tuple(k.shape)}: k "
+                             "and v are (slots, num_kv_heads, capacity, head_dim), the scales the first three")
+    for part, t, _, _ in parts:
         if not t.is_cuda:
-            raise ValueError(f"{name}.{n} must be a GPU tensor")
+            raise ValueError(f"{name}.{part} must be a GPU tensor")
         if t.device != k.device:
             raise ValueError(f"{name}'s tensors must be on one device")
         if not t.is_contiguous():
-            raise ValueError(f"{name}.{n} must be contiguous")
+            raise ValueError(f"{name}.{part} must be contiguous")
+    raise ValueError(f"{name} is not a KVCache that the kernels take")
 
 
-def _check_rows(x: torch.Tensor, name: str, cache: KVCache) -> None:
+def _check_rows(x: torch.Tensor, name: str, index: int, head_dim: int) -> Tuple[int, int, int, int]:
+    """The shape of queries, keys or values (B, S, H, D), checked."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if x.dim() != 4:
-        raise ValueError(f"{name} must be (B, S, H, D); got shape {tuple(x.shape)}")
-    if x.dtype != torch.bfloat16:
+    shape = x.shape
+    if len(shape) != 4:
+        raise ValueError(f"{name} must be (B, S, H, D); got shape {tuple(shape)}")
+    if x.dtype is not torch.bfloat16:
         raise TypeError(f"{name} must be bfloat16; got {x.dtype}")
-    if x.device != cache.k.device:
+    if x.get_device() != index:
         raise ValueError(f"{name} must be on the cache's device")
-    if x.shape[3] != cache.k.shape[3]:
-        raise ValueError(f"{name} has head dim {x.shape[3]}, the cache {cache.k.shape[3]}")
+    if shape[3] != head_dim:
+        raise ValueError(f"{name} has head dim {shape[3]}, the cache {head_dim}")
+    return shape
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x as the kernels read it: its values in memory, the head dim contiguous,
-    16-byte aligned, strides multiples of 8 (a copy where it is not so)."""
+def _rows(x: torch.Tensor):
+    """(x as the kernels read it, its address, its C ABI strides): its values in
+    memory, the head dim contiguous, 16-byte aligned, strides multiples of 8 (a
+    copy where it is not so)."""
     if x.is_neg():
         x = x.resolve_neg()
+    at = x.data_ptr()
+    if at % 16 == 0 and x.is_contiguous():
+        return x, at, None
     x = _aligned(x) if x.stride(3) == 1 else x.contiguous()
-    return x if x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
+    if x.data_ptr() % 16 != 0:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x, x.data_ptr(), _strides3(x)
 
 
-def _ints(x, n: int, dev: torch.device, name: str) -> Optional[torch.Tensor]:
-    """int32 (n,) on dev, or None."""
+def _ints(x, n: int, index: int, name: str):
+    """(int32 tensor of n values on the device, its address), or (None, None)."""
     if x is None:
-        return None
-    if not (isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.device == dev and x.is_contiguous()):
-        x = torch.as_tensor(x, device=dev)
+        return None, None
+    if not (isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.get_device() == index and x.is_contiguous()):
+        x = torch.as_tensor(x, device=torch.device("cuda", index))
         if x.is_floating_point() or x.is_complex() or x.dtype == torch.bool:
             raise TypeError(f"{name} must hold integers; got {x.dtype}")
-        # (values past 32 bits are held at its ends, outside any cache)
-        x = x.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32).contiguous() if x.dtype == torch.int64 else \
-            x.to(torch.int32).contiguous()
+        if x.dtype == torch.int64:  # (values past 32 bits are held at its ends, outside any cache)
+            x = x.clamp(-(1 << 31), (1 << 31) - 1)
+        x = x.to(torch.int32).contiguous()
     if x.numel() != n:
         raise ValueError(f"{name} must hold {n} integers; got shape {tuple(x.shape)}")
-    return x
-
-
-def _ptr(x: Optional[torch.Tensor]) -> Optional[int]:
-    return None if x is None else x.data_ptr()
-
-
-def _cache_args(c: Optional[KVCache]):
-    if c is None:
-        return None, None, None, None, 0, 0
-    return (c.k.data_ptr(), c.v.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr(), c.k.shape[0], c.k.shape[2])
+    return x, x.data_ptr()
 
 
 def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, start=None, *, num=None, slots=None) -> None:
@@ -145,22 +158,24 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, start=None,
     unknown slot) are dropped. Where two items name the same slot and position,
     the later item's token is kept.
     """
-    _check_cache(cache, "cache")
-    for n, x in (("k", k), ("v", v)):
-        _check_rows(x, n, cache)
-        if x.shape[2] != cache.k.shape[1]:
-            raise ValueError(f"{n} has {x.shape[2]} heads, the cache {cache.k.shape[1]}")
-    if k.shape != v.shape:
-        raise ValueError(f"k and v shapes differ: {tuple(k.shape)} vs {tuple(v.shape)}")
-    B, S, Hk, D = k.shape
-    dev = k.device
-    start, num, slots = (_ints(x, B, dev, n) for x, n in ((start, "start"), (num, "num"), (slots, "slots")))
+    n_slots, Hk, cap, D, index = _check_cache(cache, "cache")
+    shape = _check_rows(k, "k", index, D)
+    vshape = _check_rows(v, "v", index, D)
+    B, S, heads, _ = shape
+    if heads != Hk or vshape[2] != Hk:
+        raise ValueError(f"k and v have {heads} and {vshape[2]} heads, the cache {Hk}")
+    if shape != vshape:
+        raise ValueError(f"k and v shapes differ: {tuple(shape)} vs {tuple(vshape)}")
+    start, start_at = _ints(start, B, index, "start")
+    num, num_at = _ints(num, B, index, "num")
+    slots, slots_at = _ints(slots, B, index, "slots")
     if B == 0 or S == 0:
         return
-    k, v = _rows(k), _rows(v)
-    ck, cv, ks, vs, n_slots, cap = _cache_args(cache)
-    _lib.launch(dev, _lib.lib().vx_kv_write_fwd, k.data_ptr(), v.data_ptr(), _strides3(k), _strides3(v), ck, cv, ks,
-                vs, n_slots, cap, _ptr(start), _ptr(num), _ptr(slots), B, S, Hk, D)
+    k, k_at, k_strides = _rows(k)
+    v, v_at, v_strides = _rows(v)
+    _lib.launch(cache.k.device, _lib.lib().vx_kv_write_fwd, k_at, v_at, k_strides, v_strides, cache.k.data_ptr(),
+                cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n_slots, cap, start_at, num_at,
+                slots_at, B, S, Hk, D)
 
 
 def kv_cache_read(cache: KVCache, length: int, start=None, *, slots=None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -169,22 +184,25 @@ def kv_cache_read(cache: KVCache, length: int, start=None, *, slots=None) -> Tup
     every such value; magnitudes below 2^-126 give zero). B is the length of
     `slots`, else of `start`, else the number of slots; defaults as in
     kv_cache_write. Positions outside the cache give zeros."""
-    _check_cache(cache, "cache")
+    n_slots, Hk, cap, D, index = _check_cache(cache, "cache")
     length = int(length)
     if length < 0:
         raise ValueError(f"length must be >= 0; got {length}")
     dev = cache.k.device
-    n_slots, Hk, _, D = cache.k.shape
-    slots = None if slots is None else torch.as_tensor(slots, device=dev)
-    start = None if start is None else torch.as_tensor(start, device=dev)
+    if slots is not None and not isinstance(slots, torch.Tensor):
+        slots = torch.as_tensor(slots, device=dev)
+    if start is not None and not isinstance(start, torch.Tensor):
+        start = torch.as_tensor(start, device=dev)
     B = slots.numel() if slots is not None else start.numel() if start is not None else n_slots
-    start, slots = _ints(start, B, dev, "start"), _ints(slots, B, dev, "slots")
-    k, v = (torch.empty((B, length, Hk, D), dtype=torch.bfloat16, device=dev) for _ in range(2))
+    start, start_at = _ints(start, B, index, "start")
+    slots, slots_at = _ints(slots, B, index, "slots")
+    k = torch.empty((B, length, Hk, D), dtype=torch.bfloat16, device=dev)
+    v = torch.empty_like(k)
     if B == 0 or length == 0:
         return k, v
-    ck, cv, ks, vs, n_slots, cap = _cache_args(cache)
-    _lib.launch(dev, _lib.lib().vx_kv_read_fwd, ck, cv, ks, vs, n_slots, cap, _ptr(start), _ptr(slots), B, length, Hk,
-                D, k.data_ptr(), v.data_ptr())
+    _lib.launch(dev, _lib.lib().vx_kv_read_fwd, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+                cache.v_scale.data_ptr(), n_slots, cap, start_at, slots_at, B, length, Hk, D, k.data_ptr(),
+                v.data_ptr())
     return k, v
 
 
@@ -196,31 +214,42 @@ def _workspace_bytes(device_index: int, *sizes: int) -> int:
 
 def _attend(q: torch.Tensor, cache: KVCache, prefix: Optional[KVCache], kv_len, prefix_len, q_len, slots,
             causal: bool, scale: Optional[float], out: Optional[torch.Tensor]) -> torch.Tensor:
-    _check_cache(cache, "cache")
-    _check_rows(q, "q", cache)
-    B, Sq, H, D = q.shape
-    dev = q.device
-    n_slots, Hk, cap, _ = cache.k.shape
+    n_slots, Hk, cap, D, index = _check_cache(cache, "cache")
+    B, Sq, H, _ = shape = _check_rows(q, "q", index, D)
+    kv_len, kv_len_at = _ints(kv_len, B, index, "kv_len")
+    q_len, q_len_at = _ints(q_len, B, index, "q_len")
+    slots, slots_at = _ints(slots, B, index, "slots")
     n_prefix = p_cap = 0
+    p_k = p_v = p_ks = p_vs = p_len_at = None
     if prefix is not None:
-        _check_cache(prefix, "prefix")
-        if prefix.k.shape[1] != Hk or prefix.k.shape[3] != D or prefix.k.device != dev:
+        n_prefix, p_heads, p_cap, p_dim, p_index = _check_cache(prefix, "prefix")
+        if p_heads != Hk or p_dim != D or p_index != index:
             raise ValueError("prefix and cache must agree on heads, head dim and device")
-        n_prefix, p_cap = prefix.k.shape[0], prefix.k.shape[2]
-        prefix_len = _ints(prefix_len, n_prefix, dev, "prefix_len")
-    kv_len, q_len, slots = (_ints(x, B, dev, n) for x, n in ((kv_len, "kv_len"), (q_len, "q_len"), (slots, "slots")))
+        prefix_len, p_len_at = _ints(prefix_len, n_prefix, index, "prefix_len")
+        p_k, p_v, p_ks, p_vs = (prefix.k.data_ptr(), prefix.v.data_ptr(), prefix.k_scale.data_ptr(),
+                                prefix.v_scale.data_ptr())
+    dev = q.device
+    empty = B == 0 or Sq == 0 or H == 0
+    if not empty:
+        q, q_at, q_strides = _rows(q)
+    out_strides = None
     if out is None:
-        out = torch.empty((B, Sq, H, D), dtype=q.dtype, device=dev)
-    elif (out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1 or out.device != dev):
+        out = torch.empty_like(q) if not empty and q_strides is None else torch.empty(shape, dtype=q.dtype, device=dev)
+    elif out.shape != shape or out.dtype != q.dtype or out.stride(-1) != 1 or out.device != dev:
         raise ValueError("out must be a (B, Sq, H, D) bf16 tensor with a contiguous head dim, on q's device")
-    if B == 0 or Sq == 0 or H == 0:
+    else:
+        out_strides = _strides3(out)
+    if empty:
         return out
-    q = _rows(q)
-    ws_bytes = _workspace_bytes(dev.index, cap, n_prefix, p_cap, B, Sq, H, Hk, D)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
-    _lib.launch(dev, _lib.lib().vx_cached_attn_fwd, q.data_ptr(), out.data_ptr(), _strides3(q), _strides3(out),
-                *_cache_args(cache), *_cache_args(prefix), _ptr(kv_len), _ptr(q_len), _ptr(slots), _ptr(prefix_len),
-                B, Sq, H, Hk, D, int(bool(causal)), D ** -0.5 if scale is None else float(scale), _ptr(ws), ws_bytes)
+    ws_bytes = _workspace_bytes(index, cap, n_prefix, p_cap, B, Sq, H, Hk, D)
+    ws = ws_at = None
+    if ws_bytes > 0:
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        ws_at = ws.data_ptr()
+    _lib.launch(dev, _lib.lib().vx_cached_attn_fwd, q_at, out.data_ptr(), q_strides, out_strides, cache.k.data_ptr(),
+                cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n_slots, cap, p_k, p_v, p_ks,
+                p_vs, n_prefix, p_cap, kv_len_at, q_len_at, slots_at, p_len_at, B, Sq, H, Hk, D, 1 if causal else 0,
+                D ** -0.5 if scale is None else float(scale), ws_at, ws_bytes)
     return out
 
 
