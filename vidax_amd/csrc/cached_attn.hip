@@ -78,82 +78,83 @@ __device__ __forceinline__ int keys_of(const Streams& s, int i) {
   return slot_of(s, i) < 0 ? 0 : clamp_len(s.len, i, s.c.cap);
 }
 
-// How the streams' key tiles (TILE keys each) are cut: every stream into
-// items of `chunk` tiles (at least one), numbered one after another.
-struct Cut {
-  int chunk;
-  int first, count;  // items of the stream that was asked for
-};
-
-// The items of stream `want`. Every wave works this out for itself, 64 streams
-// per step. budget 0: one item per stream.
+// The streams' key tiles (TILE keys each) stand one after another in one line,
+// which is cut into `budget` equal ranges (none shorter than min_chunk), one
+// workgroup each: however the lengths differ, all workgroups have the same work.
+// A range's piece of a stream is a part; range w's part of stream s has the number
+// w + s, which no other has. Every wave works its range out for itself from the
+// lengths, 64 streams per step. budget 0: range w is stream w, whole.
 template <int TILE>
-__device__ __forceinline__ Cut cut_of(const Streams& s, int budget, int min_chunk, int want) {
-  if (budget == 0) return Cut{0x7fffffff, want, 1};
-  const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  int mine = 0;
-  for (int i0 = 0; i0 < s.n; i0 += 64) {
-    const int t = i0 + lane < s.n ? (keys_of(s, i0 + lane) + TILE - 1) / TILE : 0;
-    if (s.n <= 64) mine = t;
-    int64_t x = t;
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off, 64);
-    total += x;
-  }
-  Cut c{(int)max((total + budget - 1) / budget, (int64_t)min_chunk), 0, 0};
-  for (int i0 = 0; i0 <= want; i0 += 64) {
-    const int i = i0 + lane;
-    if (s.n > 64) mine = i < s.n ? (keys_of(s, i) + TILE - 1) / TILE : 0;
-    const int items = i < s.n ? max((mine + c.chunk - 1) / c.chunk, 1) : 0;
-    int before = i < want ? items : 0;
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) before += __shfl_xor(before, off, 64);
-    c.first += before;
-    if (want - i0 < 64) c.count = __shfl(items, want - i0, 64);
-  }
-  return c;
+__device__ __forceinline__ int tiles_of(const Streams& s, int i) {
+  return i < s.n ? (keys_of(s, i) + TILE - 1) / TILE : 0;
 }
 
-// The stream of item `item` and its cut (stream -1: there is no such item).
-template <int TILE>
-__device__ __forceinline__ int stream_of(const Streams& s, int budget, int min_chunk, int item, Cut& c) {
-  if (budget == 0) {
-    c = Cut{0x7fffffff, item, 1};
-    return item < s.n ? item : -1;
-  }
-  const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  int mine = 0;
-  for (int i0 = 0; i0 < s.n; i0 += 64) {
-    mine = i0 + lane < s.n ? (keys_of(s, i0 + lane) + TILE - 1) / TILE : 0;
-    int64_t x = mine;
+__device__ __forceinline__ int64_t wave_sum(int64_t x) {
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off, 64);
-    total += x;
-  }
-  c.chunk = (int)max((total + budget - 1) / budget, (int64_t)min_chunk);
-  int base = 0;
-  for (int i0 = 0; i0 < s.n; i0 += 64) {
-    const int i = i0 + lane;
-    if (s.n > 64) mine = i < s.n ? (keys_of(s, i) + TILE - 1) / TILE : 0;
-    const int items = i < s.n ? max((mine + c.chunk - 1) / c.chunk, 1) : 0;
-    int upto = items;  // inclusive scan over the lanes
+  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
+
+// Tiles of a range.
+__device__ __forceinline__ int64_t range_tiles(int64_t total, int budget, int min_chunk) {
+  const int64_t each = total >> 31 == 0 ? ((uint32_t)total + budget - 1) / (uint32_t)budget
+                                        : (total + budget - 1) / budget;
+  return max(each, (int64_t)min_chunk);
+}
+
+// Where range w begins: its first stream, that stream's tile, the range's tiles (0: none).
+struct Range {
+  int stream, tile, tiles;
+};
+template <int TILE>
+__device__ __forceinline__ Range range_of(const Streams& s, int budget, int min_chunk, int w) {
+  const int lane = threadIdx.x & 63;
+  const int first = tiles_of<TILE>(s, lane);  // (64 streams are the usual case: read once)
+  int64_t total = wave_sum(first);
+  for (int i0 = 64; i0 < s.n; i0 += 64) total += wave_sum(tiles_of<TILE>(s, i0 + lane));
+  const int64_t each = range_tiles(total, budget, min_chunk), lo = w * each;
+  Range r{0, 0, (int)max(min(each, total - lo), (int64_t)0)};
+  int64_t base = 0;
+  for (int i0 = 0; i0 < s.n && base <= lo; i0 += 64) {
+    const int t = i0 == 0 ? first : tiles_of<TILE>(s, i0 + lane);
+    int64_t upto = t;  // inclusive scan over the lanes
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(upto, off, 64);
+      const int64_t o = __shfl_up(upto, off, 64);
       if (lane >= off) upto += o;
     }
-    const uint64_t past = __builtin_amdgcn_ballot_w64(base + upto > item);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(base + upto > lo);
     if (past != 0) {
       const int l = __builtin_ctzll(past);
-      c.count = __shfl(items, l, 64);
-      c.first = base + __shfl(upto, l, 64) - c.count;
-      return i0 + l;
+      r.stream = i0 + l;
+      r.tile = (int)(lo - base - __shfl(upto - t, l, 64));
+      break;
     }
     base += __shfl(upto, 63, 64);
   }
-  return -1;
+  return Range{__builtin_amdgcn_readfirstlane(r.stream), __builtin_amdgcn_readfirstlane(r.tile),
+               __builtin_amdgcn_readfirstlane(r.tiles)};
+}
+
+// The parts of stream `want`.
+struct Parts {
+  int first, count;
+};
+template <int TILE>
+__device__ __forceinline__ Parts parts_of(const Streams& s, int budget, int min_chunk, int want) {
+  if (budget == 0) return Parts{want, 1};
+  const int lane = threadIdx.x & 63;
+  int64_t total = 0, before = 0;
+  for (int i0 = 0; i0 < s.n; i0 += 64) {
+    const int t = tiles_of<TILE>(s, i0 + lane);
+    total += wave_sum(t);
+    if (i0 <= want) before += wave_sum(i0 + lane < want ? t : 0);
+  }
+  const int mine = tiles_of<TILE>(s, want);
+  if (mine == 0) return Parts{0, 0};
+  const int64_t each = range_tiles(total, budget, min_chunk);
+  const int64_t w0 = before / each, w1 = (before + mine - 1) / each;
+  return Parts{(int)w0 + want, (int)(w1 - w0) + 1};
 }
 
 // ---- the rows of a stream
@@ -180,16 +181,16 @@ __device__ __forceinline__ int own_bound(const CachedAttnArgs& a, int b, int i, 
 struct Part {
   Streams s;
   int32_t rows, per;          // rows of a stream per kv head; batch items that share it
-  int32_t budget, min_chunk;  // of its cut (budget 0: one item per stream)
-  int32_t items;              // items to launch, per kv head and row tile: some may have nothing to do
+  int32_t budget, min_chunk;  // ranges of its tiles, per kv head and row tile (0: one per stream)
+  int32_t items;              // ranges that are launched
   int32_t prefix;             // 1: every row sees every key
   int32_t one_round;          // 1: all workgroups find a place at once (many_part)
-  int32_t direct;             // 1: a stream of one item writes its output itself
+  int32_t direct;             // 1: a stream of one part writes its output itself
   int32_t few;                // few_part, else many_part
   float* ws;                  // partial results
 };
 
-// Partial results in the workspace, one block per (item, kv head): rows x D
+// Partial results in the workspace, one block per (part, kv head): rows x D
 // unnormalised fp32 outputs, then (reference point, sum) per row.
 __device__ __forceinline__ int64_t part_floats(int64_t rows, int D) { return (rows * (D + 2) + 3) & ~(int64_t)3; }
 
@@ -221,16 +222,18 @@ struct FewCfg {
   static constexpr int kSmem = kTiles + kWaves * 32 * 8;  // then (reference point, sum) of the waves' rows
 };
 
-// One wave's softmax state and the step over 32 keys.
-template <int D>
-struct FewState {
-  bf16x8 q[D / 16];
-  f32x16 O[D / 32];
-  float m, l;
+// Keys of one kv head as few_part reads them.
+struct FewKeys {
+  uint64_t k, v;          // addresses of the first rows
+  const uint8_t* scales;  // this lane's 16 bytes of a tile's scales (lanes 0-1 K, 2-3 V)
+  int len;                // keys
+  int bound, all;         // those that this lane's row sees, those that every row does
 };
 
-template <int D>
-__device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt, const int block,
+// A range of tiles of streams of at most 32 rows (BOTH: stream `block`, the
+// group's prefix in front of its own keys). The waves take every fourth tile.
+template <int D, bool BOTH>
+__device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt, const Part* pre, const int block,
                                          unsigned char* smem) {
   using C = FewCfg<D>;
   using T = Fp8Tile<D>;
@@ -241,52 +244,27 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hf = lane >> 5, col = lane & 31;
   const int Hk = s.c.Hk, kvh = block % Hk, item = block / Hk;
-  Cut cut;
-  const int stream = __builtin_amdgcn_readfirstlane(stream_of<kFewTile>(s, pt.budget, pt.min_chunk, item, cut));
-  if (stream < 0) return;  // (the whole workgroup)
-  const int len = __builtin_amdgcn_readfirstlane(keys_of(s, stream));
-  const int tiles = (len + kFewTile - 1) / kFewTile;
-  const int chunk_no = item - __builtin_amdgcn_readfirstlane(cut.first);
-  const int chunk = __builtin_amdgcn_readfirstlane(cut.chunk);
-  const int t0 = __builtin_amdgcn_readfirstlane((int)min((int64_t)chunk_no * chunk, (int64_t)tiles));
-  const int t1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)t0 + chunk, (int64_t)tiles));
-
-  const RowMap map{a, stream, kvh, a.H / Hk, pt.per};
-  int rb, ri, rh;
-  map.place(min(col, rows - 1), rb, ri, rh);
-  FewState<D> st;
-  {
-    const bf16* q = (const bf16*)a.q + rb * a.qs[0] + ri * a.qs[1] + rh * a.qs[2] + hf * 16;
-#pragma unroll
-    for (int x = 0; x < D / 32; ++x) {
-      st.q[2 * x] = *(const bf16x8*)(q + 32 * x);
-      st.q[2 * x + 1] = *(const bf16x8*)(q + 32 * x + 8);
-    }
-  }
-  // keys this lane's row sees, and those that every row sees
-  const int bound = pt.prefix ? len : own_bound(a, rb, ri, len);
-  int all = bound;
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) all = min(all, __shfl_xor(all, off, 64));
-  all = __builtin_amdgcn_readfirstlane(all);
-#pragma unroll
-  for (int db = 0; db < D / 32; ++db) st.O[db] = f32x16{};
-  st.m = kNegBig;
-  st.l = 0.f;
-
-  // ---- staging: copy p of a tile fills 1024 / D rows; lane L takes row L / (D / 16),
-  // LDS chunk L % (D / 16), which holds the row's chunk with that number XOR the swizzle
-  const int64_t row0 = ((int64_t)slot_of(s, stream) * Hk + kvh) * s.c.cap;
-  const uint64_t k_addr = uniform_u64((uint64_t)(uintptr_t)(s.c.k + row0 * D));
-  const uint64_t v_addr = uniform_u64((uint64_t)(uintptr_t)(s.c.v + row0 * D));
   lds_u8* const ring = (lds_u8*)smem + wave * C::kRing * C::kBuf;
   const uint32_t ring_addr = (uint32_t)(uintptr_t)ring;
-  const uint8_t* scale_src = (lane & 2 ? s.c.vs : s.c.ks) + row0 + 16 * (lane & 1);
-  auto stage = [&](int t, int buf) {
+  const float c = a.scale * kLog2e;
+  // K fragment row of this lane: MFMA row x holds key (x with bits 2 and 3
+  // swapped), so that a lane's 16 scores are keys 16 j + 8 hf + 0..7, j = 0, 1:
+  // the order in which the B operand of PV takes its weights
+  const int kkey = (col & 0x13) | ((col & 4) << 1) | ((col & 8) >> 1);
+
+  auto keys = [&](const Streams& from, int stream, int len) {
+    const int64_t row0 = ((int64_t)slot_of(from, stream) * Hk + kvh) * from.c.cap;
+    return FewKeys{uniform_u64((uint64_t)(uintptr_t)(from.c.k + row0 * D)),
+                   uniform_u64((uint64_t)(uintptr_t)(from.c.v + row0 * D)),
+                   (lane & 2 ? from.c.vs : from.c.ks) + row0 + 16 * (lane & 1), len, len, len};
+  };
+  // ---- staging: copy p of a tile fills 1024 / D rows; lane L takes row L / (D / 16),
+  // LDS chunk L % (D / 16), which holds the row's chunk with that number XOR the swizzle
+  auto stage = [&](const FewKeys& x, int t, int buf) {
     const uint32_t dst = ring_addr + buf * C::kBuf;
-    const int last = len - 1 - t * kFewTile;  // last row of the tile that holds a key
-    const i32x4_rsrc rk = raw_rsrc_u64(k_addr + (uint64_t)t * C::kTileBytes);
-    const i32x4_rsrc rv = raw_rsrc_u64(v_addr + (uint64_t)t * C::kTileBytes);
+    const int last = x.len - 1 - t * kFewTile;  // last row of the tile that holds a key
+    const i32x4_rsrc rk = raw_rsrc_u64(x.k + (uint64_t)t * C::kTileBytes);
+    const i32x4_rsrc rv = raw_rsrc_u64(x.v + (uint64_t)t * C::kTileBytes);
 #pragma unroll
     for (int p = 0; p < C::kCopies; ++p) {
       const int r = p * (1024 / D) + lane / T::kChunks;
@@ -295,140 +273,191 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
       lds_dma16_buf(rk, off, dst + p * 1024);
       lds_dma16_buf(rv, off, dst + C::kTileBytes + p * 1024);
     }
-    if (lane < 4) lds_dma16(scale_src + (int64_t)t * kFewTile, dst + 2 * C::kTileBytes);
+    if (lane < 4) lds_dma16(x.scales + (int64_t)t * kFewTile, dst + 2 * C::kTileBytes);
   };
 
-  const float c = a.scale * kLog2e;
-  // K fragment row of this lane: MFMA row x holds key (x with bits 2 and 3
-  // swapped), so that a lane's 16 scores are keys 16 j + 8 hf + 0..7, j = 0, 1:
-  // the order in which the B operand of PV takes its weights
-  const int kkey = (col & 0x13) | ((col & 4) << 1) | ((col & 8) >> 1);
-  auto step = [&](int t, int buf) {
-    const lds_u8* kb = ring + buf * C::kBuf;
-    const lds_u8* vb = kb + C::kTileBytes;
-    const lds_u8* sc = vb + C::kTileBytes;
-    const uint32_t ksb = sc[kkey], vsb = sc[32 + kkey];
-    // (a value row of scale NaN reaches the queries through its key's score)
-    const float kf = __uint_as_float(max(ksb, vsb) == 255u ? 0x7fc00000u : ksb << 23);
-    u32x2 vsc[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) vsc[j] = *(const VX_LDS u32x2*)(sc + 32 + 16 * j + 8 * hf);
-    f32x16 S = f32x16{};
-#pragma unroll
-    for (int x = 0; x < D / 32; ++x) {
-      const u32x4 kr = *(const VX_LDS u32x4*)(kb + kkey * D + (((2 * x + hf) ^ T::swizzle(kkey)) * 16));
-      S = mfma32x32x16(e4m3x8_bf16(u32x2{kr[0], kr[1]}, kf), st.q[2 * x], S);
-      S = mfma32x32x16(e4m3x8_bf16(u32x2{kr[2], kr[3]}, kf), st.q[2 * x + 1], S);
-    }
-    const int key0 = t * kFewTile;
-    const bool slow = key0 + kFewTile > all;  // some row does not see some key
-    float cc = c;
-    if (slow) {
-      cc = 1.0f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        S[i] = key0 + 16 * (i >> 3) + 8 * hf + (i & 7) < bound ? S[i] * c : -__builtin_inff();
-    }
-    float mx = S[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, S[i]);
-    mx = halves_max(mx) * cc;
-    if (__builtin_amdgcn_ballot_w64(mx > st.m + kSlack) != 0) {
-      const float mn = fmaxf(st.m, mx), alpha = fast_exp2(st.m - mn);
-      st.m = mn;
-      st.l *= alpha;
-#pragma unroll
-      for (int db = 0; db < D / 32; ++db) st.O[db] *= alpha;
-    }
-    bf16x8 P[2];
-    const float mneg = -st.m;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float p = fast_exp2(__builtin_fmaf(S[8 * j + e], cc, mneg));
-        st.l += p;
-        float w = p * __uint_as_float(((vsc[j][e >> 2] >> (8 * (e & 3))) & 0xffu) << 23);
-        if (slow && !(key0 + 16 * j + 8 * hf + e < bound)) w = 0.f;  // (its scale may be anything)
-        P[j][e] = (bf16)w;
-      }
-    // V^T fragment (db, j): lane group g = lane / 16 takes dims db 32 + (g % 2) 16
-    // + 0..15 of keys 16 j + 8 (g / 2) + 0..7
-    const int vr = (lane & 15) >> 1, vkey0 = 8 * hf + vr;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int db = 0; db < D / 32; ++db) {
-        const int key = 16 * j + vkey0;
-        typedef int i32x2 __attribute__((ext_vector_type(2)));
-        const i32x2 vr8 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((VX_LDS i32x2*)(
-            vb + key * D + (((2 * db + ((lane >> 4) & 1)) ^ T::swizzle(key)) * 16) + (lane & 1) * 8));
-        st.O[db] = mfma32x32x16(e4m3x8_bf16(u32x2{(uint32_t)vr8[0], (uint32_t)vr8[1]}, 1.0f), P[j], st.O[db]);
-      }
-  };
+  Range range{item, 0, 1};
+  if (pt.budget != 0) range = range_of<kFewTile>(s, pt.budget, pt.min_chunk, item);
+  for (int stream = range.stream, first = range.tile, left = range.tiles; left > 0; ++stream, first = 0) {
+    const int len = __builtin_amdgcn_readfirstlane(keys_of(s, stream));
+    const int tiles = (len + kFewTile - 1) / kFewTile;
+    const int take = pt.budget == 0 ? tiles : min(left, tiles - first);
+    left -= pt.budget == 0 ? 1 : take;
+    if (take == 0 && pt.budget != 0) continue;
 
-  const int n = t1 - t0 > wave ? (t1 - t0 - wave + kWaves - 1) / kWaves : 0;  // this wave's tiles
-  if (n > 0) stage(t0 + wave, 0);
-  if (n > 1) stage(t0 + wave + kWaves, 1);
-  for (int it = 0; it < n; ++it) {
-    if (it + 1 < n)
-      wait_copies<C::kPerTile>();
-    else
-      wait_copies<0>();
-    step(t0 + wave + it * kWaves, it & 1);
-    if (it + 2 < n) {
-      wait_lds_reads();
-      stage(t0 + wave + (it + 2) * kWaves, it & 1);
-    }
-  }
-
-  // ---- the four waves' results: rows x D through LDS, then D / 4 lanes per row
-  __syncthreads();
-  VX_LDS float* const xo = (VX_LDS float*)((lds_u8*)smem + wave * C::kExchange);
-  const float lsum = halves_sum(st.l);
-  if (col < rows) {
+    const RowMap map{a, stream, kvh, a.H / Hk, pt.per};
+    int rb, ri, rh;
+    map.place(min(col, rows - 1), rb, ri, rh);
+    bf16x8 q[D / 16];
+    {
+      const bf16* p = (const bf16*)a.q + rb * a.qs[0] + ri * a.qs[1] + rh * a.qs[2] + hf * 16;
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *(VX_LDS f32x4*)(xo + col * C::kOutRow + db * 32 + 8 * g + 4 * hf) =
-            f32x4{st.O[db][4 * g], st.O[db][4 * g + 1], st.O[db][4 * g + 2], st.O[db][4 * g + 3]};
-    if (hf == 0) {
-      ml[wave][col][0] = st.m;
-      ml[wave][col][1] = lsum;
-    }
-  }
-  __syncthreads();
-  const bool final_rows = pt.direct && cut.count == 1;
-  float* const part = final_rows ? nullptr : pt.ws + ((int64_t)item * Hk + kvh) * part_floats(rows, D);
-  for (int x = threadIdx.x; x < rows * (D / 4); x += kThreads) {
-    const int r = x / (D / 4), d = (x % (D / 4)) * 4;
-    float M = ml[0][r][0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, ml[w][r][0]);
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float L = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float al = fast_exp2(ml[w][r][0] - M);
-      L += ml[w][r][1] * al;
-      o += *(const VX_LDS f32x4*)((lds_u8*)smem + w * C::kExchange + (r * C::kOutRow + d) * 4) * al;
-    }
-    if (final_rows) {
-      int b, i, h;
-      map.place(r, b, i, h);
-      const float inv = is_zero(L) ? 0.f : 1.0f / L;
-      bf16x4 y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = (bf16)(o[e] * inv);
-      *(bf16x4*)((bf16*)a.o + b * a.os[0] + i * a.os[1] + h * a.os[2] + d) = y;
-    } else {
-      *(f32x4*)(part + r * D + d) = o;
-      if (d == 0) {
-        part[(int64_t)rows * D + 2 * r] = M;
-        part[(int64_t)rows * D + 2 * r + 1] = L;
+      for (int x = 0; x < D / 32; ++x) {
+        q[2 * x] = *(const bf16x8*)(p + 32 * x);
+        q[2 * x + 1] = *(const bf16x8*)(p + 32 * x + 8);
       }
     }
+    FewKeys own = keys(s, stream, len), shared = own;
+    int pre_tiles = 0;
+    if (BOTH) {
+      const int group = stream / pre->per;
+      shared = keys(pre->s, group, __builtin_amdgcn_readfirstlane(keys_of(pre->s, group)));
+      pre_tiles = (shared.len + kFewTile - 1) / kFewTile;
+      if (ri >= clamp_len(a.q_len, rb, a.Sq)) shared.bound = 0;  // (a padding row)
+    }
+    if (!pt.prefix) own.bound = own_bound(a, rb, ri, len);
+    auto least = [&](int x) {
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) x = min(x, __shfl_xor(x, off, 64));
+      return __builtin_amdgcn_readfirstlane(x);
+    };
+    own.all = least(own.bound);
+    if (BOTH) shared.all = least(shared.bound);
+
+    f32x16 O[D / 32];
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) O[db] = f32x16{};
+    float m = kNegBig, l = 0.f;
+    auto step = [&](const int key0, const int bound, const int all, const int buf) {
+      const lds_u8* kb = ring + buf * C::kBuf;
+      const lds_u8* vb = kb + C::kTileBytes;
+      const lds_u8* sc = vb + C::kTileBytes;
+      const uint32_t ksb = sc[kkey], vsb = sc[32 + kkey];
+      // (a value row of scale NaN reaches the queries through its key's score)
+      const float kf = __uint_as_float(max(ksb, vsb) == 255u ? 0x7fc00000u : ksb << 23);
+      u32x2 vsc[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) vsc[j] = *(const VX_LDS u32x2*)(sc + 32 + 16 * j + 8 * hf);
+      f32x16 S = f32x16{};
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) {
+        const u32x4 kr = *(const VX_LDS u32x4*)(kb + kkey * D + (((2 * x + hf) ^ T::swizzle(kkey)) * 16));
+        S = mfma32x32x16(e4m3x8_bf16(u32x2{kr[0], kr[1]}, kf), q[2 * x], S);
+        S = mfma32x32x16(e4m3x8_bf16(u32x2{kr[2], kr[3]}, kf), q[2 * x + 1], S);
+      }
+      const bool slow = key0 + kFewTile > all;  // some row does not see some key
+      float cc = c;
+      if (slow) {
+        cc = 1.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          S[i] = key0 + 16 * (i >> 3) + 8 * hf + (i & 7) < bound ? S[i] * c : -__builtin_inff();
+      }
+      float mx = S[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, S[i]);
+      mx = halves_max(mx) * cc;
+      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
+        const float mn = fmaxf(m, mx), alpha = fast_exp2(m - mn);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) O[db] *= alpha;
+      }
+      bf16x8 P[2];
+      const float mneg = -m;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p = fast_exp2(__builtin_fmaf(S[8 * j + e], cc, mneg));
+          l += p;
+          float w = p * __uint_as_float(((vsc[j][e >> 2] >> (8 * (e & 3))) & 0xffu) << 23);
+          if (slow && !(key0 + 16 * j + 8 * hf + e < bound)) w = 0.f;  // (its scale may be anything)
+          P[j][e] = (bf16)w;
+        }
+      // V^T fragment (db, j): lane group g = lane / 16 takes dims db 32 + (g % 2) 16
+      // + 0..15 of keys 16 j + 8 (g / 2) + 0..7
+      const int vr = (lane & 15) >> 1, vkey0 = 8 * hf + vr;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) {
+          const int key = 16 * j + vkey0;
+          typedef int i32x2 __attribute__((ext_vector_type(2)));
+          const i32x2 vr8 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((VX_LDS i32x2*)(
+              vb + key * D + (((2 * db + ((lane >> 4) & 1)) ^ T::swizzle(key)) * 16) + (lane & 1) * 8));
+          O[db] = mfma32x32x16(e4m3x8_bf16(u32x2{(uint32_t)vr8[0], (uint32_t)vr8[1]}, 1.0f), P[j], O[db]);
+        }
+    };
+
+    // tile t of the part: the prefix's first, then the stream's own from `first` on
+    const int here = pre_tiles + take;
+    auto stage_at = [&](int t, int buf) {
+      if (BOTH && t < pre_tiles)
+        stage(shared, t, buf);
+      else
+        stage(own, first + t - pre_tiles, buf);
+    };
+    const int n = here > wave ? (here - wave + kWaves - 1) / kWaves : 0;  // this wave's tiles
+    if (n > 0) stage_at(wave, 0);
+    if (n > 1) stage_at(wave + kWaves, 1);
+    for (int it = 0; it < n; ++it) {
+      if (it + 1 < n)
+        wait_copies<C::kPerTile>();
+      else
+        wait_copies<0>();
+      const int t = wave + it * kWaves;
+      const bool of_prefix = BOTH && t < pre_tiles;
+      step((of_prefix ? t : first + t - pre_tiles) * kFewTile, of_prefix ? shared.bound : own.bound,
+           of_prefix ? shared.all : own.all, it & 1);
+      if (it + 2 < n) {
+        wait_lds_reads();
+        stage_at(t + 2 * kWaves, it & 1);
+      }
+    }
+
+    // ---- the four waves' results: rows x D through LDS, then D / 4 lanes per row
+    __syncthreads();
+    VX_LDS float* const xo = (VX_LDS float*)((lds_u8*)smem + wave * C::kExchange);
+    const float lsum = halves_sum(l);
+    if (col < rows) {
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *(VX_LDS f32x4*)(xo + col * C::kOutRow + db * 32 + 8 * g + 4 * hf) =
+              f32x4{O[db][4 * g], O[db][4 * g + 1], O[db][4 * g + 2], O[db][4 * g + 3]};
+      if (hf == 0) {
+        ml[wave][col][0] = m;
+        ml[wave][col][1] = lsum;
+      }
+    }
+    __syncthreads();
+    const bool final_rows = pt.direct && take == tiles;
+    float* const part =
+        final_rows ? nullptr
+                   : pt.ws + ((int64_t)(pt.budget == 0 ? item : item + stream) * Hk + kvh) * part_floats(rows, D);
+    for (int x = threadIdx.x; x < rows * (D / 4); x += kThreads) {
+      const int r = x / (D / 4), d = (x % (D / 4)) * 4;
+      float M = ml[0][r][0];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) M = fmaxf(M, ml[w][r][0]);
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      float L = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float al = fast_exp2(ml[w][r][0] - M);
+        L += ml[w][r][1] * al;
+        o += *(const VX_LDS f32x4*)((lds_u8*)smem + w * C::kExchange + (r * C::kOutRow + d) * 4) * al;
+      }
+      if (final_rows) {
+        int b, i, h;
+        map.place(r, b, i, h);
+        const float inv = is_zero(L) ? 0.f : 1.0f / L;
+        bf16x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (bf16)(o[e] * inv);
+        *(bf16x4*)((bf16*)a.o + b * a.os[0] + i * a.os[1] + h * a.os[2] + d) = y;
+      } else {
+        *(f32x4*)(part + r * D + d) = o;
+        if (d == 0) {
+          part[(int64_t)rows * D + 2 * r] = M;
+          part[(int64_t)rows * D + 2 * r + 1] = L;
+        }
+      }
+    }
+    if (left > 0) __syncthreads();  // (the rings take the next part)
   }
 }
 
@@ -451,33 +480,21 @@ struct ManyCfg {
   static constexpr int kAhead = 2;  // fragments read ahead of their MFMA
 };
 
+// Tiles first .. first + take - 1 of a stream (`whole`: all it has) for rows rt
+// kRows + 0 .. kRows - 1 of kv head kvh; `part`: the number of its partial result.
 template <int D, int W>
-__device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& pt, const int block,
-                                          unsigned char* smem) {
+__device__ __forceinline__ void many_one(const CachedAttnArgs& a, const Part& pt, const int kvh, const int rt,
+                                         const int stream, const int len, const int first, const int take,
+                                         const bool whole, const int part_no, unsigned char* smem) {
   using C = ManyCfg<D, W>;
   const Streams& s = pt.s;
-  const int rows = pt.rows;
+  const int rows = pt.rows, Hk = s.c.Hk;
   constexpr int kDB = C::kDB, kDS = C::kDS, kPV = C::kPV, kSlots = C::kSlots, kAhead = C::kAhead;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // (what follows from it is formed here, not kept over the caller's loop)
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hf = lane >> 5, col = lane & 31;
-  const int Hk = s.c.Hk;
-  const int n_rt = (rows + C::kRows - 1) / C::kRows;
-  // Order: a prompt's last row tiles, which see the most keys, first; kv heads
-  // side by side, so that with 8 of them each XCD keeps one head's keys in its L2.
-  // Where all workgroups find a place at once (two per CU), the second half runs
-  // the other way, so that a long one shares its CU with a short one.
-  const int kvh = block % Hk;
-  int place = block / Hk;
-  if (pt.one_round) {
-    const int all_places = pt.items * n_rt, half = all_places / 2;
-    if (place >= half) place = half + all_places - 1 - place;
-  }
-  const int rt = n_rt - 1 - place / pt.items, item = place % pt.items;
-  Cut cut;
-  const int stream = __builtin_amdgcn_readfirstlane(stream_of<kManyTile>(s, pt.budget, pt.min_chunk, item, cut));
-  if (stream < 0) return;  // (the whole workgroup)
-  const int len = __builtin_amdgcn_readfirstlane(keys_of(s, stream));
   const RowMap map{a, stream, kvh, a.H / Hk, pt.per};
   bf16x8 q[kDS];
   int bound;  // keys that this lane's row sees
@@ -502,12 +519,7 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
     end = __builtin_amdgcn_readfirstlane(end);
   }
   const int tiles = (end + kManyTile - 1) / kManyTile;
-  const int chunk = __builtin_amdgcn_readfirstlane(cut.chunk);
-  const int chunk_no = item - __builtin_amdgcn_readfirstlane(cut.first);
-  // (64-bit minima are vector instructions: back to scalar registers)
-  const int t0 = __builtin_amdgcn_readfirstlane((int)min((int64_t)chunk_no * chunk, (int64_t)tiles));
-  const int n = __builtin_amdgcn_readfirstlane((int)min((int64_t)chunk, (int64_t)tiles - t0));
-
+  const int t0 = first, n = min(take, tiles - first);
   f32x16 O[kDB];
 #pragma unroll
   for (int db = 0; db < kDB; ++db) O[db] = f32x16{};
@@ -526,7 +538,6 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
   const uint64_t ksg = uniform_u64((uint64_t)(uintptr_t)(s.c.ks + row0));
   const uint64_t vsg = uniform_u64((uint64_t)(uintptr_t)(s.c.vs + row0));
   constexpr int kPlanes = D / 64;
-  const int tid = threadIdx.x;
   // thread bits: chunk (2), key bits 3, 0, 1 and 2, plane, the key's other bits
   const int plane = kPlanes == 2 ? (tid >> 6) & 1 : 0;
   const int skey = ((tid >> 3) & 1) | (((tid >> 4) & 3) << 1) | (((tid >> 2) & 1) << 3) |
@@ -677,7 +688,7 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
         const float p1 = fast_exp2(__builtin_fmaf(S[i >> 3][2 * (i & 7) + 1], cc, mneg));
         pk[i] = bf16x2{(bf16)p0, (bf16)p1};
         l2[i & 1] = __builtin_amdgcn_fdot2_f32_bf16(pk[i], one2, l2[i & 1], false);
-        asm volatile("" : "+v"(pk[i]));  // (here, not where the next iteration uses it)
+        asm volatile("" ::"v"(pk[i]));  // (here, not where the next iteration uses it)
       };
       bf16x8 fr[kSlots];
 #pragma unroll
@@ -748,7 +759,7 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
 
   const float L = halves_sum(l_run);
   const int r = rt * C::kRows + wave * 32 + col;
-  if (pt.direct && cut.count == 1) {
+  if (pt.direct && whole) {
     int rb, ri, rh;
     map.place(min(r, rows - 1), rb, ri, rh);
     const float inv = is_zero(L) ? 0.f : 1.0f / L;
@@ -762,7 +773,8 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
         for (int pr = 0; pr < 2; ++pr) *(u32x4*)(o + db * 32 + 8 * (2 * pr + hf)) = out[db][pr];
     }
   } else if (r < rows) {
-    float* const part = pt.ws + ((int64_t)item * Hk + kvh) * part_floats(rows, D);
+    float* const part =
+        pt.ws + ((int64_t)part_no * Hk + kvh) * part_floats(rows, D);
 #pragma unroll
     for (int db = 0; db < kDB; ++db)
 #pragma unroll
@@ -776,10 +788,44 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
   }
 }
 
-template <int D>
-__global__ __launch_bounds__(kThreads, 2) void few_kernel(const CachedAttnArgs a, const Part own) {
+// A range of tiles of streams of more rows, for one tile of rows of one kv head.
+template <int D, int W>
+__device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& pt, const int block,
+                                          unsigned char* smem) {
+  const int Hk = pt.s.c.Hk;
+  const int n_rt = (pt.rows + ManyCfg<D, W>::kRows - 1) / ManyCfg<D, W>::kRows;
+  // Order: a prompt's last row tiles, which see the most keys, first; kv heads
+  // side by side, so that with 8 of them each XCD keeps one head's keys in its L2.
+  // Where all workgroups find a place at once (two per CU), the second half runs
+  // the other way, so that a long one shares its CU with a short one.
+  const int kvh = __builtin_amdgcn_readfirstlane(block % Hk);
+  int place = block / Hk;
+  if (pt.one_round) {
+    const int all_places = pt.items * n_rt, half = all_places / 2;
+    if (place >= half) place = half + all_places - 1 - place;
+  }
+  const int rt = __builtin_amdgcn_readfirstlane(n_rt - 1 - place / pt.items);
+  const int item = __builtin_amdgcn_readfirstlane(place % pt.items);
+  Range range{item, 0, 1};
+  if (pt.budget != 0) range = range_of<kManyTile>(pt.s, pt.budget, pt.min_chunk, item);
+  for (int stream = range.stream, first = range.tile, left = range.tiles; left > 0; ++stream, first = 0) {
+    const int len = __builtin_amdgcn_readfirstlane(keys_of(pt.s, stream));
+    const int tiles = (len + kManyTile - 1) / kManyTile;
+    const int take = pt.budget == 0 ? tiles : min(left, tiles - first);
+    left -= pt.budget == 0 ? 1 : take;
+    if (take == 0 && pt.budget != 0) continue;
+    many_one<D, W>(a, pt, kvh, rt, stream, len, first, take, take == tiles, pt.budget == 0 ? item : item + stream,
+                   smem);
+    if (left > 0) __syncthreads();  // (the tiles' buffers take the next part)
+  }
+}
+
+// BOTH: prefixes and items of few positions in one pass, the prefix read (from
+// the L2) by each item rather than merged.
+template <int D, bool BOTH>
+__global__ __launch_bounds__(kThreads, 2) void few_kernel(const CachedAttnArgs a, const Part own, const Part pre) {
   __shared__ __attribute__((aligned(256))) unsigned char smem[FewCfg<D>::kSmem];
-  few_part<D>(a, own, blockIdx.x, smem);
+  few_part<D, BOTH>(a, own, &pre, blockIdx.x, smem);
 }
 
 template <int D>
@@ -799,12 +845,12 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(const CachedAttnArg
   const int block = blockIdx.x;
   if (block < pre_blocks) {
     if constexpr (PRE_FEW)
-      few_part<D>(a, pre, block, smem);
+      few_part<D, false>(a, pre, nullptr, block, smem);
     else
       many_part<D, kWaves>(a, pre, block, smem);
   } else {
     if constexpr (OWN_FEW)
-      few_part<D>(a, own, block - pre_blocks, smem);
+      few_part<D, false>(a, own, nullptr, block - pre_blocks, smem);
     else
       many_part<D, kWaves>(a, own, block - pre_blocks, smem);
   }
@@ -821,14 +867,14 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const CachedAttnArgs a,
   __shared__ f32x4 xo[kGroups][kLanes];
   __shared__ float xml[kGroups][2];
   const int b = blockIdx.y, Hk = a.c.Hk, G = a.H / Hk;
-  const Cut oc = own.few ? cut_of<kFewTile>(own.s, own.budget, own.min_chunk, b)
-                         : cut_of<kManyTile>(own.s, own.budget, own.min_chunk, b);
+  const Parts oc = own.few ? parts_of<kFewTile>(own.s, own.budget, own.min_chunk, b)
+                           : parts_of<kManyTile>(own.s, own.budget, own.min_chunk, b);
   const bool with_prefix = pre.s.n > 0;
-  if (!with_prefix && oc.count == 1) return;  // (written by its only chunk)
-  Cut pc{0, 0, 0};
+  if (!with_prefix && oc.count == 1) return;  // (written by the part itself)
+  Parts pc{0, 0};
   if (with_prefix)
-    pc = pre.few ? cut_of<kFewTile>(pre.s, pre.budget, pre.min_chunk, b / pre.per)
-                 : cut_of<kManyTile>(pre.s, pre.budget, pre.min_chunk, b / pre.per);
+    pc = pre.few ? parts_of<kFewTile>(pre.s, pre.budget, pre.min_chunk, b / pre.per)
+                 : parts_of<kManyTile>(pre.s, pre.budget, pre.min_chunk, b / pre.per);
   const int group = threadIdx.x / kLanes, d = (threadIdx.x % kLanes) * 4;
   const int part0 = group % split;
   const int64_t x = (int64_t)blockIdx.x * (kGroups / split) + group / split;
@@ -906,25 +952,23 @@ Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, int D, in
   const int64_t row_tiles = p.few ? 1 : (rows + kManyRows - 1) / kManyRows;
   const int64_t tile = p.few ? kFewTile : kManyTile;
   const int64_t tiles = (cap + tile - 1) / tile;
-  const int64_t per_head = std::max<int64_t>(slots / (Hk * row_tiles), 1);
-  p.min_chunk = 4;
-  if (tiles > (p.few ? kFewWhole : p.min_chunk) && (p.few || streams * row_tiles * Hk < slots)) {
-    // As many items as find a place at once, where that leaves two and more per
-    // stream; else several rounds of them.
-    int64_t budget = per_head >= 2 * streams ? per_head - streams : std::max(3 * per_head, (int64_t)2 * streams);
-    p.budget = (int)std::min(budget, streams * ((tiles + p.min_chunk - 1) / p.min_chunk));
-  }
-  p.items = p.budget + streams;
-  if (p.budget == 0) p.items = streams;
-  h.most_parts = (int)std::min<int64_t>(p.budget == 0 ? 1 : p.budget, (tiles + p.min_chunk - 1) / p.min_chunk);
+  p.min_chunk = p.few ? 4 : 2;
+  if (tiles > (p.few ? kFewWhole : 4) && (p.few || streams * row_tiles * Hk < slots))
+    p.budget = (int)std::min<int64_t>(std::max<int64_t>(slots / (Hk * row_tiles), 1),
+                                      streams * ((tiles + p.min_chunk - 1) / p.min_chunk));
+  p.items = p.budget != 0 ? p.budget : streams;
+  h.most_parts = (int)std::min<int64_t>(std::max(p.budget, 1), (tiles + p.min_chunk - 1) / p.min_chunk + 1);
   h.blocks = p.items * row_tiles * Hk;
   p.one_round = h.blocks <= slots;
-  if (with_prefix || p.budget > 0) h.floats = (int64_t)p.items * Hk * ((rows * (D + 2) + 3) & ~(int64_t)3);
+  // (part numbers go up to budget + streams - 2)
+  const int64_t parts = p.budget != 0 ? p.budget + (int64_t)streams - 1 : streams;
+  if (with_prefix || p.budget > 0) h.floats = parts * Hk * ((rows * (D + 2) + 3) & ~(int64_t)3);
   return h;
 }
 
 struct Plan {
   Planned own, pre;
+  bool both = false;  // few_kernel<D, true>
 };
 
 Plan plan_of(int cap, int n_prefix, int p_cap, int B, int Sq, int H, int Hk, int D) {
@@ -933,10 +977,23 @@ Plan plan_of(int cap, int n_prefix, int p_cap, int B, int Sq, int H, int Hk, int
   const int64_t rows = (int64_t)Sq * (H / Hk);
   Plan p;
   p.own = plan_part(B, rows, 1, cap, Hk, D, slots, false, n_prefix > 0);
-  if (n_prefix > 0) {
-    const int per = B / n_prefix;
-    p.pre = plan_part(n_prefix, rows * per, per, p_cap, Hk, D, std::max(slots - p.own.blocks, slots / 2), true, true);
+  if (n_prefix == 0) return p;
+  const int per = B / n_prefix;
+  if (p.own.p.few && (cap + p_cap) / kFewTile <= kFewWhole && (int64_t)B * Hk <= slots) {
+    p.both = true;
+    p.own = plan_part(B, rows, 1, cap, Hk, D, slots, false, false);
+    p.pre.p.per = per;
+    return p;
   }
+  // The prefix's share of the chip is its share of the positions (by the
+  // capacities), three times as heavy where 128 rows read them.
+  const int64_t pre_rows = rows * per;
+  const auto weight = [&](int64_t streams, int64_t r, int64_t c) {
+    return streams * c * (r <= 32 ? 1 : 3 * ((r + kManyRows - 1) / kManyRows));
+  };
+  const int64_t w_pre = weight(n_prefix, pre_rows, p_cap), w_own = weight(B, rows, cap);
+  p.pre = plan_part(n_prefix, pre_rows, per, p_cap, Hk, D, std::max<int64_t>(slots * w_pre / (w_pre + w_own), 1), true,
+                    true);
   return p;
 }
 
@@ -952,12 +1009,15 @@ int launch(const CachedAttnArgs& a, hipStream_t st, const char** launched) {
   pre.ws = a.ws + pl.own.floats;
   const dim3 grid((unsigned)(pl.pre.blocks + pl.own.blocks)), threads(kThreads);
   const int pre_blocks = (int)pl.pre.blocks;
-  if (n_prefix == 0) {
+  if (pl.both) {
+    hipLaunchKernelGGL((few_kernel<D, true>), grid, threads, 0, st, a, own, pre);
+    *launched = D == 128 ? "few_kernel<128, true>" : "few_kernel<64, true>";
+  } else if (n_prefix == 0) {
     if (own.few)
-      hipLaunchKernelGGL(few_kernel<D>, grid, threads, 0, st, a, own);
+      hipLaunchKernelGGL((few_kernel<D, false>), grid, threads, 0, st, a, own, pre);
     else
       hipLaunchKernelGGL(many_kernel<D>, grid, threads, 0, st, a, own);
-    *launched = own.few ? (D == 128 ? "few_kernel<128>" : "few_kernel<64>")
+    *launched = own.few ? (D == 128 ? "few_kernel<128, false>" : "few_kernel<64, false>")
                         : (D == 128 ? "many_kernel<128>" : "many_kernel<64>");
   } else if (pre.few) {  // (a prefix's streams have no fewer rows than the items')
     hipLaunchKernelGGL((prefix_kernel<D, true, true>), grid, threads, 0, st, a, pre, own, pre_blocks);
@@ -970,7 +1030,7 @@ int launch(const CachedAttnArgs& a, hipStream_t st, const char** launched) {
     *launched = D == 128 ? "prefix_kernel<128, false, false>" : "prefix_kernel<64, false, false>";
   }
   int err = (int)hipGetLastError();
-  if (err == 0 && (n_prefix > 0 || own.budget > 0)) {
+  if (err == 0 && !pl.both && (n_prefix > 0 || own.budget > 0)) {
     constexpr int kGroups = kThreads / (D / 4);
     int split = 1;  // about four parts in turn per group of lanes
     while (split < kGroups && 4 * split < pl.own.most_parts + (n_prefix > 0 ? pl.pre.most_parts : 0)) split *= 2;
