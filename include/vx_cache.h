@@ -116,10 +116,12 @@ int32_t vx_cached_attn_check(const void* q, const void* out, const int64_t* q_st
 
 /*
  * Workspace bytes vx_cached_attn_fwd needs for these sizes on the current
- * device (0: none; -1 on failure). num_prefixes is 0 without a prefix.
+ * device (0: none; -1 on failure). num_prefixes is 0 without a prefix; cross is
+ * 1 for a call that is not causal and has no q_len.
  */
 int64_t vx_cached_attn_workspace_size(int32_t capacity, int32_t num_prefixes, int32_t prefix_capacity, int32_t batch,
-                                      int32_t seq_q, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim);
+                                      int32_t seq_q, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                      int32_t cross);
 
 #ifdef __cplusplus
 }

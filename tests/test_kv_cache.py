@@ -656,3 +656,39 @@ def test_refusals_of_gpu_calls(gpu):
     assert vx.cached_attention(x[:, :0], c).shape == (2, 0, 2, 64)
     assert vx.kv_cache_read(c, 0)[0].shape == (2, 0, 2, 64)
     vx.kv_cache_write(c, x[:, :0], x[:, :0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,slots", [(128, None), (64, [2, 7, 0])])
+def test_long_cross_attention(gpu, D, slots):
+    """Queries long enough for the expansion to bf16: sampled rows against the
+    oracle, all rows against the same call in shorter pieces; a NaN token makes
+    its head's rows NaN, and an item without a slot or a key gives zeros."""
+    print(f"[case] long cross attention D={D} slots={slots}", flush=True)
+    rng = np.random.default_rng(31)
+    B, Sq, H, cap, lens = 3, 4100, 3, 192, [150, 192, 0 if slots is None else 33]
+    by_slot = np.zeros(3, int)
+    for b in range(B):
+        slot = b if slots is None else slots[b]
+        if slot < 3:
+            by_slot[slot] = lens[b]
+    k = rng.standard_normal((3, cap, H, D))
+    k[0 if slots is None else 2, 17, 1, 3] = np.nan
+    cache, _ = _noise_cache(rng, 3, H, cap, D, gpu)
+    vx.kv_cache_write(cache, _bf16(k, gpu), _bf16(rng.standard_normal((3, cap, H, D)), gpu), num=by_slot)
+    q = _bf16(2 * rng.standard_normal((B, Sq, H, D)), gpu)
+    kw = dict(slots=_ints(slots, gpu), causal=False)
+    got = vx.cached_attention(q, cache, _ints(lens, gpu), **kw)
+    assert _lib.last_launch().startswith("flash_")
+    pieces = torch.cat([vx.cached_attention(q[:, i:i + 2050], cache, _ints(lens, gpu), **kw) for i in (0, 2050)], 1)
+    want_nan = torch.zeros_like(got, dtype=torch.bool)
+    want_nan[0, :, 1] = True
+    assert torch.equal(got.isnan(), want_nan) and torch.equal(pieces.isnan(), want_nan)
+    empty = 2 if slots is None else 1
+    assert (got[empty] == 0).all() and (pieces[empty] == 0).all()
+    rows = np.unique(np.linspace(0, Sq - 1, 40).astype(int))
+    keep = [0, 2]  # (head 1 of item 0 is NaN)
+    held = [x[:, keep] for x in _held(cache, by_slot)]
+    for y in (got, pieces):
+        sub, qs = y[:, rows][:, :, keep], q[:, rows][:, :, keep]
+        _assert_close(sub, qs, held, None, kv_len=lens, slots=slots, causal=False)

@@ -176,7 +176,7 @@ def lib() -> ctypes.CDLL:
             h.vx_cached_attn_check.restype = _i32
             h.vx_cached_attn_check.argtypes = _CACHED_ATTN_ARGS
             h.vx_cached_attn_workspace_size.restype = _i64
-            h.vx_cached_attn_workspace_size.argtypes = [_i32] * 8
+            h.vx_cached_attn_workspace_size.argtypes = [_i32] * 9
             h.vx_last_launch.restype = ctypes.c_char_p
             h.vx_last_launch.argtypes = []
             _lib = h

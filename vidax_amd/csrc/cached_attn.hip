@@ -85,55 +85,74 @@ __device__ __forceinline__ int keys_of(const Streams& s, int i) {
 // w + s, which no other has. Every wave works its range out for itself from the
 // lengths, 64 streams per step. budget 0: range w is stream w, whole.
 template <int TILE>
-__device__ __forceinline__ int tiles_of(const Streams& s, int i) {
-  return i < s.n ? (keys_of(s, i) + TILE - 1) / TILE : 0;
+__device__ __forceinline__ int tiles_in(int keys) {
+  return (keys + TILE - 1) / TILE;
 }
 
-__device__ __forceinline__ int64_t wave_sum(int64_t x) {
+__device__ __forceinline__ int lane_keys(const Streams& s, int i) { return i < s.n ? keys_of(s, i) : 0; }
+
+__device__ __forceinline__ int wave_sum(int x) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off, 64);
   return x;
 }
 
-// Tiles of a range.
-__device__ __forceinline__ int64_t range_tiles(int64_t total, int budget, int min_chunk) {
-  const int64_t each = total >> 31 == 0 ? ((uint32_t)total + budget - 1) / (uint32_t)budget
-                                        : (total + budget - 1) / budget;
-  return max(each, (int64_t)min_chunk);
+// Tiles of a range. (All streams' tiles together are below 2^31: checked by the C ABI.)
+__device__ __forceinline__ int range_tiles(int total, int budget, int min_chunk) {
+  return max((int)(((uint32_t)total + budget - 1) / (uint32_t)budget), min_chunk);
 }
 
-// Where range w begins: its first stream, that stream's tile, the range's tiles (0: none).
+// Where range w begins: its first stream, that one's keys, the tile in it, and the range's tiles (0: none).
 struct Range {
-  int stream, tile, tiles;
+  int stream, len, tile, tiles;
 };
 template <int TILE>
 __device__ __forceinline__ Range range_of(const Streams& s, int budget, int min_chunk, int w) {
   const int lane = threadIdx.x & 63;
-  const int first = tiles_of<TILE>(s, lane);  // (64 streams are the usual case: read once)
-  int64_t total = wave_sum(first);
-  for (int i0 = 64; i0 < s.n; i0 += 64) total += wave_sum(tiles_of<TILE>(s, i0 + lane));
-  const int64_t each = range_tiles(total, budget, min_chunk), lo = w * each;
-  Range r{0, 0, (int)max(min(each, total - lo), (int64_t)0)};
-  int64_t base = 0;
-  for (int i0 = 0; i0 < s.n && base <= lo; i0 += 64) {
-    const int t = i0 == 0 ? first : tiles_of<TILE>(s, i0 + lane);
-    int64_t upto = t;  // inclusive scan over the lanes
+  const int first = lane_keys(s, lane);  // (64 streams are the usual case: read once)
+  int total = wave_sum(tiles_in<TILE>(first));
+  for (int i0 = 64; i0 < s.n; i0 += 64) total += wave_sum(tiles_in<TILE>(lane_keys(s, i0 + lane)));
+  const int each = range_tiles(total, budget, min_chunk);
+  const int64_t lo = (int64_t)w * each;
+  Range r{0, 0, 0, 0};
+  if (lo < total) {
+    r.tiles = min(each, total - (int)lo);
+    int base = 0;
+    for (int i0 = 0;; i0 += 64) {  // (ends: lo is below the total)
+      const int keys = i0 == 0 ? first : lane_keys(s, i0 + lane), t = tiles_in<TILE>(keys);
+      int upto = t;  // inclusive scan over the lanes
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int64_t o = __shfl_up(upto, off, 64);
-      if (lane >= off) upto += o;
+      for (int off = 1; off < 64; off <<= 1) {
+        const int o = __shfl_up(upto, off, 64);
+        if (lane >= off) upto += o;
+      }
+      const uint64_t past = __builtin_amdgcn_ballot_w64(base + upto > (int)lo);
+      if (past != 0 || i0 + 64 >= s.n) {
+        const int l = past != 0 ? __builtin_ctzll(past) : 63;
+        r.stream = min(i0 + l, s.n - 1);
+        r.len = __shfl(keys, l, 64);
+        r.tile = (int)lo - base - __shfl(upto - t, l, 64);
+        break;
+      }
+      base += __shfl(upto, 63, 64);
     }
-    const uint64_t past = __builtin_amdgcn_ballot_w64(base + upto > lo);
-    if (past != 0) {
-      const int l = __builtin_ctzll(past);
-      r.stream = i0 + l;
-      r.tile = (int)(lo - base - __shfl(upto - t, l, 64));
-      break;
-    }
-    base += __shfl(upto, 63, 64);
   }
-  return Range{__builtin_amdgcn_readfirstlane(r.stream), __builtin_amdgcn_readfirstlane(r.tile),
-               __builtin_amdgcn_readfirstlane(r.tiles)};
+  return Range{__builtin_amdgcn_readfirstlane(r.stream), __builtin_amdgcn_readfirstlane(r.len),
+               __builtin_amdgcn_readfirstlane(r.tile), __builtin_amdgcn_readfirstlane(r.tiles)};
+}
+
+__device__ __forceinline__ Range whole_stream(const Streams& s, int i) {
+  return Range{i, __builtin_amdgcn_readfirstlane(keys_of(s, i)), 0, 1};
+}
+
+// The next stream that has keys, and its keys. (There is one while a range has
+// tiles left; false, past the last, only if the lengths changed under the launch.)
+__device__ __forceinline__ bool next_stream(const Streams& s, int& stream, int& len) {
+  for (++stream; stream < s.n; ++stream) {
+    len = __builtin_amdgcn_readfirstlane(keys_of(s, stream));
+    if (len > 0) return true;
+  }
+  return false;
 }
 
 // The parts of stream `want`.
@@ -144,17 +163,17 @@ template <int TILE>
 __device__ __forceinline__ Parts parts_of(const Streams& s, int budget, int min_chunk, int want) {
   if (budget == 0) return Parts{want, 1};
   const int lane = threadIdx.x & 63;
-  int64_t total = 0, before = 0;
+  int total = 0, before = 0, mine = 0;
   for (int i0 = 0; i0 < s.n; i0 += 64) {
-    const int t = tiles_of<TILE>(s, i0 + lane);
+    const int t = tiles_in<TILE>(lane_keys(s, i0 + lane));
     total += wave_sum(t);
     if (i0 <= want) before += wave_sum(i0 + lane < want ? t : 0);
+    if (want >= i0 && want < i0 + 64) mine = __shfl(t, want - i0, 64);
   }
-  const int mine = tiles_of<TILE>(s, want);
   if (mine == 0) return Parts{0, 0};
-  const int64_t each = range_tiles(total, budget, min_chunk);
-  const int64_t w0 = before / each, w1 = (before + mine - 1) / each;
-  return Parts{(int)w0 + want, (int)(w1 - w0) + 1};
+  const uint32_t each = range_tiles(total, budget, min_chunk);
+  const int w0 = (uint32_t)before / each, w1 = (uint32_t)(before + mine - 1) / each;
+  return Parts{w0 + want, w1 - w0 + 1};
 }
 
 // ---- the rows of a stream
@@ -276,14 +295,11 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
     if (lane < 4) lds_dma16(x.scales + (int64_t)t * kFewTile, dst + 2 * C::kTileBytes);
   };
 
-  Range range{item, 0, 1};
-  if (pt.budget != 0) range = range_of<kFewTile>(s, pt.budget, pt.min_chunk, item);
-  for (int stream = range.stream, first = range.tile, left = range.tiles; left > 0; ++stream, first = 0) {
-    const int len = __builtin_amdgcn_readfirstlane(keys_of(s, stream));
-    const int tiles = (len + kFewTile - 1) / kFewTile;
-    const int take = pt.budget == 0 ? tiles : min(left, tiles - first);
-    left -= pt.budget == 0 ? 1 : take;
-    if (take == 0 && pt.budget != 0) continue;
+  const Range range = pt.budget == 0 ? whole_stream(s, item) : range_of<kFewTile>(s, pt.budget, pt.min_chunk, item);
+  int stream = range.stream, len = range.len, first = range.tile, left = range.tiles;
+  while (left > 0) {
+    const int tiles = tiles_in<kFewTile>(len), take = pt.budget == 0 ? tiles : min(left, tiles - first);
+    left -= pt.budget == 0 ? left : take;
 
     const RowMap map{a, stream, kvh, a.H / Hk, pt.per};
     int rb, ri, rh;
@@ -457,7 +473,11 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
         }
       }
     }
-    if (left > 0) __syncthreads();  // (the rings take the next part)
+    if (left > 0) {
+      if (!next_stream(s, stream, len)) return;
+      first = 0;
+      __syncthreads();  // (the rings take the next part)
+    }
   }
 }
 
@@ -806,17 +826,19 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
   }
   const int rt = __builtin_amdgcn_readfirstlane(n_rt - 1 - place / pt.items);
   const int item = __builtin_amdgcn_readfirstlane(place % pt.items);
-  Range range{item, 0, 1};
-  if (pt.budget != 0) range = range_of<kManyTile>(pt.s, pt.budget, pt.min_chunk, item);
-  for (int stream = range.stream, first = range.tile, left = range.tiles; left > 0; ++stream, first = 0) {
-    const int len = __builtin_amdgcn_readfirstlane(keys_of(pt.s, stream));
-    const int tiles = (len + kManyTile - 1) / kManyTile;
-    const int take = pt.budget == 0 ? tiles : min(left, tiles - first);
-    left -= pt.budget == 0 ? 1 : take;
-    if (take == 0 && pt.budget != 0) continue;
+  const Range range =
+      pt.budget == 0 ? whole_stream(pt.s, item) : range_of<kManyTile>(pt.s, pt.budget, pt.min_chunk, item);
+  int stream = range.stream, len = range.len, first = range.tile, left = range.tiles;
+  while (left > 0) {
+    const int tiles = tiles_in<kManyTile>(len), take = pt.budget == 0 ? tiles : min(left, tiles - first);
+    left -= pt.budget == 0 ? left : take;
     many_one<D, W>(a, pt, kvh, rt, stream, len, first, take, take == tiles, pt.budget == 0 ? item : item + stream,
                    smem);
-    if (left > 0) __syncthreads();  // (the tiles' buffers take the next part)
+    if (left > 0) {
+      if (!next_stream(pt.s, stream, len)) return;
+      first = 0;
+      __syncthreads();  // (the tiles' buffers take the next part)
+    }
   }
 }
 
@@ -937,7 +959,7 @@ struct Planned {
   Part p{};
   int64_t blocks = 0;
   int64_t floats = 0;  // of partial results
-  int most_parts = 1;  // of a stream
+  int usual_parts = 1;  // of a stream
 };
 
 Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, int D, int64_t slots, bool prefix,
@@ -957,7 +979,7 @@ Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, int D, in
     p.budget = (int)std::min<int64_t>(std::max<int64_t>(slots / (Hk * row_tiles), 1),
                                       streams * ((tiles + p.min_chunk - 1) / p.min_chunk));
   p.items = p.budget != 0 ? p.budget : streams;
-  h.most_parts = (int)std::min<int64_t>(std::max(p.budget, 1), (tiles + p.min_chunk - 1) / p.min_chunk + 1);
+  h.usual_parts = p.budget / streams + 1;
   h.blocks = p.items * row_tiles * Hk;
   p.one_round = h.blocks <= slots;
   // (part numbers go up to budget + streams - 2)
@@ -985,15 +1007,21 @@ Plan plan_of(int cap, int n_prefix, int p_cap, int B, int Sq, int H, int Hk, int
     p.pre.p.per = per;
     return p;
   }
-  // The prefix's share of the chip is its share of the positions (by the
-  // capacities), three times as heavy where 128 rows read them.
+  // The prefix takes what the items' own workgroups leave, where they are whole
+  // streams on at most half of the chip: all start at once. Otherwise each takes
+  // its share of the positions (by the capacities; three times as heavy where 128
+  // rows read them).
   const int64_t pre_rows = rows * per;
   const auto weight = [&](int64_t streams, int64_t r, int64_t c) {
     return streams * c * (r <= 32 ? 1 : 3 * ((r + kManyRows - 1) / kManyRows));
   };
   const int64_t w_pre = weight(n_prefix, pre_rows, p_cap), w_own = weight(B, rows, cap);
-  p.pre = plan_part(n_prefix, pre_rows, per, p_cap, Hk, D, std::max<int64_t>(slots * w_pre / (w_pre + w_own), 1), true,
-                    true);
+  int64_t pre_slots = std::max<int64_t>(slots * w_pre / (w_pre + w_own), 1);
+  if (p.own.p.budget > 0)
+    p.own = plan_part(B, rows, 1, cap, Hk, D, std::max<int64_t>(slots - pre_slots, 1), false, true);
+  else if (p.own.blocks <= slots / 2)
+    pre_slots = slots - p.own.blocks;
+  p.pre = plan_part(n_prefix, pre_rows, per, p_cap, Hk, D, pre_slots, true, true);
   return p;
 }
 
@@ -1033,7 +1061,7 @@ int launch(const CachedAttnArgs& a, hipStream_t st, const char** launched) {
   if (err == 0 && !pl.both && (n_prefix > 0 || own.budget > 0)) {
     constexpr int kGroups = kThreads / (D / 4);
     int split = 1;  // about four parts in turn per group of lanes
-    while (split < kGroups && 4 * split < pl.own.most_parts + (n_prefix > 0 ? pl.pre.most_parts : 0)) split *= 2;
+    while (split < kGroups && 4 * split < pl.own.usual_parts + (n_prefix > 0 ? pl.pre.usual_parts : 0)) split *= 2;
     const int64_t per_wg = kGroups / split;
     hipLaunchKernelGGL(merge_kernel<D>, dim3((unsigned)(((int64_t)a.c.Hk * own.rows + per_wg - 1) / per_wg), a.B),
                        threads, 0, st, a, own, pre, split);

@@ -175,6 +175,53 @@ __global__ __launch_bounds__(kWaves * 64) void kv_read_kernel(const KvReadArgs a
   }
 }
 
+// The first limit[b] positions of each item's slot to contiguous (B, Hk, cap, D) rows
+// for the flash kernels, and those lengths, held to the cache, to len_out. A
+// token whose key or value row has scale NaN becomes a zero key with a NaN value:
+// NaN for every query, whatever weight it gets. Positions lie side by side in
+// both forms, so neighbouring waves take neighbouring positions of one head.
+template <int D>
+__global__ __launch_bounds__(kWaves * 64) void kv_expand_kernel(const KvReadArgs a) {
+  using R = Rows<D>;
+  const int lane = threadIdx.x & 63;
+  const uint32_t w = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t blocks = ((uint32_t)a.c.cap + kTokens - 1) / kTokens;
+  const uint32_t head = w / blocks, t0 = (w % blocks) * kTokens;
+  const int b = blockIdx.y;
+  const int slot = a.slots != nullptr ? a.slots[b] : b;
+  int n = a.limit != nullptr ? min(max(a.limit[b], 0), a.c.cap) : a.c.cap;
+  if ((uint32_t)slot >= (uint32_t)a.c.slots) n = 0;
+  if (w == 0 && lane == 0) a.len_out[b] = n;
+  if (head >= (uint32_t)a.c.Hk || t0 >= (uint32_t)n) return;
+  const int r = lane / R::kLanes, c = lane % R::kLanes;
+  const int64_t from = ((int64_t)slot * a.c.Hk + head) * a.c.cap + t0 + r;
+  const int64_t to = ((int64_t)b * a.c.Hk + head) * a.c.cap + t0 + r;
+  u32x4 yk[R::kPasses], yv[R::kPasses];
+  uint32_t sk[R::kPasses], sv[R::kPasses];
+#pragma unroll
+  for (int p = 0; p < R::kPasses; ++p) {  // (the capacity is a multiple of kTokens)
+    const int64_t row = from + p * R::kPerPass;
+    yk[p] = *(const u32x4*)(a.c.k + row * D + c * 16);
+    yv[p] = *(const u32x4*)(a.c.v + row * D + c * 16);
+    sk[p] = a.c.ks[row];
+    sv[p] = a.c.vs[row];
+  }
+#pragma unroll
+  for (int p = 0; p < R::kPasses; ++p) {
+    const int64_t o = (to + p * R::kPerPass) * D + c * 16;
+    const bool bad = max(sk[p], sv[p]) == 255u;
+    const u32x4 k = bad ? u32x4{0, 0, 0, 0} : yk[p];
+    const float fk = e8m0_scale(bad ? 127u : sk[p]), fv = e8m0_scale(bad ? 255u : sv[p]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      *(bf16x8*)((bf16*)a.k_out + o + 8 * i) = e4m3x8_bf16(u32x2{k[2 * i], k[2 * i + 1]}, fk);
+      *(bf16x8*)((bf16*)a.v_out + o + 8 * i) = e4m3x8_bf16(u32x2{yv[p][2 * i], yv[p][2 * i + 1]}, fv);
+    }
+  }
+}
+
+static_assert(64 % kTokens == 0, "a capacity, a multiple of 64, is one of kTokens");
+
 dim3 grid_of(int B, int S, int Hk) {
   const int64_t waves = ((int64_t)S + kTokens - 1) / kTokens * Hk;  // < 2^31 (checked by the C ABI)
   return dim3((unsigned)((waves + kWaves - 1) / kWaves), (unsigned)B);
@@ -199,6 +246,16 @@ int launch_kv_read(const KvReadArgs& a, void* stream, const char** launched) {
   else
     hipLaunchKernelGGL(kv_read_kernel<64>, grid, dim3(kWaves * 64), 0, (hipStream_t)stream, a);
   *launched = a.c.D == 128 ? "kv_read_kernel<128>" : "kv_read_kernel<64>";
+  return (int)hipGetLastError();
+}
+
+int launch_kv_expand(const KvReadArgs& a, void* stream, const char** launched) {
+  const dim3 grid = grid_of(a.B, a.c.cap, a.c.Hk);
+  if (a.c.D == 128)
+    hipLaunchKernelGGL(kv_expand_kernel<128>, grid, dim3(kWaves * 64), 0, (hipStream_t)stream, a);
+  else
+    hipLaunchKernelGGL(kv_expand_kernel<64>, grid, dim3(kWaves * 64), 0, (hipStream_t)stream, a);
+  *launched = a.c.D == 128 ? "kv_expand_kernel<128>" : "kv_expand_kernel<64>";
   return (int)hipGetLastError();
 }
 

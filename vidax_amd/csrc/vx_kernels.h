@@ -189,7 +189,8 @@ struct KvWriteArgs {
   int32_t B, S;
 };
 
-// Positions start[b] + t, t < S, of slot slots[b] to contiguous (B, S, Hk, D).
+// Positions start[b] + t, t < S, of slot slots[b] to contiguous (B, S, Hk, D), or
+// (launch_kv_expand) the first limit[b] to (B, Hk, cap, D).
 struct KvReadArgs {
   KvCache c;
   const int32_t* start;
@@ -197,6 +198,9 @@ struct KvReadArgs {
   int32_t B, S;
   void* k_out;
   void* v_out;
+  // launch_kv_expand only
+  const int32_t* limit;  // [B] or nullptr (cap)
+  int32_t* len_out;      // [B] limit, held to the cache
 };
 
 // Attention of q (B, Sq, H, D) over the first kv_len[b] positions of slot
@@ -238,6 +242,7 @@ int launch_key_masks(const KeyMaskArgs& a, void* stream, const char** launched);
 int launch_full_bias(const FullBiasArgs& a, void* stream, const char** launched);
 int launch_kv_write(const KvWriteArgs& a, void* stream, const char** launched);
 int launch_kv_read(const KvReadArgs& a, void* stream, const char** launched);
+int launch_kv_expand(const KvReadArgs& a, void* stream, const char** launched);
 int launch_cached_attn(const CachedAttnArgs& a, void* stream, const char** launched);
 
 // Measurement only: n_groups one-wave workgroups each store (XCD id, HW_ID,

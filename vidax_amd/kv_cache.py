@@ -241,7 +241,8 @@ def _attend(q: torch.Tensor, cache: KVCache, prefix: Optional[KVCache], kv_len, 
         out_strides = _strides3(out)
     if empty:
         return out
-    ws_bytes = _workspace_bytes(index, cap, n_prefix, p_cap, B, Sq, H, Hk, D)
+    ws_bytes = _workspace_bytes(index, cap, n_prefix, p_cap, B, Sq, H, Hk, D,
+                                int(not causal and q_len is None))
     ws = ws_at = None
     if ws_bytes > 0:
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
