@@ -666,7 +666,7 @@ def test_long_cross_attention(gpu, D, slots):
     its head's rows NaN, and an item without a slot or a key gives zeros."""
     print(f"[case] long cross attention D={D} slots={slots}", flush=True)
     rng = np.random.default_rng(31)
-    B, Sq, H, cap, lens = 3, 4100, 3, 192, [150, 192, 0 if slots is None else 33]
+    B, Sq, H, cap, lens = 3, 33400, 3, 192, [150, 192, 0 if slots is None else 33]
     by_slot = np.zeros(3, int)
     for b in range(B):
         slot = b if slots is None else slots[b]
@@ -680,7 +680,7 @@ def test_long_cross_attention(gpu, D, slots):
     kw = dict(slots=_ints(slots, gpu), causal=False)
     got = vx.cached_attention(q, cache, _ints(lens, gpu), **kw)
     assert _lib.last_launch().startswith("flash_")
-    pieces = torch.cat([vx.cached_attention(q[:, i:i + 2050], cache, _ints(lens, gpu), **kw) for i in (0, 2050)], 1)
+    pieces = torch.cat([vx.cached_attention(q[:, i:i + 2050], cache, _ints(lens, gpu), **kw) for i in range(0, Sq, 2050)], 1)
     want_nan = torch.zeros_like(got, dtype=torch.bool)
     want_nan[0, :, 1] = True
     assert torch.equal(got.isnan(), want_nan) and torch.equal(pieces.isnan(), want_nan)

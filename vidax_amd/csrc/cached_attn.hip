@@ -962,7 +962,27 @@ struct Planned {
   int usual_parts = 1;  // of a stream
 };
 
-Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, int D, int64_t slots, bool prefix,
+// Ranges that many_kernel cuts a stream of `tiles` tiles into, `groups` workgroups
+// without a cut: the number for which a model of the time is least. Measured at
+// head dim 128: a tile takes 1.3 us where a CU holds one workgroup and 2.1 us where
+// it holds two; the merging launch takes 6 us; a range's partial results (128 rows
+// of fp32) are written and read at 4 TB/s. (12 heads, 2048 queries: 512 keys in two
+// ranges 37 us, in one 15; a prefix of 4001 and 2900 keys under 1024 rows and 8
+// heads in 2, 4, 6 and 8 ranges 86, 77, 67 and 78 us.)
+int64_t many_ranges(int64_t groups, int64_t tiles, int D, int64_t slots, int64_t cus) {
+  int64_t best = 1;
+  double least = 0;
+  for (int64_t k = 1; k * 2 <= tiles && (k == 1 || groups * k <= slots); ++k) {
+    const double crowded = std::min(1.0, std::max(0.0, (double)(groups * k - cus) / (double)cus));
+    const double per_tile = (1.3 + 0.8 * crowded) * D / 128;
+    const double t = (double)((tiles + k - 1) / k) * per_tile +
+                     (k > 1 ? 6 + 2.0 * (double)(groups * k) * 128 * (D + 2) * 4 / 4e6 : 0);
+    if (k == 1 || t < least) best = k, least = t;
+  }
+  return best;
+}
+
+Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, int D, int64_t slots, int64_t cus, bool prefix,
                   bool with_prefix) {
   Planned h;
   Part& p = h.p;
@@ -975,9 +995,13 @@ Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, int D, in
   const int64_t tile = p.few ? kFewTile : kManyTile;
   const int64_t tiles = (cap + tile - 1) / tile;
   p.min_chunk = p.few ? 4 : 2;
-  if (tiles > (p.few ? kFewWhole : 4) && (p.few || streams * row_tiles * Hk < slots))
-    p.budget = (int)std::min<int64_t>(std::max<int64_t>(slots / (Hk * row_tiles), 1),
-                                      streams * ((tiles + p.min_chunk - 1) / p.min_chunk));
+  if (p.few) {
+    if (tiles > kFewWhole)
+      p.budget = (int)std::min<int64_t>(std::max<int64_t>(slots / Hk, 1), streams * ((tiles + p.min_chunk - 1) / p.min_chunk));
+  } else {
+    const int64_t k = many_ranges(streams * row_tiles * Hk, tiles, D, slots, cus);
+    if (k > 1) p.budget = (int)(k * streams);
+  }
   p.items = p.budget != 0 ? p.budget : streams;
   h.usual_parts = p.budget / streams + 1;
   h.blocks = p.items * row_tiles * Hk;
@@ -994,16 +1018,16 @@ struct Plan {
 };
 
 Plan plan_of(int cap, int n_prefix, int p_cap, int B, int Sq, int H, int Hk, int D) {
-  // workgroups that the device holds at once (256 if it is not known)
-  const int64_t slots = 2 * (int64_t)(device_cu_count() > 0 ? device_cu_count() : 256);
+  const int64_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
+  const int64_t slots = 2 * cus;  // workgroups that the device holds at once
   const int64_t rows = (int64_t)Sq * (H / Hk);
   Plan p;
-  p.own = plan_part(B, rows, 1, cap, Hk, D, slots, false, n_prefix > 0);
+  p.own = plan_part(B, rows, 1, cap, Hk, D, slots, cus, false, n_prefix > 0);
   if (n_prefix == 0) return p;
   const int per = B / n_prefix;
   if (p.own.p.few && (cap + p_cap) / kFewTile <= kFewWhole && (int64_t)B * Hk <= slots) {
     p.both = true;
-    p.own = plan_part(B, rows, 1, cap, Hk, D, slots, false, false);
+    p.own = plan_part(B, rows, 1, cap, Hk, D, slots, cus, false, false);
     p.pre.p.per = per;
     return p;
   }
@@ -1018,10 +1042,10 @@ Plan plan_of(int cap, int n_prefix, int p_cap, int B, int Sq, int H, int Hk, int
   const int64_t w_pre = weight(n_prefix, pre_rows, p_cap), w_own = weight(B, rows, cap);
   int64_t pre_slots = std::max<int64_t>(slots * w_pre / (w_pre + w_own), 1);
   if (p.own.p.budget > 0)
-    p.own = plan_part(B, rows, 1, cap, Hk, D, std::max<int64_t>(slots - pre_slots, 1), false, true);
+    p.own = plan_part(B, rows, 1, cap, Hk, D, std::max<int64_t>(slots - pre_slots, 1), cus, false, true);
   else if (p.own.blocks <= slots / 2)
     pre_slots = slots - p.own.blocks;
-  p.pre = plan_part(n_prefix, pre_rows, per, p_cap, Hk, D, pre_slots, true, true);
+  p.pre = plan_part(n_prefix, pre_rows, per, p_cap, Hk, D, pre_slots, cus, true, true);
   return p;
 }
 

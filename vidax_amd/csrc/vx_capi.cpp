@@ -738,13 +738,19 @@ int32_t cached_sizes_check(int32_t cap, int32_t n_prefix, int32_t p_cap, int32_t
   return VX_OK;
 }
 
-// Non-causal attention of long query sequences over shorter caches of as many
-// heads: the cached keys are expanded to bf16 once (at most twice the queries'
-// bytes) and the flash kernels read them, which hold their rate at short key
-// sequences better than many_kernel (2 x 32760 queries of 40 heads on 512 and 384
-// keys: 852 us without, 725 with the expansion).
-bool cached_attn_expands(int32_t cap, int32_t n_prefix, int32_t Sq, int32_t H, int32_t Hk, bool cross) {
-  return cross && n_prefix == 0 && H == Hk && Sq >= 4096 && cap <= Sq;
+// Non-causal attention of many query rows over shorter caches of as many heads:
+// the cached keys are expanded to bf16 once (at most twice the queries' bytes)
+// and the flash kernels read them, whose large grids lose less to the start and
+// the end of their workgroups than many_kernel's. Expanded / from the cache, us:
+//   40 heads, 32768 queries: 128 keys 179 / 252, 512 385 / 457, 4096 2258 / 2519
+//   40 heads, 8192 queries: 128 keys 57 / 64, 512 113 / 111, 4096 591 / 636
+//   12 heads, 32768 queries: 128 keys 63 / 73, 512 131 / 131, 4096 688 / 763
+//   40 heads, 4096 queries: 128 keys 37 / 36, 512 65 / 60, 4096 334 / 327
+//   12 heads, 8192 queries: 128 keys 25 / 25, 512 44 / 40, 4096 202 / 204
+constexpr int64_t kExpandRows = 300000;
+
+bool cached_attn_expands(int32_t cap, int32_t n_prefix, int32_t B, int32_t Sq, int32_t H, int32_t Hk, bool cross) {
+  return cross && n_prefix == 0 && H == Hk && cap <= Sq && (int64_t)B * H * Sq >= kExpandRows;
 }
 
 int64_t expanded_bytes(int32_t cap, int32_t B, int32_t Hk, int32_t D) { return (int64_t)B * Hk * cap * D * 2; }
@@ -1309,7 +1315,7 @@ int32_t vx_cached_attn_fwd(const void* q, void* out, const int64_t* q_strides, c
                 (long long)need, (long long)(workspace != nullptr ? workspace_bytes : 0));
   a.ws = static_cast<float*>(workspace);
   const char* launched = "";
-  if (cached_attn_expands(a.c.cap, a.prefix.slots, seq_q, num_heads, num_kv_heads, cross)) {
+  if (cached_attn_expands(a.c.cap, a.prefix.slots, batch, seq_q, num_heads, num_kv_heads, cross)) {
     const int64_t bytes = expanded_bytes(a.c.cap, batch, num_kv_heads, head_dim);
     uint8_t* const base = static_cast<uint8_t*>(workspace);
     vx::KvReadArgs x{};
@@ -1346,7 +1352,7 @@ int64_t vx_cached_attn_workspace_size(int32_t capacity, int32_t num_prefixes, in
                                       num_kv_heads, head_dim, &c) != VX_OK)
     return -1;
   ok();
-  if (cached_attn_expands(capacity, num_prefixes, seq_q, num_heads, num_kv_heads, cross != 0))
+  if (cached_attn_expands(capacity, num_prefixes, batch, seq_q, num_heads, num_kv_heads, cross != 0))
     return 2 * expanded_bytes(capacity, batch, num_kv_heads, head_dim) + 4 * (int64_t)batch;
   return vx::cached_attn_workspace(capacity, num_prefixes, prefix_capacity, batch, seq_q, num_heads, num_kv_heads,
                                    head_dim);
