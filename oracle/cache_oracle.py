@@ -1,5 +1,5 @@
 """CPU oracle of the 8-bit key/value cache and the attention over it: the
-definitions in 64 bits (numpy), one batch item, head and query at a time."""
+definitions in 64 bits (numpy)."""
 from __future__ import annotations
 
 import numpy as np
@@ -63,21 +63,28 @@ def cached_attention(q, k, v, kv_len=None, q_len=None, slots=None, causal=True, 
         m = Sq if q_len is None else min(max(int(q_len[b]), 0), Sq)
         n = cap if kv_len is None else min(max(int(kv_len[b]), 0), cap)
         slot = b if slots is None else int(slots[b])
-        for i in range(m):
-            own = min(n, max(n - m + i + 1, 0)) if causal else n
-            if not 0 <= slot < n_slots:
-                own = 0
-            for h in range(H):
-                g = h // (H // Hk)
-                kk, vv = (x[slot, g, :own] if own else np.zeros((0, D)) for x in (k, v))
-                if prefix is not None:
-                    at = b // (B // prefix[0].shape[0])
-                    p = prefix[0].shape[2] if prefix_len is None else min(max(int(prefix_len[at]), 0),
-                                                                          prefix[0].shape[2])
-                    kk, vv = (np.concatenate([x[at, g, :p], y]) for x, y in zip(prefix, (kk, vv)))
-                if len(kk):
-                    s = kk @ q[b, i, h] * scale
-                    w = np.exp(s - s.max())
-                    out[b, i, h] = w @ vv / w.sum()
-                    spread[b, i, h] = w @ np.abs(vv) / w.sum()
+        if not 0 <= slot < n_slots:
+            slot, n = 0, 0
+        p = 0
+        if prefix is not None:
+            at = b // (B // prefix[0].shape[0])
+            p_cap = prefix[0].shape[2]
+            p = p_cap if prefix_len is None else min(max(int(prefix_len[at]), 0), p_cap)
+        if m == 0 or n + p == 0:
+            continue
+        own = np.full(m, n)
+        if causal:  # (held to the keys that there are: those of a slot that is not there are none)
+            length = cap if kv_len is None else min(max(int(kv_len[b]), 0), cap)
+            own = np.minimum(n, np.maximum(length - m + np.arange(m) + 1, 0))
+        seen = np.arange(n + p)[None, :] < (p + own)[:, None]
+        for h in range(H):
+            g = h // (H // Hk)
+            kk, vv = (x[slot, g, :n] for x in (k, v))
+            if p:
+                kk, vv = (np.concatenate([x[at, g, :p], y]) for x, y in zip(prefix, (kk, vv)))
+            s = np.where(seen, q[b, :m, h] @ kk.T * scale, -np.inf)
+            w = np.exp(s - np.maximum(s.max(-1, keepdims=True), -1e300))
+            total = w.sum(-1, keepdims=True)
+            total[total == 0] = 1.0
+            out[b, :m, h], spread[b, :m, h] = w @ vv / total, w @ np.abs(vv) / total
     return out, spread

@@ -5,7 +5,8 @@ bits, on the stored values) under a bound per output value that follows from
 what the kernels round. With o the exact output and A the same weights over
 |v|:
   2^-8 |o|                         the output to bf16
-  2^-8 A                           the weights to bf16 for the product with V
+  2^-8 (A + |o|)                   the weights to bf16: w_j (1 + d_j), |d_j| <= 2^-8, over their own
+                                   sum is off by sum_j w_j d_j (v_j - o) at most
   2 (D + 2) 2^-24 L A              fp32 logits: D products and sums of at most
                                    L = max_j scale sum_d |q_d k_jd| in all; a
                                    logit off by x moves weights by at most 2 x
@@ -351,7 +352,7 @@ def _assert_close(got, q, held, prefix, **kw):
     top = max([np.abs(x[0]).max() for x in (held, prefix) if x is not None and x[0].size] or [0.0])
     L = scale * np.abs(q64).sum(-1).max() * top
     n = held[0].shape[2] + (prefix[0].shape[2] if prefix is not None else 0)
-    tol = 2.0 ** -8 * np.abs(ref) + spread * (2.0 ** -8 + 2 * (D + 2) * 2.0 ** -24 * L + 2 * (n + 64) * 2.0 ** -24)
+    tol = 2 * 2.0 ** -8 * np.abs(ref) + spread * (2.0 ** -8 + 2 * (D + 2) * 2.0 ** -24 * L + 2 * (n + 64) * 2.0 ** -24)
     err = np.abs(got.double().cpu().numpy() - ref)
     assert not np.isnan(err).any()
     at = np.unravel_index(np.argmax(err - tol), err.shape)
@@ -401,6 +402,62 @@ def test_cached_attention(gpu, case):
     torch.cuda.synchronize()
     assert torch.equal(got, again)  # the same bits
     _assert_close(got, q, _held(cache, by_slot), None, **kw)
+
+
+def _lens(rng, B, most):
+    """Lengths from none to the most, a third of them very short."""
+    n = rng.integers(0, most + 1, B)
+    short = rng.random(B) < 0.33
+    n[short] = rng.integers(0, 4, short.sum())
+    n[rng.integers(0, B)] = most
+    return n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Sq,H,Hk,D,cap,causal", [
+    (130, 1, 2, 1, 64, 2048, True),       # more items than a wave has lanes, tiles in ranges
+    (70, 3, 3, 1, 128, 1088, True),
+    (9, 1, 32, 4, 128, 4096, True),
+    (1, 1, 4, 1, 64, 16384, True),        # one long sequence over the whole chip
+    (66, 20, 4, 1, 64, 1536, True),       # the same with more rows than a tile
+    (3, 50, 4, 2, 128, 4096, True),
+    (2, 100, 2, 1, 64, 8192, False),
+    (1, 700, 5, 1, 128, 2048, True),
+])
+def test_ranges_over_many_lengths(gpu, B, Sq, H, Hk, D, cap, causal):
+    """Batches whose tiles are cut into ranges that end inside streams and span
+    empty ones."""
+    print(f"[case] ranges B={B} Sq={Sq} H={H} Hk={Hk} D={D} cap={cap} causal={causal}", flush=True)
+    rng = np.random.default_rng(B + Sq + cap)
+    lens = _lens(rng, B, cap)
+    q_len = rng.integers(0, Sq + 1, B) if Sq > 1 else None
+    cache = _cache_of(rng, B, Hk, cap, D, gpu, lens)
+    q = _bf16(2 * rng.standard_normal((B, Sq, H, D)), gpu)
+    kw = dict(kv_len=lens, q_len=q_len, causal=causal)
+    got = vx.cached_attention(q, cache, **kw)
+    assert torch.equal(got, vx.cached_attention(q, cache, **kw))
+    _assert_close(got, q, _held(cache, lens), None, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Sq,H,Hk,D,groups,p_cap,cap", [
+    (130, 1, 2, 1, 64, 65, 1024, 1088),   # two sharers each, more groups than a wave has lanes
+    (12, 1, 8, 2, 128, 1, 4096, 128),     # 48 rows on one prefix
+    (12, 1, 8, 2, 64, 3, 2048, 2048),     # ranges on both sides
+    (4, 30, 4, 2, 128, 2, 1536, 1536),
+    (64, 1, 1, 1, 128, 64, 128, 64),      # every item a prefix of its own, in one pass
+])
+def test_prefixes_over_many_lengths(gpu, B, Sq, H, Hk, D, groups, p_cap, cap):
+    print(f"[case] prefixes B={B} Sq={Sq} H={H} Hk={Hk} D={D} groups={groups} p_cap={p_cap} cap={cap}", flush=True)
+    rng = np.random.default_rng(B + Sq + p_cap)
+    lens, p_len = _lens(rng, B, cap), _lens(rng, groups, p_cap)
+    q_len = rng.integers(0, Sq + 1, B) if Sq > 1 else None
+    cache, prefix = _cache_of(rng, B, Hk, cap, D, gpu, lens), _cache_of(rng, groups, Hk, p_cap, D, gpu, p_len)
+    q = _bf16(2 * rng.standard_normal((B, Sq, H, D)), gpu)
+    kw = dict(kv_len=lens, prefix_len=p_len, q_len=q_len)
+    got = vx.shared_prefix_attention(q, prefix, cache, **kw)
+    assert torch.equal(got, vx.shared_prefix_attention(q, prefix, cache, **kw))
+    _assert_close(got, q, _held(cache, lens), _held(prefix, p_len), **kw)
 
 
 @pytest.mark.gpu

@@ -972,7 +972,7 @@ struct Planned {
 int64_t many_ranges(int64_t groups, int64_t tiles, int D, int64_t slots, int64_t cus) {
   int64_t best = 1;
   double least = 0;
-  for (int64_t k = 1; k * 2 <= tiles && (k == 1 || groups * k <= slots); ++k) {
+  for (int64_t k = 1; k * 2 <= tiles && (k == 1 || groups * k <= slots); k += 1 + k / 8) {
     const double crowded = std::min(1.0, std::max(0.0, (double)(groups * k - cus) / (double)cus));
     const double per_tile = (1.3 + 0.8 * crowded) * D / 128;
     const double t = (double)((tiles + k - 1) / k) * per_tile +

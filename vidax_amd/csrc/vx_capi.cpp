@@ -1310,6 +1310,7 @@ int32_t vx_cached_attn_fwd(const void* q, void* out, const int64_t* q_strides, c
   const bool cross = causal == 0 && q_len == nullptr;
   const int64_t need = vx_cached_attn_workspace_size(a.c.cap, a.prefix.slots, a.prefix.cap, batch, seq_q, num_heads,
                                                      num_kv_heads, head_dim, cross);
+  if (need < 0) return VX_ERR_INVALID_ARGUMENT;  // (its message)
   if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need))
     return fail(VX_ERR_INVALID_ARGUMENT, "a 16-byte aligned workspace of %lld bytes is needed (%lld given)",
                 (long long)need, (long long)(workspace != nullptr ? workspace_bytes : 0));
