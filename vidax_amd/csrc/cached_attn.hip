@@ -249,7 +249,7 @@ struct FewKeys {
   int bound, all;         // those that this lane's row sees, those that every row does
 };
 
-// A range of tiles of streams of at most 32 rows (BOTH: stream `block`, the
+// A range of tiles of streams, for 32 rows of one kv head (BOTH: stream `block`, the
 // group's prefix in front of its own keys). The waves take every fourth tile.
 template <int D, bool BOTH>
 __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt, const Part* pre, const int block,
@@ -257,12 +257,15 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
   using C = FewCfg<D>;
   using T = Fp8Tile<D>;
   const Streams& s = pt.s;
-  const int rows = pt.rows;
   float(*const ml)[32][2] = (float(*)[32][2])(smem + C::kTiles);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hf = lane >> 5, col = lane & 31;
-  const int Hk = s.c.Hk, kvh = block % Hk, item = block / Hk;
+  // kv heads side by side, then the row tiles: with 8 heads each XCD keeps one
+  // head's keys in its L2 for all of its row tiles
+  const int Hk = s.c.Hk, kvh = block % Hk, n_rt = (pt.rows + 31) / 32;
+  const int item = block / Hk / n_rt, row0 = (block / Hk - item * n_rt) * 32;
+  const int rows = min(pt.rows - row0, 32);
   lds_u8* const ring = (lds_u8*)smem + wave * C::kRing * C::kBuf;
   const uint32_t ring_addr = (uint32_t)(uintptr_t)ring;
   const float c = a.scale * kLog2e;
@@ -272,10 +275,10 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
   const int kkey = (col & 0x13) | ((col & 4) << 1) | ((col & 8) >> 1);
 
   auto keys = [&](const Streams& from, int stream, int len) {
-    const int64_t row0 = ((int64_t)slot_of(from, stream) * Hk + kvh) * from.c.cap;
-    return FewKeys{uniform_u64((uint64_t)(uintptr_t)(from.c.k + row0 * D)),
-                   uniform_u64((uint64_t)(uintptr_t)(from.c.v + row0 * D)),
-                   (lane & 2 ? from.c.vs : from.c.ks) + row0 + 16 * (lane & 1), len, len, len};
+    const int64_t at = ((int64_t)slot_of(from, stream) * Hk + kvh) * from.c.cap;
+    return FewKeys{uniform_u64((uint64_t)(uintptr_t)(from.c.k + at * D)),
+                   uniform_u64((uint64_t)(uintptr_t)(from.c.v + at * D)),
+                   (lane & 2 ? from.c.vs : from.c.ks) + at + 16 * (lane & 1), len, len, len};
   };
   // ---- staging: copy p of a tile fills 1024 / D rows; lane L takes row L / (D / 16),
   // LDS chunk L % (D / 16), which holds the row's chunk with that number XOR the swizzle
@@ -303,7 +306,7 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
 
     const RowMap map{a, stream, kvh, a.H / Hk, pt.per};
     int rb, ri, rh;
-    map.place(min(col, rows - 1), rb, ri, rh);
+    map.place(row0 + min(col, rows - 1), rb, ri, rh);
     bf16x8 q[D / 16];
     {
       const bf16* p = (const bf16*)a.q + rb * a.qs[0] + ri * a.qs[1] + rh * a.qs[2] + hf * 16;
@@ -328,6 +331,7 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
       return __builtin_amdgcn_readfirstlane(x);
     };
     own.all = least(own.bound);
+    const int any = -least(-own.bound);  // keys that some row sees
     if (BOTH) shared.all = least(shared.bound);
 
     f32x16 O[D / 32];
@@ -398,7 +402,7 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
     };
 
     // tile t of the part: the prefix's first, then the stream's own from `first` on
-    const int here = pre_tiles + take;
+    const int here = pre_tiles + max(min(take, tiles_in<kFewTile>(any) - first), 0);
     auto stage_at = [&](int t, int buf) {
       if (BOTH && t < pre_tiles)
         stage(shared, t, buf);
@@ -443,7 +447,7 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
     const bool final_rows = pt.direct && take == tiles;
     float* const part =
         final_rows ? nullptr
-                   : pt.ws + ((int64_t)(pt.budget == 0 ? item : item + stream) * Hk + kvh) * part_floats(rows, D);
+                   : pt.ws + ((int64_t)(pt.budget == 0 ? item : item + stream) * Hk + kvh) * part_floats(pt.rows, D);
     for (int x = threadIdx.x; x < rows * (D / 4); x += kThreads) {
       const int r = x / (D / 4), d = (x % (D / 4)) * 4;
       float M = ml[0][r][0];
@@ -459,17 +463,17 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
       }
       if (final_rows) {
         int b, i, h;
-        map.place(r, b, i, h);
+        map.place(row0 + r, b, i, h);
         const float inv = is_zero(L) ? 0.f : 1.0f / L;
         bf16x4 y;
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = (bf16)(o[e] * inv);
         *(bf16x4*)((bf16*)a.o + b * a.os[0] + i * a.os[1] + h * a.os[2] + d) = y;
       } else {
-        *(f32x4*)(part + r * D + d) = o;
+        *(f32x4*)(part + (int64_t)(row0 + r) * D + d) = o;
         if (d == 0) {
-          part[(int64_t)rows * D + 2 * r] = M;
-          part[(int64_t)rows * D + 2 * r + 1] = L;
+          part[(int64_t)pt.rows * D + 2 * (row0 + r)] = M;
+          part[(int64_t)pt.rows * D + 2 * (row0 + r) + 1] = L;
         }
       }
     }
@@ -966,24 +970,38 @@ struct Planned {
   int usual_parts = 1;  // of a stream
 };
 
-// Ranges that many_kernel cuts a stream of `tiles` tiles into, `groups` workgroups
-// without a cut: the number for which a model of the time is least. Measured at
-// head dim 128: a tile takes 1.3 us where a CU holds one workgroup and 2.1 us where
-// it holds two; the merging launch takes 6 us; a range's partial results (128 rows
-// of fp32) are written and read at 4 TB/s. (12 heads, 2048 queries: 512 keys in two
-// ranges 37 us, in one 15; a prefix of 4001 and 2900 keys under 1024 rows and 8
-// heads in 2, 4, 6 and 8 ranges 86, 77, 67 and 78 us.)
-int64_t many_ranges(int64_t groups, int64_t tiles, int D, int64_t slots, int64_t cus) {
+// Ranges that a stream is cut into, `groups` workgroups without a cut: the number
+// for which a model of the time is least. A workgroup has `steps` steps that take
+// t1 us each where its CU holds no other, t2 where it holds two; the merging launch
+// takes 6 us, and the partial results (rows x D of fp32 per workgroup) are written and
+// read at 4 TB/s. (12 heads, 2048 queries: 512 keys in two ranges 37 us, in one 15; a
+// prefix of 4001 and 2900 keys under 1024 rows and 8 heads in 2, 4, 6 and 8 ranges
+// 86, 77, 67 and 78 us; 8192 keys under 128 rows and 8 heads in 8, 16 and 24 23, 29
+// and 32 us with few_kernel.)
+int64_t best_ranges(int64_t groups, int64_t steps, double t1, double t2, int64_t rows, int D, int64_t slots,
+                    int64_t cus) {
   int64_t best = 1;
   double least = 0;
-  for (int64_t k = 1; k * 2 <= tiles && (k == 1 || groups * k <= slots); k += 1 + k / 8) {
+  for (int64_t k = 1; k * 2 <= steps && (k == 1 || groups * k <= slots); k += 1 + k / 8) {
     const double crowded = std::min(1.0, std::max(0.0, (double)(groups * k - cus) / (double)cus));
-    const double per_tile = (1.3 + 0.8 * crowded) * D / 128;
-    const double t = (double)((tiles + k - 1) / k) * per_tile +
-                     (k > 1 ? 6 + 2.0 * (double)(groups * k) * 128 * (D + 2) * 4 / 4e6 : 0);
+    const double t = (double)((steps + k - 1) / k) * (t1 + (t2 - t1) * crowded) * D / 128 +
+                     (k > 1 ? 6 + 2.0 * (double)(groups * k) * (double)rows * (D + 2) * 4 / 4e6 : 0);
     if (k == 1 || t < least) best = k, least = t;
   }
   return best;
+}
+
+// Whether few_kernel takes rows so many. In the time that a CU takes for a tile of
+// 64 keys and 128 rows with many_kernel (1.05 us with two workgroups, head dim
+// 128), it takes ten 32 x 32 tiles with few_kernel (1.65 us for eight waves'): 2.5
+// row tiles. So up to 64 rows and a little past each 128 few_kernel wins whatever
+// the length; at 128 rows while its shorter start and fewer partial results (about
+// 5 us) outweigh that (32 sharers' 128 rows on 8192 keys of 8 heads 22.7 us, with
+// many_kernel 25.7; 1024 rows on 4001 keys 67 and 60; 4000 rows on 5003 210 and 139).
+bool runs_few(int64_t heads, int64_t rows, int64_t cap, int D, int64_t cus) {
+  if (rows <= 32) return true;
+  const double x = (double)(heads * ((cap + kManyTile - 1) / kManyTile)) / (double)cus * D / 128;
+  return 0.4125 * (double)((rows + 31) / 32) * x < 1.05 * (double)((rows + kManyRows - 1) / kManyRows) * x + 5;
 }
 
 Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, int D, int64_t slots, int64_t cus, bool prefix,
@@ -992,18 +1010,21 @@ Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, int D, in
   Part& p = h.p;
   p.rows = (int)rows;
   p.per = per;
-  p.few = rows <= 32;
+  p.few = runs_few(streams * (int64_t)Hk, rows, cap, D, cus);
   p.prefix = prefix;
   p.direct = !with_prefix;
-  const int64_t row_tiles = p.few ? 1 : (rows + kManyRows - 1) / kManyRows;
+  const int64_t row_tiles = p.few ? (rows + 31) / 32 : (rows + kManyRows - 1) / kManyRows;
   const int64_t tile = p.few ? kFewTile : kManyTile;
-  const int64_t tiles = (cap + tile - 1) / tile;
+  const int64_t tiles = (cap + tile - 1) / tile, groups = streams * row_tiles * Hk;
   p.min_chunk = p.few ? 4 : 2;
-  if (p.few) {
+  if (p.few && row_tiles == 1) {
+    // (partial results of few rows: as many ranges as find a place)
     if (tiles > kFewWhole)
-      p.budget = (int)std::min<int64_t>(std::max<int64_t>(slots / Hk, 1), streams * ((tiles + p.min_chunk - 1) / p.min_chunk));
+      p.budget = (int)std::min<int64_t>(std::max<int64_t>(slots / Hk, 1),
+                                        streams * ((tiles + p.min_chunk - 1) / p.min_chunk));
   } else {
-    const int64_t k = many_ranges(streams * row_tiles * Hk, tiles, D, slots, cus);
+    const int64_t k = p.few ? best_ranges(groups, (tiles + kWaves - 1) / kWaves, 0.9, 1.65, 32, D, slots, cus)
+                            : best_ranges(groups, tiles, 1.3, 2.1, kManyRows, D, slots, cus);
     if (k > 1) p.budget = (int)(k * streams);
   }
   p.items = p.budget != 0 ? p.budget : streams;
@@ -1029,7 +1050,7 @@ Plan plan_of(int cap, int n_prefix, int p_cap, int B, int Sq, int H, int Hk, int
   p.own = plan_part(B, rows, 1, cap, Hk, D, slots, cus, false, n_prefix > 0);
   if (n_prefix == 0) return p;
   const int per = B / n_prefix;
-  if (p.own.p.few && (cap + p_cap) / kFewTile <= kFewWhole && (int64_t)B * Hk <= slots) {
+  if (rows <= 32 && (cap + p_cap) / kFewTile <= kFewWhole && (int64_t)B * Hk <= slots) {
     p.both = true;
     p.own = plan_part(B, rows, 1, cap, Hk, D, slots, cus, false, false);
     p.pre.p.per = per;
@@ -1075,7 +1096,7 @@ int launch(const CachedAttnArgs& a, hipStream_t st, const char** launched) {
       hipLaunchKernelGGL(many_kernel<D>, grid, threads, 0, st, a, own);
     *launched = own.few ? (D == 128 ? "few_kernel<128, false>" : "few_kernel<64, false>")
                         : (D == 128 ? "many_kernel<128>" : "many_kernel<64>");
-  } else if (pre.few) {  // (a prefix's streams have no fewer rows than the items')
+  } else if (pre.few && own.few) {
     hipLaunchKernelGGL((prefix_kernel<D, true, true>), grid, threads, 0, st, a, pre, own, pre_blocks);
     *launched = D == 128 ? "prefix_kernel<128, true, true>" : "prefix_kernel<64, true, true>";
   } else if (own.few) {
