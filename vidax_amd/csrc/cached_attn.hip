@@ -228,7 +228,7 @@ struct Fp8Tile {
 // ------------------------------------------------------------------ few rows
 constexpr int kFewTile = 32;  // keys per tile of few_kernel
 
-template <int D>
+template <int D, int W>
 struct FewCfg {
   static constexpr int kTileBytes = kFewTile * D;        // of K, and of V
   static constexpr int kCopies = kTileBytes / 1024;      // DMA copies of each
@@ -237,8 +237,8 @@ struct FewCfg {
   static constexpr int kRing = 2;
   static constexpr int kOutRow = D + 4;                  // fp32 values between rows of the exchange
   static constexpr int kExchange = 32 * kOutRow * 4;
-  static constexpr int kTiles = (kRing * kBuf > kExchange ? kRing * kBuf : kExchange) * kWaves;
-  static constexpr int kSmem = kTiles + kWaves * 32 * 8;  // then (reference point, sum) of the waves' rows
+  static constexpr int kTiles = (kRing * kBuf > kExchange ? kRing * kBuf : kExchange) * W;
+  static constexpr int kSmem = kTiles + W * 32 * 8;  // then (reference point, sum) of the waves' rows
 };
 
 // Keys of one kv head as few_part reads them.
@@ -250,11 +250,11 @@ struct FewKeys {
 };
 
 // A range of tiles of streams, for 32 rows of one kv head (BOTH: stream `block`, the
-// group's prefix in front of its own keys). The waves take every fourth tile.
-template <int D, bool BOTH>
+// group's prefix in front of its own keys). The W waves take every W-th tile.
+template <int D, int W, bool BOTH>
 __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt, const Part* pre, const int block,
                                          unsigned char* smem) {
-  using C = FewCfg<D>;
+  using C = FewCfg<D, W>;
   using T = Fp8Tile<D>;
   const Streams& s = pt.s;
   float(*const ml)[32][2] = (float(*)[32][2])(smem + C::kTiles);
@@ -409,25 +409,25 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
       else
         stage(own, first + t - pre_tiles, buf);
     };
-    const int n = here > wave ? (here - wave + kWaves - 1) / kWaves : 0;  // this wave's tiles
+    const int n = here > wave ? (here - wave + W - 1) / W : 0;  // this wave's tiles
     if (n > 0) stage_at(wave, 0);
-    if (n > 1) stage_at(wave + kWaves, 1);
+    if (n > 1) stage_at(wave + W, 1);
     for (int it = 0; it < n; ++it) {
       if (it + 1 < n)
         wait_copies<C::kPerTile>();
       else
         wait_copies<0>();
-      const int t = wave + it * kWaves;
+      const int t = wave + it * W;
       const bool of_prefix = BOTH && t < pre_tiles;
       step((of_prefix ? t : first + t - pre_tiles) * kFewTile, of_prefix ? shared.bound : own.bound,
            of_prefix ? shared.all : own.all, it & 1);
       if (it + 2 < n) {
         wait_lds_reads();
-        stage_at(t + 2 * kWaves, it & 1);
+        stage_at(t + 2 * W, it & 1);
       }
     }
 
-    // ---- the four waves' results: rows x D through LDS, then D / 4 lanes per row
+    // ---- the waves' results: rows x D through LDS, then D / 4 lanes per row
     __syncthreads();
     VX_LDS float* const xo = (VX_LDS float*)((lds_u8*)smem + wave * C::kExchange);
     const float lsum = halves_sum(l);
@@ -448,15 +448,15 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
     float* const part =
         final_rows ? nullptr
                    : pt.ws + ((int64_t)(pt.budget == 0 ? item : item + stream) * Hk + kvh) * part_floats(pt.rows, D);
-    for (int x = threadIdx.x; x < rows * (D / 4); x += kThreads) {
+    for (int x = threadIdx.x; x < rows * (D / 4); x += W * 64) {
       const int r = x / (D / 4), d = (x % (D / 4)) * 4;
       float M = ml[0][r][0];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) M = fmaxf(M, ml[w][r][0]);
+      for (int w = 1; w < W; ++w) M = fmaxf(M, ml[w][r][0]);
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
       float L = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
+      for (int w = 0; w < W; ++w) {
         const float al = fast_exp2(ml[w][r][0] - M);
         L += ml[w][r][1] * al;
         o += *(const VX_LDS f32x4*)((lds_u8*)smem + w * C::kExchange + (r * C::kOutRow + d) * 4) * al;
@@ -851,11 +851,12 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
 }
 
 // BOTH: prefixes and items of few positions in one pass, the prefix read (from
-// the L2) by each item rather than merged.
-template <int D, bool BOTH>
-__global__ __launch_bounds__(kThreads, 2) void few_kernel(const CachedAttnArgs a, const Part own, const Part pre) {
-  __shared__ __attribute__((aligned(256))) unsigned char smem[FewCfg<D>::kSmem];
-  few_part<D, BOTH>(a, own, &pre, blockIdx.x, smem);
+// the L2) by each item rather than merged. W: eight waves where the grid leaves a
+// CU to each workgroup.
+template <int D, int W, bool BOTH>
+__global__ __launch_bounds__(W * 64, 2) void few_kernel(const CachedAttnArgs a, const Part own, const Part pre) {
+  __shared__ __attribute__((aligned(256))) unsigned char smem[FewCfg<D, W>::kSmem];
+  few_part<D, W, BOTH>(a, own, &pre, blockIdx.x, smem);
 }
 
 template <int D>
@@ -869,18 +870,18 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const CachedAttnArgs 
 template <int D, bool PRE_FEW, bool OWN_FEW>
 __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(const CachedAttnArgs a, const Part pre, const Part own,
                                                            const int pre_blocks) {
-  constexpr int kFew = FewCfg<D>::kSmem, kMany = ManyCfg<D, kWaves>::kSmem;
+  constexpr int kFew = FewCfg<D, kWaves>::kSmem, kMany = ManyCfg<D, kWaves>::kSmem;
   constexpr int kPre = PRE_FEW ? kFew : kMany, kOwn = OWN_FEW ? kFew : kMany;
   __shared__ __attribute__((aligned(256))) unsigned char smem[kPre > kOwn ? kPre : kOwn];
   const int block = blockIdx.x;
   if (block < pre_blocks) {
     if constexpr (PRE_FEW)
-      few_part<D, false>(a, pre, nullptr, block, smem);
+      few_part<D, kWaves, false>(a, pre, nullptr, block, smem);
     else
       many_part<D, kWaves>(a, pre, block, smem);
   } else {
     if constexpr (OWN_FEW)
-      few_part<D, false>(a, own, nullptr, block - pre_blocks, smem);
+      few_part<D, kWaves, false>(a, own, nullptr, block - pre_blocks, smem);
     else
       many_part<D, kWaves>(a, own, block - pre_blocks, smem);
   }
@@ -1039,7 +1040,8 @@ Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, int D, in
 
 struct Plan {
   Planned own, pre;
-  bool both = false;  // few_kernel<D, true>
+  bool both = false;  // few_kernel<D, W, true>
+  bool wide = false;  // few_kernel's W: 8, else 4
 };
 
 Plan plan_of(int cap, int n_prefix, int p_cap, int B, int Sq, int H, int Hk, int D) {
@@ -1048,6 +1050,11 @@ Plan plan_of(int cap, int n_prefix, int p_cap, int B, int Sq, int H, int Hk, int
   const int64_t rows = (int64_t)Sq * (H / Hk);
   Plan p;
   p.own = plan_part(B, rows, 1, cap, Hk, D, slots, cus, false, n_prefix > 0);
+  // Eight waves where each workgroup has a CU to itself and its waves several tiles
+  // (8 / 4 waves: 12 heads, 700 keys 10.2 / 10.6 us; 16 items of 8 queries and 64
+  // heads on 4096 keys 38 / 44; 8 of 40 queries on 1500 keys of 8 heads 17.3 / 18.7)
+  const int64_t few_tiles = ((int64_t)cap + (n_prefix > 0 ? p_cap : 0)) / kFewTile;
+  p.wide = p.own.p.few && p.own.blocks <= cus && p.own.p.budget == 0 && few_tiles > kWaves;
   if (n_prefix == 0) return p;
   const int per = B / n_prefix;
   if (rows <= 32 && (cap + p_cap) / kFewTile <= kFewWhole && (int64_t)B * Hk <= slots) {
@@ -1086,16 +1093,25 @@ int launch(const CachedAttnArgs& a, hipStream_t st, const char** launched) {
   pre.ws = a.ws + pl.own.floats;
   const dim3 grid((unsigned)(pl.pre.blocks + pl.own.blocks)), threads(kThreads);
   const int pre_blocks = (int)pl.pre.blocks;
+  const bool wide = pl.wide;
+  const dim3 few_threads(wide ? 512 : 256);
   if (pl.both) {
-    hipLaunchKernelGGL((few_kernel<D, true>), grid, threads, 0, st, a, own, pre);
-    *launched = D == 128 ? "few_kernel<128, true>" : "few_kernel<64, true>";
-  } else if (n_prefix == 0) {
-    if (own.few)
-      hipLaunchKernelGGL((few_kernel<D, false>), grid, threads, 0, st, a, own, pre);
+    if (wide)
+      hipLaunchKernelGGL((few_kernel<D, 8, true>), grid, few_threads, 0, st, a, own, pre);
     else
-      hipLaunchKernelGGL(many_kernel<D>, grid, threads, 0, st, a, own);
-    *launched = own.few ? (D == 128 ? "few_kernel<128, false>" : "few_kernel<64, false>")
-                        : (D == 128 ? "many_kernel<128>" : "many_kernel<64>");
+      hipLaunchKernelGGL((few_kernel<D, 4, true>), grid, few_threads, 0, st, a, own, pre);
+    *launched = wide ? (D == 128 ? "few_kernel<128, 8, true>" : "few_kernel<64, 8, true>")
+                     : (D == 128 ? "few_kernel<128, 4, true>" : "few_kernel<64, 4, true>");
+  } else if (n_prefix == 0 && own.few) {
+    if (wide)
+      hipLaunchKernelGGL((few_kernel<D, 8, false>), grid, few_threads, 0, st, a, own, pre);
+    else
+      hipLaunchKernelGGL((few_kernel<D, 4, false>), grid, few_threads, 0, st, a, own, pre);
+    *launched = wide ? (D == 128 ? "few_kernel<128, 8, false>" : "few_kernel<64, 8, false>")
+                     : (D == 128 ? "few_kernel<128, 4, false>" : "few_kernel<64, 4, false>");
+  } else if (n_prefix == 0) {
+    hipLaunchKernelGGL(many_kernel<D>, grid, threads, 0, st, a, own);
+    *launched = D == 128 ? "many_kernel<128>" : "many_kernel<64>";
   } else if (pre.few && own.few) {
     hipLaunchKernelGGL((prefix_kernel<D, true, true>), grid, threads, 0, st, a, pre, own, pre_blocks);
     *launched = D == 128 ? "prefix_kernel<128, true, true>" : "prefix_kernel<64, true, true>";
