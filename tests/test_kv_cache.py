@@ -446,6 +446,8 @@ def test_ranges_over_many_lengths(gpu, B, Sq, H, Hk, D, cap, causal):
     (12, 1, 8, 2, 64, 3, 2048, 2048),     # ranges on both sides
     (4, 30, 4, 2, 128, 2, 1536, 1536),
     (64, 1, 1, 1, 128, 64, 128, 64),      # every item a prefix of its own, in one pass
+    (2, 600, 8, 8, 128, 2, 64, 2048),     # a short prefix in front of long prompts
+    (2, 300, 4, 4, 64, 1, 4096, 320),     # the other way
 ])
 def test_prefixes_over_many_lengths(gpu, B, Sq, H, Hk, D, groups, p_cap, cap):
     print(f"[case] prefixes B={B} Sq={Sq} H={H} Hk={Hk} D={D} groups={groups} p_cap={p_cap} cap={cap}", flush=True)
