@@ -9,8 +9,10 @@
  * A row of head_dim values with scale byte s stands for value * 2^(s - 127); s
  * is the smallest byte >= 1 for which the row's largest magnitude is at most
  * 448 * 2^(s - 127), so a stored value is off by at most 2^-4 of itself, or
- * 2^-10 of the scale where it is below 2^-6 of it. A row that holds a NaN or an infinity has
- * scale byte 255 and reads as NaN; no other byte stands for one.
+ * 2^-10 of the scale where it is below 2^-6 of it. A row that holds a NaN or an
+ * infinity has zeros and scale byte 255, and reads as NaN; no other byte stands for
+ * one. (Rows from elsewhere: no value byte within a length may be e4m3's NaN, 0x7f
+ * or 0xff, and the value bytes of a row of scale 255 are zeros.)
  * capacity is a multiple of 64, head_dim 64 or 128.
  *
  * Lengths, positions and slots are device arrays, so that a captured graph can
@@ -93,6 +95,8 @@ int32_t vx_kv_read_check(const void* cache_k, const void* cache_v, const uint8_t
  *   workspace     vx_cached_attn_workspace_size() bytes of device memory,
  *                 16-byte aligned, untouched until the work on `stream` has
  *                 finished; calls that overlap need workspaces of their own
+ * A weight is at most 2^8 before the division by the sum, and is multiplied by its
+ * value row's scale in bf16's range: values from 2^-100 to 2^100 keep their precision.
  * A query without a visible key gives zeros. A key or value row of scale 255
  * makes NaN the outputs of exactly those queries of its head that see it.
  */

@@ -128,6 +128,22 @@ def test_checks_refuse(check, kw, code, frag):
     assert frag in _lib.last_error()
 
 
+@pytest.mark.parametrize("check,fits,refused", [
+    (_write_check, dict(S=2 ** 21, Hk=511), dict(S=2 ** 21, Hk=512)),
+    (_read_check, dict(S=2 ** 21, Hk=511), dict(S=2 ** 21, Hk=512)),
+    # 65535 items of one query: a tile per item and head
+    (_attn_check, dict(B=65535, S=1, H=255, Hk=255, slots=A), dict(B=65535, S=1, H=256, Hk=256, slots=A)),
+    (_attn_check, dict(B=1, S=2 ** 22, H=127, Hk=127), dict(B=1, S=2 ** 22, H=128, Hk=128)),
+    # (a prefix's tiles beside the items' own; its merge's rows)
+    (_attn_check, dict(PREFIX, B=2, p_n=2, S=2 ** 21, H=63, Hk=63), dict(PREFIX, B=2, p_n=2, S=2 ** 21, H=64, Hk=64)),
+    (_attn_check, dict(PREFIX, B=1, p_n=1, S=2 ** 21, H=63, Hk=63), dict(PREFIX, B=1, p_n=1, S=2 ** 21, H=64, Hk=64)),
+])
+def test_checks_refuse_grids_past_32_bits(check, fits, refused):
+    """The threads of a launch, 64 for 16 positions and 256 for 32 rows, are counted in 32 bits."""
+    assert check(**fits) == _lib.VX_OK, _lib.last_error()
+    assert check(**refused) == UNSUPPORTED and "too" in _lib.last_error()
+
+
 def test_injected_error_is_reported():
     L = _lib.lib()
     L.vx_debug_inject_error(_lib.VX_ERR_LAUNCH)

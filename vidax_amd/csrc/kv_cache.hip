@@ -14,6 +14,10 @@
 // cache's. A wave takes 16 positions of one head, keys and values (all its loads
 // in flight before the first is used), and neighbouring waves neighbouring
 // heads, whose bf16 rows lie side by side.
+// Measured: 32760 positions of 40 heads of 128 read in 219 to 248 us (4.1 to 4.6 TB/s;
+// a copy of 1 GiB runs at 4.8), 7800 of 12 heads written in 13 us and read back in 15
+// (partly from cache). Not kept: non-temporal stores (32760 positions 248 -> 363
+// us), 32 positions per wave (248 -> 235 us, 512 positions 8.5 -> 9.1).
 #include "vx_fp8_cache.hpp"
 #include "vx_kernels.h"
 

@@ -672,7 +672,8 @@ int32_t cache_batch_check(const int32_t* i0, const int32_t* i1, const int32_t* s
 }
 
 int32_t kv_grid_check(int32_t S, int32_t Hk) {
-  if (((int64_t)S + vx::kKvTokensPerWave - 1) / vx::kKvTokensPerWave * Hk > INT32_MAX)
+  // (a grid's threads, 64 a wave, are counted in 32 bits)
+  if (((int64_t)S + vx::kKvTokensPerWave - 1) / vx::kKvTokensPerWave * Hk > (INT32_MAX >> 5) - 4)
     return fail(VX_ERR_UNSUPPORTED, "seq (%d) times num_kv_heads (%d) is too large", S, Hk);
   return ok();
 }
@@ -717,9 +718,10 @@ int32_t kv_read_check(const void* ck, const void* cv, const uint8_t* cks, const 
   return kv_grid_check(S, Hk);
 }
 
-// Query rows that share a cached head, tiles of them and an item's rows are
-// held in 31 bits by the kernels and their grids.
-constexpr int64_t kMaxSharedRows = 1 << 30;
+// A grid's threads are counted in 32 bits, 256 to a workgroup. A workgroup takes 32
+// rows of a cached head at least (ranges of few rows: a few workgroups per CU), one
+// of a merge behind a prefix eight.
+constexpr int64_t kMaxWorkgroups = (1 << 24) - 4096;
 
 int32_t cached_sizes_check(int32_t cap, int32_t n_prefix, int32_t p_cap, int32_t B, int32_t Sq, int32_t H, int32_t Hk) {
   if (B < 1 || B > 65535) return fail(VX_ERR_INVALID_ARGUMENT, "batch (%d) must be in 1..65535", B);
@@ -730,10 +732,10 @@ int32_t cached_sizes_check(int32_t cap, int32_t n_prefix, int32_t p_cap, int32_t
   if (n_prefix < 0 || (n_prefix > 0 && B % n_prefix != 0))
     return fail(VX_ERR_INVALID_ARGUMENT, "batch (%d) must be a multiple of num_prefixes (%d)", B, n_prefix);
   const int64_t rows = (int64_t)Sq * (H / Hk), sharers = n_prefix > 0 ? B / n_prefix : 1;
-  if (rows > kMaxSharedRows || sharers * rows > kMaxSharedRows || (rows + 127) / 128 * B > kMaxSharedRows / 4 / Hk ||
-      (int64_t)H * Sq > 4 * kMaxSharedRows)
+  const int64_t row_tiles = ((rows + 31) / 32 * B + (sharers * rows + 31) / 32 * n_prefix) * Hk;
+  if (row_tiles > kMaxWorkgroups || (n_prefix > 0 && (int64_t)H * Sq > 8 * kMaxWorkgroups))
     return fail(VX_ERR_UNSUPPORTED, "%d queries of %d heads for %d items are too many", Sq, H, B);
-  if ((int64_t)B * (cap / 32 + 1) > 2 * kMaxSharedRows - 1 || (int64_t)n_prefix * (p_cap / 32 + 1) > 2 * kMaxSharedRows - 1)
+  if ((int64_t)B * (cap / 32 + 1) > INT32_MAX || (int64_t)n_prefix * (p_cap / 32 + 1) > INT32_MAX)
     return fail(VX_ERR_UNSUPPORTED, "%d items of up to %d positions are too many", B, cap);
   return VX_OK;
 }
