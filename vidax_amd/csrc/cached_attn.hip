@@ -22,7 +22,7 @@
 // barrier in the loop), and converts them behind the LDS reads: K with its scale in
 // the same instruction, V unscaled, its scales multiplied into the weights, since
 // the transposed read gives a lane eight keys of one dim. It is bound by memory for
-// single tokens: 64 sequences of 150 to 8192 keys, 8 kv heads, 562 MB in 107 us (5.2
+// single tokens: 64 sequences of 227 to 8192 keys, 8 kv heads, 562 MB in 107 us (5.2
 // TB/s); two of 131000 and 105009 keys 488 MB in 89 us (5.5 TB/s).
 // many_part converts each 64-key tile once for its four waves, on the way to LDS,
 // and runs the matrix cores of a tile beside the next one's softmax and conversions:
@@ -983,8 +983,8 @@ struct Planned {
 // t1 us each where its CU holds no other, t2 where it holds two; the merging launch
 // takes 6 us, and the partial results (rows x D of fp32 per workgroup) are written and
 // read at 4 TB/s. (12 heads, 2048 queries: 512 keys in two ranges 37 us, in one 15; a
-// prefix of 4001 and 2900 keys under 1024 rows and 8 heads in 2, 4, 6 and 8 ranges
-// 86, 77, 67 and 78 us; 8192 keys under 128 rows and 8 heads in 8, 16 and 24 23, 29
+// prefix of 4001 and 3520 keys under 1024 rows and 8 heads in 2, 4, 6 and 8 ranges
+// 86, 60, 66 and 69 us; 8192 keys under 128 rows and 8 heads in 8, 16 and 24 23, 29
 // and 32 us with few_kernel.)
 int64_t best_ranges(int64_t groups, int64_t steps, double t1, double t2, int64_t rows, int D, int64_t slots,
                     int64_t cus) {
