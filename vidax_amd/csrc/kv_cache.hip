@@ -17,7 +17,8 @@
 // Measured: 32760 positions of 40 heads of 128 read in 219 to 248 us (4.1 to 4.6 TB/s;
 // a copy of 1 GiB runs at 4.8), 7800 of 12 heads written in 13 us and read back in 15
 // (partly from cache). Not kept: non-temporal stores (32760 positions 248 -> 363
-// us), 32 positions per wave (248 -> 235 us, 512 positions 8.5 -> 9.1).
+// us), 32 or 64 positions per wave (40 heads of 128: 512 positions 8.5, 9.1 and 9.1 us,
+// 8192 41, 42 and 39, 32768 249, 236 and 238; 16 heads of 64, 32768 33.6, 34.7 and 41.7).
 #include "vx_fp8_cache.hpp"
 #include "vx_kernels.h"
 
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(kWaves * 64) void kv_expand_kernel(const KvReadArgs
 static_assert(64 % kTokens == 0, "a capacity, a multiple of 64, is one of kTokens");
 
 dim3 grid_of(int B, int S, int Hk) {
-  const int64_t waves = ((int64_t)S + kTokens - 1) / kTokens * Hk;  // < 2^31 (checked by the C ABI)
+  const int64_t waves = ((int64_t)S + kTokens - 1) / kTokens * Hk;  // < 2^26 (checked by the C ABI)
   return dim3((unsigned)((waves + kWaves - 1) / kWaves), (unsigned)B);
 }
 
