@@ -144,6 +144,15 @@ def test_checks_refuse_grids_past_32_bits(check, fits, refused):
     assert check(**refused) == UNSUPPORTED and "too" in _lib.last_error()
 
 
+@pytest.mark.parametrize("cap,p_cap", [(64, 2 ** 31 - 64), (2 ** 31 - 64, 64), (2 ** 30, 2 ** 30), (1024, 64)])
+def test_capacities_whose_sum_passes_32_bits_are_long(cap, p_cap):
+    """A prefix and items of more than 1024 positions together are cut into parts, which need a workspace;
+    shorter ones take one pass without any."""
+    size = _lib.lib().vx_cached_attn_workspace_size
+    assert size(cap, 1, p_cap, 1, 1, 1, 1, 64, 0) > 0
+    assert size(960, 1, 64, 1, 1, 1, 1, 64, 0) == 0
+
+
 def test_injected_error_is_reported():
     L = _lib.lib()
     L.vx_debug_inject_error(_lib.VX_ERR_LAUNCH)

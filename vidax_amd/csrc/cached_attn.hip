@@ -1064,7 +1064,8 @@ Plan plan_of(int cap, int n_prefix, int p_cap, int B, int Sq, int H, int Hk, int
   p.wide = p.own.p.few && p.own.blocks <= cus && p.own.p.budget == 0 && few_tiles > kWaves;
   if (n_prefix == 0) return p;
   const int per = B / n_prefix;
-  if (rows <= 32 && (cap + p_cap) / kFewTile <= kFewWhole && (int64_t)B * Hk <= slots) {
+  // (each item then reads its group's whole prefix: streams that are not cut)
+  if (rows <= 32 && few_tiles <= kFewWhole && (int64_t)B * Hk <= slots) {
     p.both = true;
     p.own = plan_part(B, rows, 1, cap, Hk, D, slots, cus, false, false);
     p.pre.p.per = per;
