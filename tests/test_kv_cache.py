@@ -183,6 +183,25 @@ def test_python_refusals_on_the_host():
     assert vx.create_kv_cache(2, 65, 3, 128, device="cpu").k.shape == (2, 3, 128, 128)
 
 
+@pytest.mark.parametrize("make", [tuple, list, lambda c: c._replace(v_scale=None), lambda c: c[:3], lambda c: None])
+def test_what_is_no_cache_is_refused(make):
+    c = vx.create_kv_cache(1, 64, 1, 64, device="cpu")
+    q = torch.zeros((1, 1, 1, 64), dtype=torch.bfloat16)
+    for call, name in ((lambda x: vx.kv_cache_write(x, q, q), "cache"), (lambda x: vx.kv_cache_read(x, 1), "cache"),
+                       (lambda x: vx.cached_attention(q, x), "cache"),
+                       (lambda x: vx.shared_prefix_attention(q, c, x), "cache")):
+        with pytest.raises(TypeError, match=f"{name} must be a KVCache"):
+            call(make(c))
+
+
+@pytest.mark.gpu
+def test_a_plain_tuple_is_no_prefix(gpu):
+    c = vx.create_kv_cache(1, 64, 1, 64, device=gpu)
+    q = torch.zeros((1, 1, 1, 64), dtype=torch.bfloat16, device=gpu)
+    with pytest.raises(TypeError, match="prefix must be a KVCache"):
+        vx.shared_prefix_attention(q, tuple(c), c)
+
+
 def test_oracle_rounding():
     """The oracle's rows against torch's conversion of the same scaled values."""
     rng = np.random.default_rng(1)

@@ -63,6 +63,8 @@ def create_kv_cache(num_slots: int, capacity: int, num_kv_heads: int, head_dim: 
 def _check_cache(cache: KVCache, name: str) -> Tuple[int, int, int, int, int]:
     """(slots, num_kv_heads, capacity, head_dim, device index) of a cache whose
     tensors go together (the C ABI checks sizes and alignment)."""
+    if not isinstance(cache, KVCache):
+        raise TypeError(f"{name} must be a KVCache")
     try:
         k, v, ks, vs = cache
         shape = k.shape
@@ -76,8 +78,8 @@ def _check_cache(cache: KVCache, name: str) -> Tuple[int, int, int, int, int]:
     except (AttributeError, TypeError, ValueError):
         pass
     # what is wrong
-    if not isinstance(cache, tuple) or len(cache) != 4 or not all(isinstance(t, torch.Tensor) for t in cache):
-        raise TypeError(f"{name} must be a KVCache")
+    if not all(isinstance(t, torch.Tensor) for t in cache):
+        raise TypeError(f"{name} must be a KVCache of four tensors")
     parts = tuple(zip(("k", "v", "k_scale", "v_scale"), cache, (_E4M3, _E4M3, _E8M0, _E8M0), (4, 4, 3, 3)))
     k = cache[0]
     for part, t, dtype, dims in parts:
