@@ -721,6 +721,75 @@ def test_graph_replays_follow_the_lengths(gpu):
             assert all(torch.equal(o, e) for o, e in zip(out, ref))
 
 
+def _step_with_host_integers(cache, x, host):
+    """Every operator once, its integers on the host."""
+    vx.kv_cache_write(cache, x, x, host([3, 9]), num=host([1, 1]), slots=host([1, 0]))
+    return (*vx.kv_cache_read(cache, 64, slots=host([1, 0])), vx.cached_attention(x, cache, host([4, 20])),
+            vx.shared_prefix_attention(x, cache, cache, host([20, 4]), prefix_len=host([7, 8]), q_len=host([1, 0])))
+
+
+HOST = {"list": list, "numpy": np.array, "tensor": torch.tensor, "int32": lambda v: torch.tensor(v, dtype=torch.int32),
+        "pinned": lambda v: torch.tensor(v, dtype=torch.int32).pin_memory()}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("host", HOST.values(), ids=list(HOST))
+def test_host_integers_wait_for_nothing(gpu, host):
+    """Calls whose lengths, positions and slots are host values return while the
+    stream is still at work, and give what device tensors give; the caller may
+    change its values as soon as the call returns."""
+    g = torch.Generator(device=gpu).manual_seed(12)
+    x = torch.randn((2, 1, 2, 64), generator=g, device=gpu).bfloat16()
+    caches = [vx.create_kv_cache(2, 64, 2, 64, device=gpu) for _ in range(3)]
+    work = torch.randn((8192, 8192), generator=g, device=gpu).bfloat16()
+    want = _step_with_host_integers(caches[0], x, lambda v: _ints(v, gpu))
+    made = []
+
+    def given(v):
+        made.append(host(v))
+        return made[-1]
+
+    for c in caches[1:]:  # (the first round may still allocate)
+        torch.cuda.synchronize()
+        for _ in range(40):  # about 35 ms
+            torch.matmul(work, work)
+        busy = torch.cuda.Event()
+        busy.record()
+        got = _step_with_host_integers(c, x, given)
+        waited = busy.query()
+        for m in made:
+            for i in range(2):
+                m[i] = 63
+        made.clear()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all((a == b).all() for a, b in zip(_bytes(c), _bytes(caches[0])))
+    assert not waited
+
+
+@pytest.mark.gpu
+def test_host_integers_are_refused_under_capture(gpu):
+    c = vx.create_kv_cache(2, 64, 2, 64, device=gpu)
+    x = torch.ones((2, 1, 2, 64), dtype=torch.bfloat16, device=gpu)
+    want = vx.cached_attention(x, c, _ints([4, 5], gpu))  # (and the library is loaded)
+    n = _ints([4, 5], gpu)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call, name in ((lambda: vx.kv_cache_write(c, x, x, [1, 2]), "start"),
+                           (lambda: vx.kv_cache_read(c, 3, slots=[0, 1]), "slots"),
+                           (lambda: vx.cached_attention(x, c, torch.tensor([4, 5])), "kv_len"),
+                           (lambda: vx.shared_prefix_attention(x, c, c, prefix_len=np.array([4, 5])), "prefix_len")):
+            with pytest.raises(ValueError, match=f"{name} must be a device tensor"):
+                call()
+        got = vx.cached_attention(x, c, n)
+    for _ in range(3):
+        got.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 @pytest.mark.gpu
 def test_refusals_of_gpu_calls(gpu):
     c = vx.create_kv_cache(2, 64, 2, 64, device=gpu)

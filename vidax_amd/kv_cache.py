@@ -15,7 +15,8 @@ not), and `shared_prefix_attention` attends over a prefix that the items of a
 batch share, read once for all of them, and each item's own tokens. Every call
 launches HIP kernels on torch's current stream and never waits for the GPU;
 lengths, positions and slots are device tensors, so a captured graph may be
-replayed while they change.
+replayed while they change. (Lists, arrays and host tensors are copied there
+behind the stream's earlier work, which a capture refuses.)
 """
 from __future__ import annotations
 
@@ -134,15 +135,29 @@ def _ints(x, n: int, index: int, name: str):
     if x is None:
         return None, None
     if not (isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.get_device() == index and x.is_contiguous()):
-        x = torch.as_tensor(x, device=torch.device("cuda", index))
+        x = torch.as_tensor(x)
         if x.is_floating_point() or x.is_complex() or x.dtype == torch.bool:
             raise TypeError(f"{name} must hold integers; got {x.dtype}")
         if x.dtype == torch.int64:  # (values past 32 bits are held at its ends, outside any cache)
             x = x.clamp(-(1 << 31), (1 << 31) - 1)
-        x = x.to(torch.int32).contiguous()
+        x = _on_device(x.to(torch.int32), index, name).contiguous()
     if x.numel() != n:
         raise ValueError(f"{name} must hold {n} integers; got shape {tuple(x.shape)}")
     return x, x.data_ptr()
+
+
+def _on_device(x: torch.Tensor, index: int, name: str) -> torch.Tensor:
+    """x on the device. Host values go by way of pinned memory of the call's own:
+    the copy waits its turn on the stream, the call does not, and the caller may
+    change x at once. (A captured copy would read that memory again at every replay.)"""
+    if x.device.type != "cpu":
+        return x.to(torch.device("cuda", index))
+    with torch.cuda.device(index):
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError(f"{name} must be a device tensor while a graph is captured")
+        held = torch.empty(x.shape, dtype=x.dtype, pin_memory=True)
+        held.copy_(x)
+        return held.to(torch.device("cuda", index), non_blocking=True)
 
 
 def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, start=None, *, num=None, slots=None) -> None:
@@ -192,9 +207,9 @@ def kv_cache_read(cache: KVCache, length: int, start=None, *, slots=None) -> Tup
         raise ValueError(f"length must be >= 0; got {length}")
     dev = cache.k.device
     if slots is not None and not isinstance(slots, torch.Tensor):
-        slots = torch.as_tensor(slots, device=dev)
+        slots = torch.as_tensor(slots)
     if start is not None and not isinstance(start, torch.Tensor):
-        start = torch.as_tensor(start, device=dev)
+        start = torch.as_tensor(start)
     B = slots.numel() if slots is not None else start.numel() if start is not None else n_slots
     start, start_at = _ints(start, B, index, "start")
     slots, slots_at = _ints(slots, B, index, "slots")
