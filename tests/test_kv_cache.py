@@ -768,6 +768,28 @@ def test_host_integers_wait_for_nothing(gpu, host):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int16, torch.uint16, torch.uint32, torch.int64, torch.uint64])
+@pytest.mark.parametrize("on", ["host", "gpu"])
+def test_integers_of_any_type(gpu, dtype, on):
+    """Integers of other types than int32 count as what they are: the largest of their type as a length past
+    the capacity and a position past the end."""
+    g = torch.Generator(device=gpu).manual_seed(14)
+    x = torch.randn((2, 1, 2, 64), generator=g, device=gpu).bfloat16()
+    k = torch.randn((2, 64, 2, 64), generator=g, device=gpu).bfloat16()
+    cache = vx.create_kv_cache(2, 64, 2, 64, device=gpu)
+    vx.kv_cache_write(cache, k, k)
+    before = _bytes(cache)
+    top = torch.from_numpy(np.array([np.iinfo(str(dtype).split(".")[1]).max, 5], str(dtype).split(".")[1]))
+    top = top.to(gpu) if on == "gpu" else top
+    assert top.dtype == dtype
+    assert torch.equal(vx.cached_attention(x, cache, top), vx.cached_attention(x, cache, _ints([64, 5], gpu)))
+    assert (vx.kv_cache_read(cache, 1, top)[0][0] == 0).all()
+    vx.kv_cache_write(cache, x, x, top)
+    after = _bytes(cache)
+    assert all((a[0] == b[0]).all() for a, b in zip(after, before)) and (after[0][1, :, 5] != before[0][1, :, 5]).any()
+
+
+@pytest.mark.gpu
 def test_host_integers_are_refused_under_capture(gpu):
     c = vx.create_kv_cache(2, 64, 2, 64, device=gpu)
     x = torch.ones((2, 1, 2, 64), dtype=torch.bfloat16, device=gpu)

@@ -138,7 +138,13 @@ def _ints(x, n: int, index: int, name: str):
         x = torch.as_tensor(x)
         if x.is_floating_point() or x.is_complex() or x.dtype == torch.bool:
             raise TypeError(f"{name} must hold integers; got {x.dtype}")
-        if x.dtype == torch.int64:  # (values past 32 bits are held at its ends, outside any cache)
+        # (values past 32 bits are held at its ends, outside any cache)
+        if x.dtype == torch.uint32:
+            x = x.to(torch.int64)
+        elif x.dtype == torch.uint64:
+            x = x.view(torch.int64)
+            x = x.masked_fill(x < 0, (1 << 31) - 1)
+        if x.dtype == torch.int64:
             x = x.clamp(-(1 << 31), (1 << 31) - 1)
         x = _on_device(x.to(torch.int32), index, name).contiguous()
     if x.numel() != n:
