@@ -790,6 +790,18 @@ def test_integers_of_any_type(gpu, dtype, on):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("none", [[], (), np.array([], np.int64), torch.tensor([], dtype=torch.int64)], ids=repr)
+def test_integers_of_no_items(gpu, none):
+    c = vx.create_kv_cache(2, 64, 2, 64, device=gpu)
+    x = torch.zeros((0, 3, 2, 64), dtype=torch.bfloat16, device=gpu)
+    vx.kv_cache_write(c, x, x, none, num=none, slots=none)
+    assert vx.kv_cache_read(c, 3, none, slots=none)[0].shape == (0, 3, 2, 64)
+    assert vx.cached_attention(x, c, none, q_len=none, slots=none).shape == x.shape
+    with pytest.raises(ValueError, match="kv_len must hold 2"):
+        vx.cached_attention(x.new_zeros((2, 1, 2, 64)), c, none)
+
+
+@pytest.mark.gpu
 def test_host_integers_are_refused_under_capture(gpu):
     c = vx.create_kv_cache(2, 64, 2, 64, device=gpu)
     x = torch.ones((2, 1, 2, 64), dtype=torch.bfloat16, device=gpu)

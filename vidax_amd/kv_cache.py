@@ -135,7 +135,10 @@ def _ints(x, n: int, index: int, name: str):
     if x is None:
         return None, None
     if not (isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.get_device() == index and x.is_contiguous()):
-        x = torch.as_tensor(x)
+        if not isinstance(x, torch.Tensor):
+            x = torch.as_tensor(x)
+            if x.numel() == 0:  # (an empty list has no integers to tell its type)
+                x = x.to(torch.int32)
         if x.is_floating_point() or x.is_complex() or x.dtype == torch.bool:
             raise TypeError(f"{name} must hold integers; got {x.dtype}")
         # (values past 32 bits are held at its ends, outside any cache)
@@ -212,11 +215,8 @@ def kv_cache_read(cache: KVCache, length: int, start=None, *, slots=None) -> Tup
     if length < 0:
         raise ValueError(f"length must be >= 0; got {length}")
     dev = cache.k.device
-    if slots is not None and not isinstance(slots, torch.Tensor):
-        slots = torch.as_tensor(slots)
-    if start is not None and not isinstance(start, torch.Tensor):
-        start = torch.as_tensor(start)
-    B = slots.numel() if slots is not None else start.numel() if start is not None else n_slots
+    items = slots if slots is not None else start
+    B = torch.as_tensor(items).numel() if items is not None else n_slots
     start, start_at = _ints(start, B, index, "start")
     slots, slots_at = _ints(slots, B, index, "slots")
     k = torch.empty((B, length, Hk, D), dtype=torch.bfloat16, device=dev)
