@@ -97,6 +97,8 @@ int32_t vx_kv_read_check(const void* cache_k, const void* cache_v, const uint8_t
  *                 finished; calls that overlap need workspaces of their own
  * A weight is at most 2^8 before the division by the sum, and is multiplied by its
  * value row's scale in bf16's range: values from 2^-100 to 2^100 keep their precision.
+ * The logits (scale * q . k, and q . k itself) may be of any size that fp32 holds,
+ * times log2(e); up to 2^24 in calls that run in the flash kernels (vx_last_launch).
  * A query without a visible key gives zeros. A key or value row of scale 255
  * makes NaN the outputs of exactly those queries of its head that see it.
  */

@@ -603,6 +603,54 @@ def test_large_logits_and_rows(gpu):
     assert np.isfinite(got).all() and np.abs(got - ref).max() <= 0.25 * 2.0 ** 110
 
 
+LARGE = [  # B, Sq, H, Hk, D, cap, kv_len, prefix capacity, kernel
+    (2, 1, 4, 2, 128, 128, [128, 77], 0, "few_kernel<128"),
+    (2, 3, 4, 2, 64, 2048, [2048, 1999], 0, "few_kernel<64"),           # in ranges
+    (2, 512, 32, 4, 128, 576, [576, 500], 0, "many_kernel<128>"),
+    (4, 512, 32, 4, 64, 576, [576, 500, 1, 64], 0, "many_kernel<64>"),
+    (2, 1, 4, 2, 128, 64, [64, 20], 192, "few_kernel<128, 8, true>"),
+    (2, 5, 8, 2, 64, 64, [64, 20], 2048, "prefix_kernel<64"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [-2.0 ** 125, -2.0 ** 105, -2.0 ** 40, -2.0 ** 25, 2.0 ** 25, 2.0 ** 40, 2.0 ** 125])
+@pytest.mark.parametrize("case", LARGE, ids=[c[-1] + ("" if c[5] < 2048 else " in ranges") for c in LARGE])
+def test_logits_of_any_size(gpu, case, size):
+    """Logits of 2^25 to 2^125 of either sign: all weight on the keys of the largest
+    one, evenly. (The products are exact, one dim each, and the logits differ by an
+    eighth or more of their size, so the weights are equal or nothing, and their
+    rounding is one common factor of at most 2^-8: the bound of the module's docstring
+    without its term for inexact logits.)"""
+    B, Sq, H, Hk, D, cap, kv_len, p_cap, kernel = case
+    print(f"[case] logits of {size} in {case}", flush=True)
+    rng = np.random.default_rng(17)
+
+    def cache_of(n, positions):
+        k = np.zeros((n, positions, Hk, D))
+        k[..., 5] = rng.choice([1.0, 1.125, 1.25, 1.5, 1.75], (n, positions, Hk))
+        c = vx.create_kv_cache(n, positions, Hk, D, device=gpu)
+        vx.kv_cache_write(c, _bf16(k * 2.0 ** 60, gpu), _bf16(rng.standard_normal(k.shape), gpu))
+        return c
+
+    cache, q = cache_of(B, cap), np.zeros((B, Sq, H, D))
+    q[..., 5] = size / 2.0 ** 60
+    q = _bf16(q, gpu)
+    kw = dict(kv_len=kv_len, causal=True, scale=1.0)
+    prefix = None
+    if p_cap:
+        prefix = cache_of(1, p_cap)
+        got = vx.shared_prefix_attention(q, prefix, cache, _ints(kv_len, gpu), prefix_len=_ints([p_cap - 30], gpu), scale=1.0)
+        kw["prefix_len"] = [p_cap - 30]
+    else:
+        got = vx.cached_attention(q, cache, _ints(kv_len, gpu), scale=1.0)
+    assert _lib.last_launch().startswith(kernel)
+    ref, spread = O.cached_attention(q.double().cpu().numpy(), *_held(cache), prefix=_held(prefix) if p_cap else None, **kw)
+    tol = 2 * 2.0 ** -8 * np.abs(ref) + spread * (2.0 ** -8 + 2 * (cap + p_cap + 64) * 2.0 ** -24)
+    err = np.abs(got.double().cpu().numpy() - ref)
+    assert (err <= tol).all(), (np.argwhere(~(err <= tol))[:3], np.isnan(err).sum())
+
+
 @pytest.mark.gpu
 def test_offsets_past_32_bits(gpu):
     """The last slot of a cache whose arrays are above 4 GiB."""

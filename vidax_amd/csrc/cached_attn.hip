@@ -40,8 +40,13 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
-constexpr float kNegBig = -1.0e30f;  // finite "no key seen yet" reference point
-constexpr float kSlack = 8.0f;       // weights up to 2^kSlack before the reference point moves
+constexpr float kNone = -__FLT_MAX__;  // "no key seen yet": a reference point that no score lies below
+constexpr float kSlack = 8.0f;         // weights up to 2^kSlack before the reference point moves
+// A weight is 2^(score * c - m) in one fused operation, m such a product, rounded. Past
+// this magnitude of m that rounding (up to 2^-24 of it) is more than a factor of two of
+// the weight, and far past it weights are all infinite or nothing. A workgroup that
+// ends a part with such an m does it once more with the products rounded on both sides.
+constexpr float kFar = 16777216.0f;
 
 typedef VX_LDS unsigned char lds_u8;
 // (a pointer made from an integer is a flat one unless its type says more, and a
@@ -54,6 +59,8 @@ __device__ __forceinline__ void wait_copies() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > kFar && m > kNone; }
 
 // x == 0 by its bits, hidden from the compiler (which may take floats to be no NaN).
 __device__ __forceinline__ bool is_zero(float x) {
@@ -245,7 +252,8 @@ struct FewCfg {
   static constexpr int kOutRow = D + 4;                  // fp32 values between rows of the exchange
   static constexpr int kExchange = 32 * kOutRow * 4;
   static constexpr int kTiles = (kRing * kBuf > kExchange ? kRing * kBuf : kExchange) * W;
-  static constexpr int kSmem = kTiles + W * 32 * 8;  // then (reference point, sum) of the waves' rows
+  static constexpr int kFlags = kTiles + W * 32 * 8;  // then (reference point, sum) of the waves' rows
+  static constexpr int kSmem = kFlags + W * 4;        // ... whether any of them is far, per wave
 };
 
 // Keys of one kv head as few_part reads them.
@@ -265,6 +273,7 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
   using T = Fp8Tile<D>;
   const Streams& s = pt.s;
   float(*const ml)[32][2] = (float(*)[32][2])(smem + C::kTiles);
+  VX_LDS int* const far = (VX_LDS int*)((lds_u8*)smem + C::kFlags);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hf = lane >> 5, col = lane & 31;
@@ -307,9 +316,9 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
 
   const Range range = pt.budget == 0 ? whole_stream(s, item) : range_of<kFewTile>(s, pt.budget, pt.min_chunk, item);
   int stream = range.stream, len = range.len, first = range.tile, left = range.tiles;
+  bool rounded = false;  // the products are
   while (left > 0) {
     const int tiles = tiles_in<kFewTile>(len), take = pt.budget == 0 ? tiles : min(left, tiles - first);
-    left -= pt.budget == 0 ? left : take;
 
     const RowMap map{a, stream, kvh, a.H / Hk, pt.per};
     int rb, ri, rh;
@@ -340,11 +349,12 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
     own.all = least(own.bound);
     const int any = -least(-own.bound);  // keys that some row sees
     if (BOTH) shared.all = least(shared.bound);
+    if (rounded) own.all = shared.all = 0;
 
     f32x16 O[D / 32];
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) O[db] = f32x16{};
-    float m = kNegBig, l = 0.f;
+    float m = kNone, l = 0.f;
     auto step = [&](const int key0, const int bound, const int all, const int buf) {
       const lds_u8* kb = ring + buf * C::kBuf;
       const lds_u8* vb = kb + C::kTileBytes;
@@ -362,7 +372,7 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
         S = mfma32x32x16(e4m3x8_bf16(u32x2{kr[0], kr[1]}, kf), q[2 * x], S);
         S = mfma32x32x16(e4m3x8_bf16(u32x2{kr[2], kr[3]}, kf), q[2 * x + 1], S);
       }
-      const bool slow = key0 + kFewTile > all;  // some row does not see some key
+      const bool slow = key0 + kFewTile > all;  // some row does not see some key (or the products are rounded)
       float cc = c;
       if (slow) {
         cc = 1.0f;
@@ -450,7 +460,18 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
         ml[wave][col][1] = lsum;
       }
     }
+    const bool some_far = __builtin_amdgcn_ballot_w64(is_far(m)) != 0;
+    if (lane == 0) far[wave] = some_far;
     __syncthreads();
+    int any_far = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) any_far |= far[w];
+    if (!rounded && __builtin_amdgcn_readfirstlane(any_far) != 0) {
+      rounded = true;
+      __syncthreads();  // (the rings take the part again)
+      continue;
+    }
+    rounded = false;
     const bool final_rows = pt.direct && take == tiles;
     float* const part =
         final_rows ? nullptr
@@ -484,6 +505,7 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
         }
       }
     }
+    left -= pt.budget == 0 ? left : take;
     if (left > 0) {
       if (!next_stream(s, stream, len)) return;
       first = 0;
@@ -512,11 +534,14 @@ struct ManyCfg {
 };
 
 // Tiles first .. first + take - 1 of a stream (`whole`: all it has) for rows rt
-// kRows + 0 .. kRows - 1 of kv head kvh; `part`: the number of its partial result.
+// kRows + 0 .. kRows - 1 of kv head kvh; part_no: the number of its partial result.
+// False, with nothing written, if a reference point is far and the products are not
+// `rounded`.
 template <int D, int W>
-__device__ __forceinline__ void many_one(const CachedAttnArgs& a, const Part& pt, const int kvh, const int rt,
+__device__ __forceinline__ bool many_one(const CachedAttnArgs& a, const Part& pt, const int kvh, const int rt,
                                          const int stream, const int len, const int first, const int take,
-                                         const bool whole, const int part_no, unsigned char* smem) {
+                                         const bool whole, const int part_no, const bool rounded,
+                                         unsigned char* smem) {
   using C = ManyCfg<D, W>;
   const Streams& s = pt.s;
   const int rows = pt.rows, Hk = s.c.Hk;
@@ -540,7 +565,7 @@ __device__ __forceinline__ void many_one(const CachedAttnArgs& a, const Part& pt
   int all = bound;  // keys that every row of the wave sees
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) all = min(all, __shfl_xor(all, off, 64));
-  all = __builtin_amdgcn_readfirstlane(all);
+  all = rounded ? 0 : __builtin_amdgcn_readfirstlane(all);
   // keys that any row of the workgroup sees
   int end = len;
   if (!pt.prefix) {
@@ -554,7 +579,7 @@ __device__ __forceinline__ void many_one(const CachedAttnArgs& a, const Part& pt
   f32x16 O[kDB];
 #pragma unroll
   for (int db = 0; db < kDB; ++db) O[db] = f32x16{};
-  float m_run = kNegBig, l_run = 0.f;
+  float m_run = kNone, l_run = 0.f;
   const float c = a.scale * kLog2e;
 
   // ---- staging: a thread takes 16-byte chunks (16 values of one key) of K and
@@ -790,6 +815,17 @@ __device__ __forceinline__ void many_one(const CachedAttnArgs& a, const Part& pt
     } else {
       last_pv(Odd{}, Pp);
     }
+    if (!rounded) {
+      // (one answer for the workgroup, whose waves share the tiles)
+      VX_LDS int* const far = (VX_LDS int*)(lds_u8*)smem;
+      __syncthreads();
+      far[wave] = __builtin_amdgcn_ballot_w64(is_far(m_run)) != 0;
+      __syncthreads();
+      int any_far = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) any_far |= far[w];
+      if (__builtin_amdgcn_readfirstlane(any_far) != 0) return false;
+    }
   }
 
   const float L = halves_sum(l_run);
@@ -821,6 +857,7 @@ __device__ __forceinline__ void many_one(const CachedAttnArgs& a, const Part& pt
       part[(int64_t)rows * D + 2 * r + 1] = L;
     }
   }
+  return true;
 }
 
 // A range of tiles of streams of more rows, for one tile of rows of one kv head.
@@ -844,11 +881,17 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
   const Range range =
       pt.budget == 0 ? whole_stream(pt.s, item) : range_of<kManyTile>(pt.s, pt.budget, pt.min_chunk, item);
   int stream = range.stream, len = range.len, first = range.tile, left = range.tiles;
+  bool rounded = false;
   while (left > 0) {
     const int tiles = tiles_in<kManyTile>(len), take = pt.budget == 0 ? tiles : min(left, tiles - first);
+    if (!many_one<D, W>(a, pt, kvh, rt, stream, len, first, take, take == tiles,
+                        pt.budget == 0 ? item : item + stream, rounded, smem)) {
+      rounded = true;
+      __syncthreads();  // (the tiles' buffers take the part again)
+      continue;
+    }
+    rounded = false;
     left -= pt.budget == 0 ? left : take;
-    many_one<D, W>(a, pt, kvh, rt, stream, len, first, take, take == tiles, pt.budget == 0 ? item : item + stream,
-                   smem);
     if (left > 0) {
       if (!next_stream(pt.s, stream, len)) return;
       first = 0;
@@ -918,7 +961,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const CachedAttnArgs a,
   const int64_t x = (int64_t)blockIdx.x * (kGroups / split) + group / split;
   const bool real = x < (int64_t)Hk * own.rows;
   const int kvh = real ? (int)(x / own.rows) : 0, r = real ? (int)(x - (int64_t)kvh * own.rows) : 0;
-  float M = kNegBig, L = 0.f;
+  float M = kNone, L = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   const int total = real ? pc.count + oc.count : 0;
   const int64_t pre_block = part_floats(pre.rows, D), own_block = part_floats(own.rows, D);

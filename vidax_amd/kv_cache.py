@@ -216,7 +216,7 @@ def kv_cache_read(cache: KVCache, length: int, start=None, *, slots=None) -> Tup
         raise ValueError(f"length must be >= 0; got {length}")
     dev = cache.k.device
     items = slots if slots is not None else start
-    B = torch.as_tensor(items).numel() if items is not None else n_slots
+    B = n_slots if items is None else (items if isinstance(items, torch.Tensor) else torch.as_tensor(items)).numel()
     start, start_at = _ints(start, B, index, "start")
     slots, slots_at = _ints(slots, B, index, "slots")
     k = torch.empty((B, length, Hk, D), dtype=torch.bfloat16, device=dev)
