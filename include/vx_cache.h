@@ -94,11 +94,14 @@ int32_t vx_kv_read_check(const void* cache_k, const void* cache_v, const uint8_t
  *                 [0, prefix_capacity]
  *   workspace     vx_cached_attn_workspace_size() bytes of device memory,
  *                 16-byte aligned, untouched until the work on `stream` has
- *                 finished; calls that overlap need workspaces of their own
+ *                 finished; calls that overlap need workspaces of their own.
+ *                 (Some calls expand the cached keys and values to bf16 in it:
+ *                 see vx_cached_attn_workspace_size.)
  * A weight is at most 2^8 before the division by the sum, and is multiplied by its
  * value row's scale in bf16's range: values from 2^-100 to 2^100 keep their precision.
  * The logits (scale * q . k, and q . k itself) may be of any size that fp32 holds,
- * times log2(e); up to 2^24 in calls that run in the flash kernels (vx_last_launch).
+ * times log2(e); calls that expand the cache (see the workspace) take magnitudes up
+ * to 2^24.
  * A query without a visible key gives zeros. A key or value row of scale 255
  * makes NaN the outputs of exactly those queries of its head that see it.
  */
@@ -124,6 +127,14 @@ int32_t vx_cached_attn_check(const void* q, const void* out, const int64_t* q_st
  * Workspace bytes vx_cached_attn_fwd needs for these sizes on the current
  * device (0: none; -1 on failure). num_prefixes is 0 without a prefix; cross is
  * 1 for a call that is not causal and has no q_len.
+ *
+ * Where a cross call has no prefix, as many heads as the cache, seq_q >= capacity
+ * and batch * num_heads * seq_q >= 300000, the cached keys and values are expanded
+ * to bf16 in the workspace: 4 * head_dim bytes per position, head and batch item of
+ * the capacity (not of kv_len; what lies past kv_len is not written): at most twice
+ * the bytes of q. A capacity above seq_q, or a q_len, leaves such a call with the
+ * kernels that read the cache as it is and need no workspace: 3 to 48 % more time
+ * (2 x 32760 queries of 40 heads on 512 and 384 keys 664 us, with q_len 804 to 842).
  */
 int64_t vx_cached_attn_workspace_size(int32_t capacity, int32_t num_prefixes, int32_t prefix_capacity, int32_t batch,
                                       int32_t seq_q, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
