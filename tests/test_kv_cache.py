@@ -651,6 +651,43 @@ def test_logits_of_any_size(gpu, case, size):
     assert (err <= tol).all(), (np.argwhere(~(err <= tol))[:3], np.isnan(err).sum())
 
 
+EVEN = LARGE + [(2, 257, 3, 3, 64, 320, [320, 77], 0, "few_kernel<64"), (1, 4096, 74, 74, 128, 128, [100], 0, "flash_")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", EVEN, ids=[c[-1] + f" {c[5]}" for c in EVEN])
+def test_the_weights_sum_to_one(gpu, case):
+    """Values that are the same for all keys come out as they are, bit for bit: the
+    sum that divides is that of the weights that multiply them. Here all weights but
+    one of 32 are 2^-0.99609, which bf16 rounds down by 0.27 %: over the sum of the
+    unrounded ones, a value 1 would become 1 - 2^-8. (fp32 sums of 2^12 terms are off by
+    2^-12 at most, half a step of bf16 below 1 is 2^-9.)"""
+    B, Sq, H, Hk, D, cap, kv_len, p_cap, kernel = case
+    print(f"[case] weights of {case}", flush=True)
+
+    def cache_of(n, positions):
+        c = vx.create_kv_cache(n, positions, Hk, D, device=gpu)
+        k, v = np.zeros((n, positions, Hk, D)), np.ones((n, positions, Hk, D))
+        k[..., 3] = -1.0
+        k[:, ::32] = 0.0
+        vx.kv_cache_write(c, _bf16(k, gpu), _bf16(v * 2.0 ** np.arange(-3, Hk - 3)[:, None], gpu))
+        return c
+
+    cache = cache_of(B, cap)
+    q, n = torch.full((B, Sq, H, D), 0.99609375, dtype=torch.bfloat16, device=gpu), _ints(kv_len, gpu)
+    scale = float(np.log(2.0))  # (logits in log2 units)
+    if p_cap:
+        got = vx.shared_prefix_attention(q, cache_of(1, p_cap), cache, n, prefix_len=_ints([p_cap - 30], gpu), scale=scale)
+    else:
+        got = vx.cached_attention(q, cache, n, causal=kernel != "flash_", scale=scale)
+    assert _lib.last_launch().startswith(kernel)
+    want = vx.kv_cache_read(cache, 1)[1][:1].repeat_interleave(H // Hk, 2).expand(B, Sq, H, D).clone()
+    if kernel != "flash_" and not p_cap:  # (causal queries in front of the first key see none)
+        for b, m in enumerate(kv_len):
+            want[b, :max(Sq - m, 0)] = 0
+    assert torch.equal(got, want), int((got != want).sum())
+
+
 @pytest.mark.gpu
 def test_offsets_past_32_bits(gpu):
     """The last slot of a cache whose arrays are above 4 GiB."""

@@ -16,7 +16,10 @@
 // and the two halves of a wave exchange them by one v_permlane32_swap. e4m3
 // values are exact in bf16, and so are they times a power of two, so the only
 // roundings are the weights' and the output's to bf16; scores, sums, outputs and
-// partial results are fp32.
+// partial results are fp32. (The weights are rounded because the MFMA takes bf16: fp32
+// ones would be two products, high and low part, for a relative error against 64 bits
+// of 1.6e-3, the output's rounding alone, in place of 1.6e-3 to 1.8e-3. The sum that
+// divides is that of the rounded weights, so values that agree come out as they are.)
 //
 // few_part reads K and V as they lie, by DMA to LDS rings of the waves' own (no
 // barrier in the loop), and converts them behind the LDS reads: K with its scale in
@@ -391,17 +394,25 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) O[db] *= alpha;
       }
+      // The weights times their value rows' scales, rounded to bf16 (a power of two changes
+      // no rounding), and the sum of the rounded weights, so that those that multiply V
+      // sum to one (as in many_part).
       bf16x8 P[2];
       const float mneg = -m;
+      const bf16x2 one2 = {(bf16)1.0f, (bf16)1.0f};
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p = fast_exp2(__builtin_fmaf(S[8 * j + e], cc, mneg));
-          l += p;
-          float w = p * __uint_as_float(((vsc[j][e >> 2] >> (8 * (e & 3))) & 0xffu) << 23);
-          if (slow && !(key0 + 16 * j + 8 * hf + e < bound)) w = 0.f;  // (its scale may be anything)
-          P[j][e] = (bf16)w;
+        for (int e = 0; e < 8; e += 2) {
+          float p[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            p[i] = fast_exp2(__builtin_fmaf(S[8 * j + e + i], cc, mneg));
+            float w = p[i] * __uint_as_float(((vsc[j][e >> 2] >> (8 * ((e & 3) + i))) & 0xffu) << 23);
+            if (slow && !(key0 + 16 * j + 8 * hf + e + i < bound)) w = 0.f;  // (its scale may be anything)
+            P[j][e + i] = (bf16)w;
+          }
+          l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{(bf16)p[0], (bf16)p[1]}, one2, l, false);
         }
       // V^T fragment (db, j): lane group g = lane / 16 takes dims db 32 + (g % 2) 16
       // + 0..15 of keys 16 j + 8 (g / 2) + 0..7
