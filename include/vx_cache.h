@@ -28,6 +28,10 @@
 extern "C" {
 #endif
 
+/* Version of this header's entries (major * 10000 + minor * 100 + patch): 1.0.0. A library
+ * without them does not export this one; vx_abi_version() is that of vx_attn.h alone. */
+int32_t vx_cache_abi_version(void);
+
 /*
  * Quantises new tokens' keys and values into the cache: token t of batch item
  * b goes to position start[b] + t of slot slots[b].

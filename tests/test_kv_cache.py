@@ -36,6 +36,10 @@ def test_cache_symbols_are_exported():
     assert all(hasattr(_lib.lib(), n) for n in names)
 
 
+def test_cache_abi_version():
+    assert _lib.lib().vx_cache_abi_version() == 10000
+
+
 def _write_check(**kw):
     a = dict(k=A, v=A, kst=None, vst=None, ck=A, cv=A, ks=A, vs=A, slots_n=4, cap=128, start=None, num=None,
              slots=None, B=2, S=3, Hk=2, D=64)

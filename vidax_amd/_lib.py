@@ -53,6 +53,7 @@ EXPORTED_SYMBOLS = (
 )
 
 CACHE_SYMBOLS = (  # include/vx_cache.h
+    "vx_cache_abi_version",
     "vx_kv_write_fwd",
     "vx_kv_write_check",
     "vx_kv_read_fwd",
@@ -163,6 +164,8 @@ def lib() -> ctypes.CDLL:
             h.vx_key_masks_fwd.argtypes = [_p, _i64p, _p, _i64p, _i32, _i32, _p, _p, _p, _i64, _p]
             h.vx_full_bias_fwd.restype = _i32
             h.vx_full_bias_fwd.argtypes = [_p, _i64p, _p, _i64p, _i32, _i32, _i32, _i32, _p, _p]
+            h.vx_cache_abi_version.restype = _i32
+            h.vx_cache_abi_version.argtypes = []
             h.vx_kv_write_fwd.restype = _i32
             h.vx_kv_write_fwd.argtypes = _KV_WRITE_ARGS + [_p]
             h.vx_kv_write_check.restype = _i32

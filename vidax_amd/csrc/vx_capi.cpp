@@ -1230,6 +1230,8 @@ int32_t vx_rmsnorm_scale_rope_fwd(const void* x, void* out, const float* weight,
   return ok();
 }
 
+int32_t vx_cache_abi_version(void) { return 10000; }
+
 int32_t vx_kv_write_check(const void* k, const void* v, const int64_t* k_strides, const int64_t* v_strides,
                           const void* cache_k, const void* cache_v, const uint8_t* k_scale, const uint8_t* v_scale,
                           int32_t num_slots, int32_t capacity, const int32_t* start, const int32_t* num,
