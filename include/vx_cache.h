@@ -60,8 +60,9 @@ int32_t vx_kv_write_check(const void* k, const void* v, const int64_t* k_strides
  * Reads seq positions from start[b] of slot slots[b] on back as bf16: k_out
  * and v_out, contiguous (batch, seq, num_kv_heads, head_dim), 16-byte aligned.
  * start and slots as in vx_kv_write_fwd. Positions outside the cache give
- * zeros. The bf16 values are the stored ones exactly (magnitudes below 2^-126
- * give zero).
+ * zeros. The bf16 values are the stored ones rounded to bf16, which holds all of
+ * magnitudes 2^-126 to below 2^128 exactly (a bf16 value above 1.9375 * 2^127 is
+ * stored as 2^128, and reads as infinite).
  */
 int32_t vx_kv_read_fwd(const void* cache_k, const void* cache_v, const uint8_t* k_scale, const uint8_t* v_scale,
                        int32_t num_slots, int32_t capacity, const int32_t* start, const int32_t* slots,

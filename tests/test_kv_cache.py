@@ -369,6 +369,26 @@ def test_read(gpu, B, S, Hk, D, cap, start, slots):
         assert (got.double().cpu().numpy() == want).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_read_every_byte(gpu, D):
+    """Every value byte but the NaN codes under every scale byte, as a cache made elsewhere may hold them."""
+    raw = np.delete(np.arange(256), [0x7f, 0xff]).astype(np.uint8)
+    codes = np.stack([np.roll(np.resize(raw, 256 * D), 7 * s).reshape(1, 256, D) for s in range(256)])
+    scales = np.broadcast_to(np.arange(256, dtype=np.uint8)[:, None, None], (256, 1, 256)).copy()
+    codes[255] = 0
+    t = [torch.from_numpy(x).to(gpu) for x in (codes, scales)]
+    cache = vx.KVCache(t[0].view(E4M3), t[0].clone().view(E4M3), t[1].view(E8M0), t[1].clone().view(E8M0))
+    want = torch.from_numpy(O.values(codes, scales)).transpose(1, 2)  # (slots, positions, 1, D)
+    for got in vx.kv_cache_read(cache, 256):
+        x = got.double().cpu()
+        ref = want.float().bfloat16().double()  # (values have four bits: exact in fp32; in bf16 down to 2^-130)
+        same = (x == ref) | (x.isnan() & ref.isnan())
+        assert same.all(), [(int(s), float(want[s][~same[s]][0]), float(x[s][~same[s]][0]))
+                            for s in (~same).any(-1).any(-1).any(-1).nonzero()[:5, 0]]
+        assert ((ref == want) | want.isnan() | (want.abs() < 2.0 ** -126) | (want.abs() >= 2.0 ** 128)).all()
+
+
 def _cache_of(rng, slots, Hk, cap, D, gpu, lens=None, std=1.0):
     """A cache of random tokens; positions from lens[slot] on hold arbitrary
     bytes (NaN codes and scales among them)."""

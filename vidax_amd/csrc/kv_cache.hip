@@ -7,7 +7,7 @@
 // more where the mantissa is above 1.75 (never below 1: rows smaller than that
 // lose their lowest bits). The product by a power of two is exact, so each
 // value is rounded once, to nearest even.
-// read: the same back, exact in bf16.
+// read: the same back, exact in bf16 (subnormal values of it rounded to nearest).
 //
 // Both are bound by their bytes: 2 D + D + 1 per row. A row takes D / 16 lanes,
 // 16 values each: whole 256-byte lines on the bf16 side, 128-byte ones on the

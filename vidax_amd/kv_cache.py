@@ -206,8 +206,8 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, start=None,
 
 def kv_cache_read(cache: KVCache, length: int, start=None, *, slots=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(k, v), each (B, length, num_kv_heads, head_dim) bf16: positions start[b]
-    .. start[b] + length - 1 of slot slots[b], as they are stored (bf16 holds
-    every such value; magnitudes below 2^-126 give zero). B is the length of
+    .. start[b] + length - 1 of slot slots[b], as they are stored, rounded to bf16
+    (which holds all such values of magnitudes 2^-126 to below 2^128). B is the length of
     `slots`, else of `start`, else the number of slots; defaults as in
     kv_cache_write. Positions outside the cache give zeros."""
     n_slots, Hk, cap, D, index = _check_cache(cache, "cache")
