@@ -549,6 +549,161 @@ def test_cached_attention_defaults_strides_and_out(gpu):
         assert (rest == 7.0).all()  # nothing beside the output rows
 
 
+PLANS = [
+    # kernel, parts (the workspace holds some); B, Sq, H, Hk, D, cap, kv_len, q_len, causal; groups, prefix cap, prefix_len
+    ("many_kernel<128>", False, 2, 500, 32, 4, 128, 640, [640, 577], [500, 333], True, 0, 0, None),
+    ("many_kernel<64>", False, 4, 500, 32, 4, 64, 640, [601, 1, 0, 640], [499, 500, 17, 0], True, 0, 0, None),
+    ("many_kernel<128>", False, 2, 500, 32, 4, 128, 640, [63, 640], [500, 500], False, 0, 0, None),
+    ("many_kernel<64>", False, 4, 500, 32, 4, 64, 640, [601, 1, 0, 640], [499, 500, 17, 0], False, 0, 0, None),
+    ("many_kernel<128>", True, 3, 300, 8, 8, 128, 3520, [3500, 0, 1777], [300, 7, 299], True, 0, 0, None),
+    ("many_kernel<64>", True, 3, 300, 8, 8, 64, 7040, [7040, 129, 3333], [299, 300, 1], True, 0, 0, None),
+    ("many_kernel<128>", True, 3, 300, 8, 8, 128, 3520, [1, 3520, 65], None, False, 0, 0, None),
+    ("many_kernel<64>", True, 3, 300, 8, 8, 64, 7040, [0, 5001, 7000], [200, 300, 300], False, 0, 0, None),
+    ("prefix_kernel<128, false, true>", True, 16, 16, 16, 8, 128, 128, [3 + 8 * i for i in range(16)], None, True, 1, 4288,
+     [4201]),
+    ("prefix_kernel<64, false, true>", True, 16, 16, 16, 8, 64, 128, [8 * i for i in range(16)], [i + 1 for i in range(16)],
+     True, 2, 8576, [8576, 31]),
+    ("prefix_kernel<128, false, false>", True, 2, 500, 32, 4, 128, 640, [600, 501], [499, 500], True, 1, 640, [601]),
+    ("prefix_kernel<64, false, false>", True, 4, 500, 32, 4, 64, 640, [600, 0, 640, 1], [499, 500, 1, 77], True, 2, 1280,
+     [1201, 0]),
+    ("prefix_kernel<128, true, false>", True, 2, 500, 32, 4, 128, 640, [600, 501], [499, 500], True, 1, 64, [33]),
+    ("prefix_kernel<64, true, false>", True, 4, 500, 32, 4, 64, 640, [600, 0, 640, 1], None, False, 1, 64, [64]),
+    ("prefix_kernel<128, true, true>", True, 4, 5, 8, 2, 128, 2048, [2048, 5, 0, 700], [5, 1, 2, 4], True, 2, 192, [192, 1]),
+    ("prefix_kernel<64, true, true>", True, 4, 5, 8, 2, 64, 64, [64, 5, 0, 33], None, True, 1, 2048, [2001]),
+    ("few_kernel<128, 4, false>", True, 4, 1, 8, 2, 128, 2048, [2048, 5, 0, 700], None, True, 0, 0, None),
+    ("few_kernel<64, 4, false>", True, 2, 9, 8, 2, 64, 4096, [4001, 9], [9, 8], True, 0, 0, None),
+    ("few_kernel<64, 8, false>", False, 3, 5, 4, 2, 64, 320, [320, 5, 100], [5, 5, 2], True, 0, 0, None),
+    ("few_kernel<64, 4, true>", False, 40, 1, 16, 8, 64, 64, [i % 65 for i in range(40)], None, True, 2, 192, [190, 1]),
+    ("few_kernel<64, 8, true>", False, 2, 3, 4, 2, 64, 64, [64, 3], [3, 2], True, 1, 192, [190]),
+    ("few_kernel<128, 8, false>", False, 3, 5, 4, 2, 128, 320, [320, 5, 100], [5, 5, 2], True, 0, 0, None),
+    ("few_kernel<128, 4, true>", False, 40, 1, 16, 8, 128, 64, [i % 65 for i in range(40)], None, True, 2, 192, [190, 1]),
+    ("few_kernel<128, 8, true>", False, 2, 3, 4, 2, 128, 64, [64, 3], [3, 2], True, 1, 192, [190]),
+    ("few_kernel<128, 4, false>", False, 3, 1, 4, 2, 128, 128, [100, 0, 128], None, True, 0, 0, None),
+    ("few_kernel<64, 4, false>", False, 3, 40, 4, 2, 64, 128, [100, 0, 128], [40, 3, 39], False, 0, 0, None),
+]
+
+
+def _attend(case, gpu, cache, prefix, q):
+    """The call of a case of PLANS, on the kernel that it is there for."""
+    kernel, parts, B, Sq, H, Hk, D, cap, kv_len, q_len, causal, groups, p_cap, p_len = case
+    kw = dict(q_len=_ints(q_len, gpu), causal=causal)
+    size = _lib.lib().vx_cached_attn_workspace_size(cap, groups, p_cap, B, Sq, H, Hk, D, int(not causal and q_len is None))
+    assert (size > 0) == parts
+    if groups:
+        got = vx.shared_prefix_attention(q, prefix, cache, _ints(kv_len, gpu), prefix_len=_ints(p_len, gpu), **kw)
+    else:
+        got = vx.cached_attention(q, cache, _ints(kv_len, gpu), **kw)
+    assert _lib.last_launch() == kernel
+    return got
+
+
+PLAN_IDS = [f"{c[0]}{' parts' if c[1] else ''}{'' if c[10] else ' cross'}" for c in PLANS]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", PLANS, ids=PLAN_IDS)
+def test_every_kernel_of_the_plan(gpu, case):
+    kernel, _, B, Sq, H, Hk, D, cap, kv_len, q_len, causal, groups, p_cap, p_len = case
+    print(f"[case] {case}", flush=True)
+    rng = np.random.default_rng(Sq + cap + p_cap + D)
+    cache = _cache_of(rng, B, Hk, cap, D, gpu, kv_len)
+    prefix = _cache_of(rng, groups, Hk, p_cap, D, gpu, p_len) if groups else None
+    q = _bf16(2 * rng.standard_normal((B, Sq, H, D)), gpu)
+    if q_len is not None:  # (padding rows may hold anything)
+        for b, n in enumerate(q_len):
+            q[b, n:] = float("nan")
+    got = _attend(case, gpu, cache, prefix, q)
+    assert torch.equal(got, _attend(case, gpu, cache, prefix, q))
+    if q_len is not None:
+        for b, n in enumerate(q_len):
+            q[b, n:] = 0.0
+    _assert_close(got, q, _held(cache, kv_len), _held(prefix, p_len) if groups else None, kv_len=kv_len, q_len=q_len,
+                  causal=causal, **(dict(prefix_len=p_len) if groups else {}))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("case", PLANS, ids=PLAN_IDS)
+def test_nan_rows_in_every_kernel_of_the_plan(gpu, case, which):
+    """A NaN token of the cache, then one of the prefix, reaches the queries of its
+    head that see it and no others, through ranges and merges too."""
+    kernel, _, B, Sq, H, Hk, D, cap, kv_len, q_len, causal, groups, p_cap, p_len = case
+    print(f"[case] NaN in {which}, {case}", flush=True)
+    rng = np.random.default_rng(9)
+    b, head = int(np.argmax(np.minimum(kv_len, q_len or [Sq] * B))), Hk - 1
+    m, n = (q_len[b] if q_len else Sq), kv_len[b]
+    for where in ("own", "prefix") if groups else ("own",):
+        at = n - (m + 1) // 2 if where == "own" else p_len[0] // 2
+        caches = []
+        for slots, positions, spot in ((B, cap, b if where == "own" else -1),
+                                       (groups, p_cap, 0 if where == "prefix" else -1)):
+            if slots == 0:
+                caches.append(None)
+                continue
+            x = {i: rng.standard_normal((slots, positions, Hk, D)) for i in "kv"}
+            if spot >= 0:
+                x[which][spot, max(at, 0), head, 11] = np.nan
+            caches.append(vx.create_kv_cache(slots, positions, Hk, D, device=gpu))
+            vx.kv_cache_write(caches[-1], _bf16(x["k"], gpu), _bf16(x["v"], gpu))
+        q = _bf16(rng.standard_normal((B, Sq, H, D)), gpu)
+        got = _attend(case, gpu, *caches, q)
+        want = torch.zeros((B, Sq, H, D), dtype=torch.bool, device=gpu)
+        G = H // Hk
+        if where == "own":
+            first = max(at, 0) - n + m if causal else 0  # the first query that sees it
+            want[b, max(first, 0):m, head * G:] = True
+        else:
+            for i in range(B // groups):
+                want[i, :q_len[i] if q_len else Sq, head * G:] = True
+        assert torch.equal(got.isnan(), want), where
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [PLANS[0], PLANS[4], PLANS[11], None], ids=["many", "many in parts", "prefix", "expanded"])
+def test_graph_replays_of_long_calls(gpu, case):
+    """Captured calls of many queries (with prefixes, in parts, expanded to bf16),
+    replayed while lengths, queries and eager calls between the replays change;
+    every replay equals the eager result bit for bit."""
+    if case is None:
+        case = ("flash", True, 1, 4224, 72, 72, 64, 128, [128], None, False, 0, 0, None)
+    kernel, _, B, Sq, H, Hk, D, cap, _, q_len, causal, groups, p_cap, _ = case
+    print(f"[case] replays of {case}", flush=True)
+    rng = np.random.default_rng(10)
+    cache = _cache_of(rng, B, Hk, cap, D, gpu)
+    prefix = _cache_of(rng, groups, Hk, p_cap, D, gpu) if groups else None
+    q = torch.empty((B, Sq, H, D), dtype=torch.bfloat16, device=gpu)
+    kv_len, m = (torch.zeros(B, dtype=torch.int32, device=gpu) for _ in range(2))
+    p_len = torch.zeros(max(groups, 1), dtype=torch.int32, device=gpu)
+
+    def call():
+        kw = dict(q_len=m if q_len is not None else None, causal=causal)
+        if groups:
+            return vx.shared_prefix_attention(q, prefix, cache, kv_len, prefix_len=p_len, **kw)
+        return vx.cached_attention(q, cache, kv_len, **kw)
+
+    def set_inputs(share):
+        for t, most in ((kv_len, cap), (m, Sq), (p_len, p_cap)):
+            t.copy_(torch.tensor([int(most * share) // (i + 1) for i in range(t.numel())], dtype=torch.int32))
+        q.copy_(torch.randn(q.shape, device=gpu))
+
+    set_inputs(1.0)
+    call()  # warm-up
+    assert _lib.last_launch().startswith(kernel)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for share in (1.0, 0.37, 0.0, 0.9):
+        set_inputs(share)
+        want = call()  # eager work between the replays
+        torch.cuda.synchronize()
+        out.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        print(f"  replay at {share}", flush=True)
+        assert torch.equal(out, want)
+
+
 PREFIXES = [
     # B, Sq, H, Hk, D, groups, prefix cap, prefix_len, cap, kv_len, q_len, slots, causal
     (1, 1, 1, 1, 64, 1, 64, [64], 64, [1], None, None, True),
