@@ -528,16 +528,16 @@ __device__ __forceinline__ void few_part(const CachedAttnArgs& a, const Part& pt
 // ------------------------------------------------------------------ many rows
 constexpr int kManyTile = 64;  // keys per tile of many_part
 
-// A workgroup of W waves of 32 rows. LDS: two K tiles, two V tiles of bf16; a
+// A workgroup of kWaves waves of 32 rows. LDS: two K tiles, two V tiles of bf16; a
 // tile is D / 64 half planes of 64 keys x 128 bytes, a row's 16-byte chunks XOR
 // half_swizzle (as in flash_fwd.hip).
-template <int D, int W>
+template <int D>
 struct ManyCfg {
-  static constexpr int kRows = 32 * W;
+  static constexpr int kRows = 32 * kWaves;
   static constexpr int kHalf = kManyTile * 128;         // 64 keys x 64 dims
   static constexpr int kTileBytes = kManyTile * D * 2;  // of K, and of V
   static constexpr int kVBuf = 0, kKBuf = 2 * kTileBytes;
-  static constexpr int kLoads = kManyTile * (D / 16) / (W * 64);  // 16-byte chunks of K, and of V, per thread
+  static constexpr int kLoads = kManyTile * (D / 16) / kThreads;  // 16-byte chunks of K, and of V, per thread
   static constexpr int kSmem = 4 * kTileBytes;
   static constexpr int kDB = D / 32, kDS = D / 16;
   static constexpr int kPV = 4 * kDB, kQK = 2 * kDS, kSlots = kPV + kQK;
@@ -548,12 +548,12 @@ struct ManyCfg {
 // kRows + 0 .. kRows - 1 of kv head kvh; part_no: the number of its partial result.
 // False, with nothing written, if a reference point is far and the products are not
 // `rounded`.
-template <int D, int W>
+template <int D>
 __device__ __forceinline__ bool many_one(const CachedAttnArgs& a, const Part& pt, const int kvh, const int rt,
                                          const int stream, const int len, const int first, const int take,
                                          const bool whole, const int part_no, const bool rounded,
                                          unsigned char* smem) {
-  using C = ManyCfg<D, W>;
+  using C = ManyCfg<D>;
   const Streams& s = pt.s;
   const int rows = pt.rows, Hk = s.c.Hk;
   constexpr int kDB = C::kDB, kDS = C::kDS, kPV = C::kPV, kSlots = C::kSlots, kAhead = C::kAhead;
@@ -683,9 +683,9 @@ __device__ __forceinline__ bool many_one(const CachedAttnArgs& a, const Part& pt
     Raw w0;
     load(kg, 0, w0);
     load(kg, min(1, n - 1), wk);
-    const int kZero = W * 64 * 16;
+    const int kZero = kThreads * 16;
 #pragma unroll
-    for (int p = 0; p < C::kTileBytes / (W * 64 * 16); ++p)
+    for (int p = 0; p < C::kTileBytes / (kThreads * 16); ++p)
       *(VX_LDS u32x4*)((lds_u8*)smem + C::kVBuf + C::kTileBytes + p * kZero + tid * 16) = u32x4{0, 0, 0, 0};
     store_all(w0, true, C::kKBuf);
     store_all(wk, true, C::kKBuf + C::kTileBytes);
@@ -834,7 +834,7 @@ __device__ __forceinline__ bool many_one(const CachedAttnArgs& a, const Part& pt
       __syncthreads();
       int any_far = 0;
 #pragma unroll
-      for (int w = 0; w < W; ++w) any_far |= far[w];
+      for (int w = 0; w < kWaves; ++w) any_far |= far[w];
       if (__builtin_amdgcn_readfirstlane(any_far) != 0) return false;
     }
   }
@@ -872,11 +872,11 @@ __device__ __forceinline__ bool many_one(const CachedAttnArgs& a, const Part& pt
 }
 
 // A range of tiles of streams of more rows, for one tile of rows of one kv head.
-template <int D, int W>
+template <int D>
 __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& pt, const int block,
                                           unsigned char* smem) {
   const int Hk = pt.s.c.Hk;
-  const int n_rt = (pt.rows + ManyCfg<D, W>::kRows - 1) / ManyCfg<D, W>::kRows;
+  const int n_rt = (pt.rows + ManyCfg<D>::kRows - 1) / ManyCfg<D>::kRows;
   // Order: a prompt's last row tiles, which see the most keys, first; kv heads
   // side by side, so that with 8 of them each XCD keeps one head's keys in its L2.
   // Where all workgroups find a place at once (two per CU), the second half runs
@@ -895,8 +895,8 @@ __device__ __forceinline__ void many_part(const CachedAttnArgs& a, const Part& p
   bool rounded = false;
   while (left > 0) {
     const int tiles = tiles_in<kManyTile>(len), take = pt.budget == 0 ? tiles : min(left, tiles - first);
-    if (!many_one<D, W>(a, pt, kvh, rt, stream, len, first, take, take == tiles,
-                        pt.budget == 0 ? item : item + stream, rounded, smem)) {
+    if (!many_one<D>(a, pt, kvh, rt, stream, len, first, take, take == tiles, pt.budget == 0 ? item : item + stream,
+                     rounded, smem)) {
       rounded = true;
       __syncthreads();  // (the tiles' buffers take the part again)
       continue;
@@ -922,8 +922,8 @@ __global__ __launch_bounds__(W * 64, 2) void few_kernel(const CachedAttnArgs a, 
 
 template <int D>
 __global__ __launch_bounds__(kThreads, 2) void many_kernel(const CachedAttnArgs a, const Part own) {
-  __shared__ __attribute__((aligned(256))) unsigned char smem[ManyCfg<D, kWaves>::kSmem];
-  many_part<D, kWaves>(a, own, blockIdx.x, smem);
+  __shared__ __attribute__((aligned(256))) unsigned char smem[ManyCfg<D>::kSmem];
+  many_part<D>(a, own, blockIdx.x, smem);
 }
 
 // A prefix's chunks (the first pre_blocks workgroups) and the items' own, side by
@@ -931,7 +931,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const CachedAttnArgs 
 template <int D, bool PRE_FEW, bool OWN_FEW>
 __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(const CachedAttnArgs a, const Part pre, const Part own,
                                                            const int pre_blocks) {
-  constexpr int kFew = FewCfg<D, kWaves>::kSmem, kMany = ManyCfg<D, kWaves>::kSmem;
+  constexpr int kFew = FewCfg<D, kWaves>::kSmem, kMany = ManyCfg<D>::kSmem;
   constexpr int kPre = PRE_FEW ? kFew : kMany, kOwn = OWN_FEW ? kFew : kMany;
   __shared__ __attribute__((aligned(256))) unsigned char smem[kPre > kOwn ? kPre : kOwn];
   const int block = blockIdx.x;
@@ -939,12 +939,12 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_kernel(const CachedAttnArg
     if constexpr (PRE_FEW)
       few_part<D, kWaves, false>(a, pre, nullptr, block, smem);
     else
-      many_part<D, kWaves>(a, pre, block, smem);
+      many_part<D>(a, pre, block, smem);
   } else {
     if constexpr (OWN_FEW)
       few_part<D, kWaves, false>(a, own, nullptr, block - pre_blocks, smem);
     else
-      many_part<D, kWaves>(a, own, block - pre_blocks, smem);
+      many_part<D>(a, own, block - pre_blocks, smem);
   }
 }
 
