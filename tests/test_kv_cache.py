@@ -1089,6 +1089,17 @@ def test_host_integers_are_refused_under_capture(gpu):
 
 
 @pytest.mark.gpu
+def test_more_tokens_than_32_bits_count_are_refused(gpu):
+    """(an expanded row: 2^32 + 3 tokens in 128 bytes)"""
+    c = vx.create_kv_cache(1, 64, 1, 64, device=gpu)
+    x = torch.ones((1, 1, 1, 64), dtype=torch.bfloat16, device=gpu)
+    for n in (2 ** 31, 2 ** 32 + 3):
+        with pytest.raises(NotImplementedError, match="tokens per item"):
+            vx.kv_cache_write(c, x.expand(1, n, 1, 64), x.expand(1, n, 1, 64))
+    assert (_bytes(c)[0] == 0).all()
+
+
+@pytest.mark.gpu
 def test_refusals_of_gpu_calls(gpu):
     c = vx.create_kv_cache(2, 64, 2, 64, device=gpu)
     x = torch.zeros((2, 3, 2, 64), dtype=torch.bfloat16, device=gpu)

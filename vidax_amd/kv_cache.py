@@ -33,6 +33,7 @@ __all__ = ["KVCache", "create_kv_cache", "kv_cache_write", "kv_cache_read", "cac
 
 _E4M3 = torch.float8_e4m3fn
 _E8M0 = torch.float8_e8m0fnu
+_MOST = (1 << 31) - 1  # sizes are 32-bit numbers in the C ABI
 
 
 class KVCache(NamedTuple):
@@ -112,6 +113,8 @@ def _check_rows(x: torch.Tensor, name: str, index: int, head_dim: int) -> Tuple[
         raise ValueError(f"{name} must be on the cache's device")
     if shape[3] != head_dim:
         raise ValueError(f"{name} has head dim {shape[3]}, the cache {head_dim}")
+    if shape[1] > _MOST:
+        raise NotImplementedError(f"{name} has {shape[1]} tokens per item (at most 2^31 - 1)")
     return shape
 
 
