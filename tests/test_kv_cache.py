@@ -1100,6 +1100,21 @@ def test_more_tokens_than_32_bits_count_are_refused(gpu):
 
 
 @pytest.mark.gpu
+def test_outputs_that_cannot_hold_the_values_are_refused(gpu):
+    """Views that negate what they hold, or hold several values in one place."""
+    c = vx.create_kv_cache(2, 64, 2, 64, device=gpu)
+    x = torch.ones((2, 3, 2, 64), dtype=torch.bfloat16, device=gpu)
+    vx.kv_cache_write(c, x, x)
+    out = torch.full_like(x, 7.0)
+    for bad in (torch._neg_view(out), out[:1].expand(2, 3, 2, 64), out[:, :1].expand(2, 3, 2, 64)):
+        with pytest.raises(ValueError, match="out must be"):
+            vx.cached_attention(x, c, [3, 3], out=bad)
+    assert (out == 7.0).all()
+    assert vx.cached_attention(x[:1], c, [3], out=out[:1].expand(1, 3, 2, 64)).data_ptr() == out.data_ptr()
+    assert (out[0] == 1.0).all()
+
+
+@pytest.mark.gpu
 def test_refusals_of_gpu_calls(gpu):
     c = vx.create_kv_cache(2, 64, 2, 64, device=gpu)
     x = torch.zeros((2, 3, 2, 64), dtype=torch.bfloat16, device=gpu)

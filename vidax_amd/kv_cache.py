@@ -263,6 +263,8 @@ def _attend(q: torch.Tensor, cache: KVCache, prefix: Optional[KVCache], kv_len, 
         out = torch.empty_like(q) if not empty and q_strides is None else torch.empty(shape, dtype=q.dtype, device=dev)
     elif out.shape != shape or out.dtype != q.dtype or out.stride(-1) != 1 or out.device != dev:
         raise ValueError("out must be a (B, Sq, H, D) bf16 tensor with a contiguous head dim, on q's device")
+    elif out.is_neg() or any(st == 0 and n > 1 for st, n in zip(out.stride(), shape)):
+        raise ValueError("out must be a tensor that holds its values as they are, each in memory of its own")
     else:
         out_strides = _strides3(out)
     if empty:
