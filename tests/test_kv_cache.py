@@ -659,6 +659,30 @@ def test_nan_rows_in_every_kernel_of_the_plan(gpu, case, which):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("case", PLANS, ids=PLAN_IDS)
+def test_queries_that_are_not_finite(gpu, case):
+    """A NaN and an infinite query row become NaN, whatever their neighbours in a tile."""
+    kernel, _, B, Sq, H, Hk, D, cap, kv_len, q_len, causal, groups, p_cap, p_len = case
+    print(f"[case] {case}", flush=True)
+    rng = np.random.default_rng(Sq + cap + p_cap)
+    cache = _cache_of(rng, B, Hk, cap, D, gpu, kv_len)
+    prefix = _cache_of(rng, groups, Hk, p_cap, D, gpu, p_len) if groups else None
+    q = _bf16(2 * rng.standard_normal((B, Sq, H, D)), gpu)
+    b = int(np.argmax(np.minimum(kv_len, q_len or [Sq] * B)))
+    last = (q_len[b] if q_len else Sq) - 1
+    q[b, last, 0], q[b, last, H - 1] = 0.0, 0.0
+    finite = _attend(case, gpu, cache, prefix, q)
+    bad = q.clone()
+    bad[b, last, 0, 5], bad[b, last, H - 1] = float("nan"), float("inf")
+    got = _attend(case, gpu, cache, prefix, bad)
+    want = torch.zeros(got.shape, dtype=torch.bool, device=gpu)
+    want[b, last, 0], want[b, last, H - 1] = True, True
+    assert torch.equal(got.isnan(), want)
+    _assert_close(torch.where(want, finite, got), q, _held(cache, kv_len), _held(prefix, p_len) if groups else None,
+                  kv_len=kv_len, q_len=q_len, causal=causal, **(dict(prefix_len=p_len) if groups else {}))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("case", [PLANS[0], PLANS[4], PLANS[11], None], ids=["many", "many in parts", "prefix", "expanded"])
 def test_graph_replays_of_long_calls(gpu, case):
     """Captured calls of many queries (with prefixes, in parts, expanded to bf16),
