@@ -25,13 +25,13 @@
 // barrier in the loop), and converts them behind the LDS reads: K with its scale in
 // the same instruction, V unscaled, its scales multiplied into the weights, since
 // the transposed read gives a lane eight keys of one dim. It is bound by memory for
-// single tokens: 64 sequences of 227 to 8192 keys, 8 kv heads, 562 MB in 107 us (5.2
-// TB/s); two of 131000 and 105009 keys 488 MB in 89 us (5.5 TB/s).
+// single tokens: 64 sequences of 227 to 8192 keys, 8 kv heads, 562 MB in 105 us (5.4
+// TB/s); two of 131000 and 105009 keys 488 MB in 90 us (5.4 TB/s).
 // many_part converts each 64-key tile once for its four waves, on the way to LDS,
 // and runs the matrix cores of a tile beside the next one's softmax and conversions:
-// 1000 and 943 queries of 32 heads on 5003 and 4324 keys 136 to 145 us (0.92 to 0.98
-// PFLOP/s; the matrix cores are busy 43 % of the launch, which is one round of
-// workgroups of unequal length).
+// 1000 and 943 queries of 32 heads on 5003 and 4324 keys 138 us (0.96 PFLOP/s; 150 to
+// 175 us in the first calls after an idle time). The matrix cores are busy 44 % of that
+// and the VALU 45 %: a tile's products and its softmax and conversions hardly overlap.
 #include "vx_fp8_cache.hpp"
 #include "vx_kernels.h"
 

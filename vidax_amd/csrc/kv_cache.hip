@@ -14,8 +14,8 @@
 // cache's. A wave takes 16 positions of one head, keys and values (all its loads
 // in flight before the first is used), and neighbouring waves neighbouring
 // heads, whose bf16 rows lie side by side.
-// Measured: 32760 positions of 40 heads of 128 read in 219 to 248 us (4.1 to 4.6 TB/s;
-// a copy of 1 GiB runs at 4.8), 7800 of 12 heads written in 13 us and read back in 15
+// Measured: 32760 positions of 40 heads of 128 read in 214 to 257 us (3.9 to 4.7 TB/s;
+// a copy of 1 GiB runs at 5.2), 7800 of 12 heads written in 13 us and read back in 16
 // (partly from cache). Not kept: non-temporal stores (32760 positions 248 -> 363
 // us), 32 or 64 positions per wave (40 heads of 128: 512 positions 8.5, 9.1 and 9.1 us,
 // 8192 41, 42 and 39, 32768 249, 236 and 238; 16 heads of 64, 32768 33.6, 34.7 and 41.7).
