@@ -1037,7 +1037,7 @@ def test_host_integers_wait_for_nothing(gpu, host):
         made.append(host(v))
         return made[-1]
 
-    for c in caches[1:]:  # (the first round may still allocate)
+    for c in caches[1:]:  # (the first pass may still allocate)
         torch.cuda.synchronize()
         for _ in range(40):  # about 35 ms
             torch.matmul(work, work)
