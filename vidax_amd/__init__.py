@@ -11,10 +11,14 @@ and the q/k prologue in front of them:
   apply_abs_rope3d, na3d_qk_norm_rope     (src/vidax/models/ltx2_5/diffusion_vae.py)
 and an 8-bit key/value cache with the attention over it:
   KVCache, create_kv_cache, kv_cache_write, kv_cache_read, cached_attention, shared_prefix_attention
-all backed by libvx_attn.so (C ABI: include/vx_attn.h, include/vx_cache.h).
+and the steps of a rollout or a decoding loop over that cache:
+  AxisRope, create_axis_rope, apply_axis_rope, kv_cache_write_rope, windowed_attention, tree_attention
+all backed by libvx_attn.so (C ABI: include/vx_attn.h, include/vx_cache.h, include/vx_decode.h).
 """
 from .attention import (dot_product_attention, flash_attention, flash_supported, local_attention,
                         masked_self_attention)
+from .decode import (AxisRope, apply_axis_rope, create_axis_rope, kv_cache_write_rope, tree_attention,
+                     windowed_attention)
 from .kv_cache import (KVCache, cached_attention, create_kv_cache, kv_cache_read, kv_cache_write,
                        shared_prefix_attention)
 from .natten import na3d_block_attention, neighborhood_attention_3d
@@ -46,4 +50,10 @@ __all__ = [
     "kv_cache_read",
     "cached_attention",
     "shared_prefix_attention",
+    "AxisRope",
+    "create_axis_rope",
+    "apply_axis_rope",
+    "kv_cache_write_rope",
+    "windowed_attention",
+    "tree_attention",
 ]

@@ -1,5 +1,5 @@
-"""ctypes binding of libvx_attn.so (the C ABI in include/vx_attn.h and
-include/vx_cache.h).
+"""ctypes binding of libvx_attn.so (the C ABI in include/vx_attn.h,
+include/vx_cache.h and include/vx_decode.h).
 
 torch is imported before the library is opened so that the library binds to
 the HIP runtime torch already loaded (both resolve `libamdhip64.so.7`): device
@@ -63,6 +63,20 @@ CACHE_SYMBOLS = (  # include/vx_cache.h
     "vx_cached_attn_workspace_size",
 )
 
+DECODE_SYMBOLS = (  # include/vx_decode.h
+    "vx_decode_abi_version",
+    "vx_axis_rope_fwd",
+    "vx_axis_rope_check",
+    "vx_kv_write_rope_fwd",
+    "vx_kv_write_rope_check",
+    "vx_window_attn_fwd",
+    "vx_window_attn_check",
+    "vx_window_attn_workspace_size",
+    "vx_tree_attn_fwd",
+    "vx_tree_attn_check",
+    "vx_tree_attn_workspace_size",
+)
+
 _lock = threading.Lock()
 _lib = None
 
@@ -84,6 +98,11 @@ _PROLOGUE_ARGS = [_p, _p, _p, _f32, _i32, _p, _p, _i64, _i32, _i32, _i32, _i32, 
 _KV_WRITE_ARGS = [_p, _p, _i64p, _i64p] + [_p] * 4 + [_i32, _i32, _p, _p, _p] + [_i32] * 4
 _KV_READ_ARGS = [_p] * 4 + [_i32, _i32, _p, _p] + [_i32] * 4 + [_p, _p]
 _CACHED_ATTN_ARGS = [_p, _p, _i64p, _i64p] + ([_p] * 4 + [_i32, _i32]) * 2 + [_p] * 4 + [_i32] * 6 + [_f32]
+_ROPE_ARGS = [_p, _i64p, _i32, _p, _p, _i32]  # positions, strides, axes, turns, axis, halves
+_AXIS_ROPE_ARGS = [_p, _p, _i64p] + _ROPE_ARGS + [_i32] * 5
+_KV_WRITE_ROPE_ARGS = _KV_WRITE_ARGS[:-4] + _ROPE_ARGS + [_i32] * 4
+_WINDOW_ATTN_ARGS = [_p, _p, _i64p, _i64p] + [_p] * 4 + [_i32, _i32] + [_p] * 3 + [_i32] * 8 + [_f32]
+_TREE_ATTN_ARGS = [_p, _p, _i64p, _i64p] + [_p] * 4 + [_i32, _i32] + [_p] * 4 + [_i64] + [_i32] * 5 + [_f32]
 _SCALED_PROLOGUE_ARGS = _PROLOGUE_ARGS[:5] + [_f32] + _PROLOGUE_ARGS[5:]
 
 
@@ -180,6 +199,18 @@ def lib() -> ctypes.CDLL:
             h.vx_cached_attn_check.argtypes = _CACHED_ATTN_ARGS
             h.vx_cached_attn_workspace_size.restype = _i64
             h.vx_cached_attn_workspace_size.argtypes = [_i32] * 9
+            h.vx_decode_abi_version.restype = _i32
+            h.vx_decode_abi_version.argtypes = []
+            for name, args, more in (("axis_rope", _AXIS_ROPE_ARGS, []), ("kv_write_rope", _KV_WRITE_ROPE_ARGS, []),
+                                     ("window_attn", _WINDOW_ATTN_ARGS, [_p, _i64]),
+                                     ("tree_attn", _TREE_ATTN_ARGS, [_p, _i64])):
+                for entry, types in ((f"vx_{name}_fwd", args + more + [_p]), (f"vx_{name}_check", args)):
+                    getattr(h, entry).restype = _i32
+                    getattr(h, entry).argtypes = types
+            h.vx_window_attn_workspace_size.restype = _i64
+            h.vx_window_attn_workspace_size.argtypes = [_i32] * 9
+            h.vx_tree_attn_workspace_size.restype = _i64
+            h.vx_tree_attn_workspace_size.argtypes = [_i32] * 6
             h.vx_last_launch.restype = ctypes.c_char_p
             h.vx_last_launch.argtypes = []
             _lib = h

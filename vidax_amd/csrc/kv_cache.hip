@@ -19,7 +19,7 @@
 // (partly from cache). Not kept: non-temporal stores (32760 positions 248 -> 363
 // us), 32 or 64 positions per wave (40 heads of 128: 512 positions 8.5, 9.1 and 9.1 us,
 // 8192 41, 42 and 39, 32768 249, 236 and 238; 16 heads of 64, 32768 33.6, 34.7 and 41.7).
-#include "vx_fp8_cache.hpp"
+#include "vx_axis_rope.hpp"
 #include "vx_kernels.h"
 
 #include <algorithm>
@@ -70,8 +70,41 @@ __device__ __forceinline__ u32x4 quantise(const u32x4 (&x)[2], uint32_t s) {
   return y;
 }
 
+// Largest magnitude of 16 fp32 values, over the lanes of their row, as bits.
 template <int D>
-__global__ __launch_bounds__(kWaves * 64) void kv_write_kernel(const KvWriteArgs a) {
+__device__ __forceinline__ uint32_t row_amax(const float (&x)[2][8]) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r = max(r, __float_as_uint(x[i >> 3][i & 7]) & 0x7fffffffu);
+#pragma unroll
+  for (int off = 1; off < Rows<D>::kLanes; off <<= 1) r = max(r, (uint32_t)__shfl_xor((int)r, off, 64));
+  return r;
+}
+
+// Scale byte of a row with this largest magnitude (fp32 bits).
+__device__ __forceinline__ uint32_t scale_byte32(uint32_t amax) {
+  const int e = (int)(amax >> 23);
+  return e == 255 ? 255u : (uint32_t)max(e - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0), 1);
+}
+
+// 16 fp32 values times 2^(127 - s), rounded to e4m3 (zeros for a row of scale NaN).
+__device__ __forceinline__ u32x4 quantise(const float (&x)[2][8], uint32_t s) {
+  const float f = __uint_as_float((254u - s) << 23);
+  u32x4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float* v = &x[i >> 1][4 * (i & 1)];
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * f, v[1] * f, 0, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * f, v[3] * f, r, true);
+    y[i] = s == 255u ? 0u : (uint32_t)r;
+  }
+  return y;
+}
+
+// PAIRS: keys are turned (kNoRope: as they are) on the way, in fp32, and rounded once.
+// Then lanes take their channels as the pairs lie (see vx_axis_rope.hpp).
+template <int D, int PAIRS>
+__device__ __forceinline__ void write_rows(const KvWriteArgs& a, const AxisRope& rope) {
   using R = Rows<D>;
   const int lane = threadIdx.x & 63;
   const uint32_t w = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -86,18 +119,30 @@ __global__ __launch_bounds__(kWaves * 64) void kv_write_kernel(const KvWriteArgs
   const int r = lane / R::kLanes, c = lane % R::kLanes;
   bool keep[R::kPasses];
   u32x4 xk[R::kPasses][2], xv[R::kPasses][2];
+  RopePlace place[R::kPasses];
 #pragma unroll
   for (int p = 0; p < R::kPasses; ++p) {
     const int64_t t = t0 + p * R::kPerPass + r, pos = first + t;
     keep[p] = t < n && pos >= 0 && pos < a.c.cap;
     const int64_t ti = min(t, (int64_t)n - 1);  // (rows past the end load the last one)
-    const bf16* pk = (const bf16*)a.k + b * a.ks[0] + ti * a.ks[1] + head * a.ks[2] + c * 16;
-    const bf16* pv = (const bf16*)a.v + b * a.vs[0] + ti * a.vs[1] + head * a.vs[2] + c * 16;
+    if constexpr (PAIRS == kHalves) {
+      const bf16* pk = (const bf16*)a.k + b * a.ks[0] + ti * a.ks[1] + head * a.ks[2] + c * 8;
+      const bf16* pv = (const bf16*)a.v + b * a.vs[0] + ti * a.vs[1] + head * a.vs[2] + c * 8;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      xk[p][i] = *(const u32x4*)(pk + 8 * i);
-      xv[p][i] = *(const u32x4*)(pv + 8 * i);
+      for (int i = 0; i < 2; ++i) {
+        xk[p][i] = *(const u32x4*)(pk + D / 2 * i);
+        xv[p][i] = *(const u32x4*)(pv + D / 2 * i);
+      }
+    } else {
+      const bf16* pk = (const bf16*)a.k + b * a.ks[0] + ti * a.ks[1] + head * a.ks[2] + c * 16;
+      const bf16* pv = (const bf16*)a.v + b * a.vs[0] + ti * a.vs[1] + head * a.vs[2] + c * 16;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        xk[p][i] = *(const u32x4*)(pk + 8 * i);
+        xv[p][i] = *(const u32x4*)(pv + 8 * i);
+      }
     }
+    if constexpr (PAIRS != kNoRope) place[p] = rope_place(rope, b * rope.ps[0] + ti * rope.ps[1]);
   }
   // Positions that a later batch item writes in the same slot are left to it,
   // so that no row mixes two tokens' values and scales.
@@ -124,18 +169,50 @@ __global__ __launch_bounds__(kWaves * 64) void kv_write_kernel(const KvWriteArgs
   const int64_t row0 = ((int64_t)slot * hk + head) * a.c.cap;
 #pragma unroll
   for (int p = 0; p < R::kPasses; ++p) {
-    const uint32_t sk = scale_byte(row_amax<D>(xk[p])), sv = scale_byte(row_amax<D>(xv[p]));
-    const u32x4 yk = quantise(xk[p], sk), yv = quantise(xv[p], sv);
+    uint32_t sk;
+    float y[2][8];  // keys, turned
+    if constexpr (PAIRS == kNoRope) {
+      sk = scale_byte(row_amax<D>(xk[p]));
+    } else {
+      float s[8], co[8];
+      rope_angles(rope_table<D>(rope, c), place[p], false, s, co);
+      rope_turn<PAIRS>(xk[p], s, co, y);
+      sk = scale_byte32(row_amax<D>(y));
+    }
+    const uint32_t sv = scale_byte(row_amax<D>(xv[p]));
+    u32x4 yk;
+    if constexpr (PAIRS == kNoRope)
+      yk = quantise(xk[p], sk);
+    else
+      yk = quantise(y, sk);
+    const u32x4 yv = quantise(xv[p], sv);
     if (keep[p]) {
       const int64_t row = row0 + first + t0 + p * R::kPerPass + r;
-      *(u32x4*)(a.c.k + row * D + c * 16) = yk;
-      *(u32x4*)(a.c.v + row * D + c * 16) = yv;
+      if constexpr (PAIRS == kHalves) {
+        *(u32x2*)(a.c.k + row * D + c * 8) = u32x2{yk[0], yk[1]};
+        *(u32x2*)(a.c.k + row * D + D / 2 + c * 8) = u32x2{yk[2], yk[3]};
+        *(u32x2*)(a.c.v + row * D + c * 8) = u32x2{yv[0], yv[1]};
+        *(u32x2*)(a.c.v + row * D + D / 2 + c * 8) = u32x2{yv[2], yv[3]};
+      } else {
+        *(u32x4*)(a.c.k + row * D + c * 16) = yk;
+        *(u32x4*)(a.c.v + row * D + c * 16) = yv;
+      }
       if (c == 0) {
         a.c.ks[row] = (uint8_t)sk;
         a.c.vs[row] = (uint8_t)sv;
       }
     }
   }
+}
+
+template <int D>
+__global__ __launch_bounds__(kWaves * 64) void kv_write_kernel(const KvWriteArgs a) {
+  write_rows<D, kNoRope>(a, AxisRope{});
+}
+
+template <int D, int PAIRS>
+__global__ __launch_bounds__(kWaves * 64) void kv_write_rope_kernel(const KvWriteArgs a, const AxisRope rope) {
+  write_rows<D, PAIRS>(a, rope);
 }
 
 template <int D>
@@ -241,6 +318,22 @@ int launch_kv_write(const KvWriteArgs& a, void* stream, const char** launched) {
   else
     hipLaunchKernelGGL(kv_write_kernel<64>, grid, dim3(kWaves * 64), 0, (hipStream_t)stream, a);
   *launched = a.c.D == 128 ? "kv_write_kernel<128>" : "kv_write_kernel<64>";
+  return (int)hipGetLastError();
+}
+
+int launch_kv_write_rope(const KvWriteArgs& a, const AxisRope& rope, void* stream, const char** launched) {
+  const dim3 grid = grid_of(a.B, a.S, a.c.Hk), threads(kWaves * 64);
+  const hipStream_t st = (hipStream_t)stream;
+  if (a.c.D == 128 && rope.halves)
+    hipLaunchKernelGGL((kv_write_rope_kernel<128, kHalves>), grid, threads, 0, st, a, rope);
+  else if (a.c.D == 128)
+    hipLaunchKernelGGL((kv_write_rope_kernel<128, kAdjacent>), grid, threads, 0, st, a, rope);
+  else if (rope.halves)
+    hipLaunchKernelGGL((kv_write_rope_kernel<64, kHalves>), grid, threads, 0, st, a, rope);
+  else
+    hipLaunchKernelGGL((kv_write_rope_kernel<64, kAdjacent>), grid, threads, 0, st, a, rope);
+  *launched = a.c.D == 128 ? (rope.halves ? "kv_write_rope_kernel<128, halves>" : "kv_write_rope_kernel<128, adjacent>")
+                           : (rope.halves ? "kv_write_rope_kernel<64, halves>" : "kv_write_rope_kernel<64, adjacent>");
   return (int)hipGetLastError();
 }
 

@@ -1,0 +1,79 @@
+// Attention over the 8-bit key/value cache whose queries see less than all tokens
+// up to theirs: a sliding window behind a few first tokens, or a tree of drafted
+// tokens. The kernels are those of cached_attn.hpp (few_part, many_part, merge),
+// which mask by a row's own rule in the tiles where its rows differ:
+//
+//   window  keys j < e with j >= e - window or j < sinks, e one past the query's
+//           position (causal) or past the last token. A stream's tiles are those
+//           of its sinks and of the union of its rows' windows, so the ranges that
+//           workgroups take hold no tile that nobody sees, and each tile of rows
+//           skips what its own rows do not see; only tiles at a row's border, at
+//           either end, are masked key by key.
+//   tree    keys in front of the drafted ones as ever; of those, the query's
+//           ancestors and itself, as bits in LDS that each row walks out from the
+//           parents once per part (fill_tree): a tile takes 32 of a row's bits from
+//           two words of them, one VALU instruction.
+#include "cached_attn.hpp"
+
+namespace vx {
+namespace {
+
+// Positions that a tile of rows sees at most, for the plan: of a cache of `cap`.
+int seen_most(int cap, int Sq, int G, int window, int sinks, bool causal) {
+  if (window == 0) return cap;
+  const int64_t queries = causal ? std::min(Sq, kManyRows / G + 1) : 1;
+  const int64_t most = ((int64_t)sinks + 63) / 64 * 64 + ((int64_t)window + queries + 63) / 64 * 64 + 64;
+  return (int)std::min<int64_t>(cap, most);
+}
+
+template <int D, int MASK>
+int launch(const MaskedAttnArgs& a, hipStream_t st, const char** launched) {
+  const int seen = seen_most(a.c.cap, a.Sq, a.H / a.c.Hk, a.window, a.sinks, a.causal != 0);
+  Plan pl = plan_of(seen, 0, 0, a.B, a.Sq, a.H, a.c.Hk, D);
+  Part& own = pl.own.p;
+  own.s = Streams{a.c, a.kv_len, a.slots, a.B};
+  own.ws = a.ws;
+  const dim3 grid((unsigned)pl.own.blocks), threads(kThreads);
+  if (own.few && pl.wide) {
+    hipLaunchKernelGGL((few_masked_kernel<D, 8, MASK>), grid, dim3(512), 0, st, a, own);
+    *launched = MASK == kTree ? (D == 128 ? "few_masked_kernel<128, 8, tree>" : "few_masked_kernel<64, 8, tree>")
+                              : (D == 128 ? "few_masked_kernel<128, 8, window>" : "few_masked_kernel<64, 8, window>");
+  } else if (own.few) {
+    hipLaunchKernelGGL((few_masked_kernel<D, 4, MASK>), grid, threads, 0, st, a, own);
+    *launched = MASK == kTree ? (D == 128 ? "few_masked_kernel<128, 4, tree>" : "few_masked_kernel<64, 4, tree>")
+                              : (D == 128 ? "few_masked_kernel<128, 4, window>" : "few_masked_kernel<64, 4, window>");
+  } else {
+    hipLaunchKernelGGL((many_masked_kernel<D, MASK>), grid, threads, 0, st, a, own);
+    *launched = MASK == kTree ? (D == 128 ? "many_masked_kernel<128, tree>" : "many_masked_kernel<64, tree>")
+                              : (D == 128 ? "many_masked_kernel<128, window>" : "many_masked_kernel<64, window>");
+  }
+  int err = (int)hipGetLastError();
+  if (err == 0 && own.budget > 0) {
+    const int split = merge_split(pl.own.usual_parts, D);
+    const int64_t per_wg = kThreads / (D / 4) / split;
+    // (a tree's ranges are those of all its keys)
+    constexpr int kRanges = MASK == kWindow ? kWindow : kPlain;
+    hipLaunchKernelGGL((merge_kernel<D, kRanges>),
+                       dim3((unsigned)(((int64_t)a.c.Hk * own.rows + per_wg - 1) / per_wg), a.B), threads, 0, st, a,
+                       own, Part{}, split);
+    err = (int)hipGetLastError();
+  }
+  return err;
+}
+
+}  // namespace
+
+int64_t masked_attn_workspace(int32_t cap, int32_t B, int32_t Sq, int32_t H, int32_t Hk, int32_t D, int32_t window,
+                              int32_t sinks, bool causal) {
+  const Plan p = plan_of(seen_most(cap, Sq, H / Hk, window, sinks, causal), 0, 0, B, Sq, H, Hk, D);
+  return p.own.floats * (int64_t)sizeof(float);
+}
+
+int launch_masked_attn(const MaskedAttnArgs& a, void* stream, const char** launched) {
+  const hipStream_t st = (hipStream_t)stream;
+  if (a.parents != nullptr)
+    return a.c.D == 128 ? launch<128, kTree>(a, st, launched) : launch<64, kTree>(a, st, launched);
+  return a.c.D == 128 ? launch<128, kWindow>(a, st, launched) : launch<64, kWindow>(a, st, launched);
+}
+
+}  // namespace vx

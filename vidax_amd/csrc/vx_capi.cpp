@@ -1,10 +1,10 @@
 // C ABI of the attention kernels (declared in include/vx_attn.h) and of the 8-bit
-// cache (include/vx_cache.h).
+// cache (include/vx_cache.h, include/vx_decode.h).
 //
 // Plain C++ with no HIP dependency: argument checks, error reporting and the
 // failure-injection hook run on a host without a GPU. The kernels are reached
 // through vx::launch_* (flash_fwd.hip, na3d_fwd.hip, qk_prologue.hip, kv_cache.hip,
-// cached_attn.hip).
+// cached_attn.hip, masked_attn.hip, axis_rope.hip).
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -18,6 +18,7 @@
 
 #include "../../include/vx_attn.h"
 #include "../../include/vx_cache.h"
+#include "../../include/vx_decode.h"
 #include "vx_kernels.h"
 
 namespace {
@@ -799,6 +800,129 @@ int32_t cached_attn_check(const void* q, const void* out, const int64_t* qs, con
   return ok();
 }
 
+// ---- rotary positions, and attention of less than all keys
+int32_t axis_rope_check(const int32_t* positions, const int64_t* strides, int32_t axes, const uint64_t* turns,
+                        const int32_t* axis, int32_t halves, vx::AxisRope* r) {
+  if (positions == nullptr || strides == nullptr || turns == nullptr || axis == nullptr)
+    return fail(VX_ERR_INVALID_ARGUMENT, "positions, position_strides, turns and axis must be non-NULL");
+  if (!aligned4(positions) || !aligned4(axis) || (reinterpret_cast<uintptr_t>(turns) & 7u) != 0)
+    return fail(VX_ERR_INVALID_ARGUMENT, "positions and axis must be 4-byte, turns 8-byte aligned");
+  if (axes < 1 || axes > vx::kRopeAxes)
+    return fail(VX_ERR_UNSUPPORTED, "num_axes (%d) must be in 1..%d", axes, vx::kRopeAxes);
+  if (halves != 0 && halves != 1) return fail(VX_ERR_INVALID_ARGUMENT, "halves must be 0 or 1");
+  for (int i = 0; i < 3; ++i) {
+    if (strides[i] < 0) return fail(VX_ERR_INVALID_ARGUMENT, "position_strides must be >= 0");
+    r->ps[i] = strides[i];
+  }
+  r->positions = positions;
+  r->axes = axes;
+  r->turns = turns;
+  r->axis = axis;
+  r->halves = halves;
+  return VX_OK;
+}
+
+int32_t axis_rope_args(const void* x, const void* out, const int64_t* xs, const int32_t* positions,
+                       const int64_t* ps, int32_t axes, const uint64_t* turns, const int32_t* axis, int32_t halves,
+                       int32_t inverse, int32_t B, int32_t S, int32_t H, int32_t D, vx::AxisRopeArgs* a) {
+  if (x == nullptr || out == nullptr) return fail(VX_ERR_INVALID_ARGUMENT, "x and out must be non-NULL");
+  if (!aligned16(x) || !aligned16(out)) return fail(VX_ERR_INVALID_ARGUMENT, "x and out must be 16-byte aligned");
+  if (B < 1 || B > 65535) return fail(VX_ERR_INVALID_ARGUMENT, "batch (%d) must be in 1..65535", B);
+  if (S < 1) return fail(VX_ERR_INVALID_ARGUMENT, "seq (%d) must be >= 1", S);
+  if (H < 1 || H > 65535) return fail(VX_ERR_INVALID_ARGUMENT, "num_heads (%d) must be in 1..65535", H);
+  if (D != 64 && D != 128)
+    return fail(VX_ERR_UNSUPPORTED, "head_dim %d is not supported (this build handles 64 and 128)", D);
+  if (inverse != 0 && inverse != 1) return fail(VX_ERR_INVALID_ARGUMENT, "inverse must be 0 or 1");
+  int32_t rc;
+  if ((rc = axis_rope_check(positions, ps, axes, turns, axis, halves, &a->rope)) != VX_OK) return rc;
+  strides_or_default(xs, S, H, D, a->xs);
+  if ((rc = check_strides("x", a->xs, S)) != VX_OK) return rc;
+  // (a grid's threads, 64 for 32 heads of a token at most, are counted in 32 bits)
+  if ((int64_t)S * ((H + 31) / 32) > (INT32_MAX >> 5) - 4)
+    return fail(VX_ERR_UNSUPPORTED, "seq (%d) times num_heads (%d) is too large", S, H);
+  a->x = x;
+  a->o = const_cast<void*>(out);
+  a->inverse = inverse;
+  a->B = B;
+  a->S = S;
+  a->H = H;
+  a->D = D;
+  return ok();
+}
+
+int32_t window_check(int32_t window, int32_t sinks) {
+  if (window < 1 || sinks < 0)
+    return fail(VX_ERR_INVALID_ARGUMENT, "window (%d) must be >= 1 and sinks (%d) >= 0", window, sinks);
+  return VX_OK;
+}
+
+int32_t tree_check(int32_t Sq) {
+  if (Sq > vx::kTreeMost)
+    return fail(VX_ERR_UNSUPPORTED, "%d drafted tokens are too many (at most %d)", Sq, vx::kTreeMost);
+  return VX_OK;
+}
+
+// Checks the sizes of a masked call and gives its workspace (-1: refused).
+int64_t masked_workspace(int32_t cap, int32_t B, int32_t Sq, int32_t H, int32_t Hk, int32_t D, int32_t window,
+                         int32_t sinks, bool causal) {
+  vx::KvCache c;
+  const void* some = reinterpret_cast<const void*>(uintptr_t(1) << 20);  // (an aligned address, not looked at)
+  const uint8_t* scales = static_cast<const uint8_t*>(some);
+  if (cache_check("cache", some, some, scales, scales, 1, cap, Hk, D, &c) != VX_OK ||
+      cached_sizes_check(cap, 0, 0, B, Sq, H, Hk) != VX_OK)
+    return -1;
+  ok();
+  return vx::masked_attn_workspace(cap, B, Sq, H, Hk, D, window, sinks, causal);
+}
+
+int32_t masked_launch(vx::MaskedAttnArgs& a, int64_t need, void* workspace, int64_t bytes, void* stream) {
+  if (need < 0) return VX_ERR_INVALID_ARGUMENT;  // (its message)
+  if (need > 0 && (workspace == nullptr || !aligned16(workspace) || bytes < need))
+    return fail(VX_ERR_INVALID_ARGUMENT, "a 16-byte aligned workspace of %lld bytes is needed (%lld given)",
+                (long long)need, (long long)(workspace != nullptr ? bytes : 0));
+  a.ws = static_cast<float*>(workspace);
+  const char* launched = "";
+  const int err = vx::launch_masked_attn(a, stream, &launched);
+  if (err != 0) return fail(VX_ERR_LAUNCH, "masked attention launch failed (hipError_t %d)", err);
+  g_last_launch = launched;
+  return ok();
+}
+
+int32_t window_attn_check(const void* q, const void* out, const int64_t* qs, const int64_t* os, const void* ck,
+                          const void* cv, const uint8_t* cks, const uint8_t* cvs, int32_t slots, int32_t cap,
+                          const int32_t* kv_len, const int32_t* q_len, const int32_t* slot_of, int32_t B, int32_t Sq,
+                          int32_t H, int32_t Hk, int32_t D, int32_t window, int32_t sinks, int32_t causal,
+                          float scale, vx::MaskedAttnArgs* a) {
+  int32_t rc;
+  if ((rc = cached_attn_check(q, out, qs, os, ck, cv, cks, cvs, slots, cap, nullptr, nullptr, nullptr, nullptr, 0, 0,
+                              kv_len, q_len, slot_of, nullptr, B, Sq, H, Hk, D, causal, scale, a)) != VX_OK)
+    return rc;
+  if ((rc = window_check(window, sinks)) != VX_OK) return rc;
+  a->window = window;
+  a->sinks = sinks;
+  a->parents = nullptr;
+  a->parents_stride = 0;
+  return VX_OK;
+}
+
+int32_t tree_attn_check(const void* q, const void* out, const int64_t* qs, const int64_t* os, const void* ck,
+                        const void* cv, const uint8_t* cks, const uint8_t* cvs, int32_t slots, int32_t cap,
+                        const int32_t* kv_len, const int32_t* q_len, const int32_t* slot_of, const int32_t* parents,
+                        int64_t parents_stride, int32_t B, int32_t Sq, int32_t H, int32_t Hk, int32_t D, float scale,
+                        vx::MaskedAttnArgs* a) {
+  int32_t rc;
+  if ((rc = cached_attn_check(q, out, qs, os, ck, cv, cks, cvs, slots, cap, nullptr, nullptr, nullptr, nullptr, 0, 0,
+                              kv_len, q_len, slot_of, nullptr, B, Sq, H, Hk, D, 1, scale, a)) != VX_OK)
+    return rc;
+  if ((rc = tree_check(Sq)) != VX_OK) return rc;
+  if (parents == nullptr || !aligned4(parents) || parents_stride < 0)
+    return fail(VX_ERR_INVALID_ARGUMENT, "parents must be non-NULL and 4-byte aligned, parents_stride >= 0");
+  a->window = a->sinks = 0;
+  a->parents = parents;
+  a->parents_stride = parents_stride;
+  return VX_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1361,6 +1485,137 @@ int64_t vx_cached_attn_workspace_size(int32_t capacity, int32_t num_prefixes, in
     return 2 * expanded_bytes(capacity, batch, num_kv_heads, head_dim) + 4 * (int64_t)batch;
   return vx::cached_attn_workspace(capacity, num_prefixes, prefix_capacity, batch, seq_q, num_heads, num_kv_heads,
                                    head_dim);
+}
+
+int32_t vx_decode_abi_version(void) { return 10000; }
+
+int32_t vx_axis_rope_check(const void* x, const void* out, const int64_t* x_strides, const int32_t* positions,
+                           const int64_t* position_strides, int32_t num_axes, const uint64_t* turns,
+                           const int32_t* axis, int32_t halves, int32_t inverse, int32_t batch, int32_t seq,
+                           int32_t num_heads, int32_t head_dim) {
+  vx::AxisRopeArgs a;
+  return axis_rope_args(x, out, x_strides, positions, position_strides, num_axes, turns, axis, halves, inverse, batch,
+                        seq, num_heads, head_dim, &a);
+}
+
+int32_t vx_axis_rope_fwd(const void* x, void* out, const int64_t* x_strides, const int32_t* positions,
+                         const int64_t* position_strides, int32_t num_axes, const uint64_t* turns,
+                         const int32_t* axis, int32_t halves, int32_t inverse, int32_t batch, int32_t seq,
+                         int32_t num_heads, int32_t head_dim, void* stream) {
+  vx::AxisRopeArgs a;
+  int32_t rc = axis_rope_args(x, out, x_strides, positions, position_strides, num_axes, turns, axis, halves, inverse,
+                              batch, seq, num_heads, head_dim, &a);
+  if (rc != VX_OK) return rc;
+  if ((rc = injected()) != VX_OK) return rc;
+  const char* launched = "";
+  const int err = vx::launch_axis_rope(a, stream, &launched);
+  if (err != 0) return fail(VX_ERR_LAUNCH, "axis rope launch failed (hipError_t %d)", err);
+  g_last_launch = launched;
+  return ok();
+}
+
+int32_t vx_kv_write_rope_check(const void* k, const void* v, const int64_t* k_strides, const int64_t* v_strides,
+                               const void* cache_k, const void* cache_v, const uint8_t* k_scale,
+                               const uint8_t* v_scale, int32_t num_slots, int32_t capacity, const int32_t* start,
+                               const int32_t* num, const int32_t* slots, const int32_t* positions,
+                               const int64_t* position_strides, int32_t num_axes, const uint64_t* turns,
+                               const int32_t* axis, int32_t halves, int32_t batch, int32_t seq, int32_t num_kv_heads,
+                               int32_t head_dim) {
+  vx::KvWriteArgs a;
+  vx::AxisRope r;
+  int32_t rc;
+  if ((rc = axis_rope_check(positions, position_strides, num_axes, turns, axis, halves, &r)) != VX_OK) return rc;
+  return kv_write_check(k, v, k_strides, v_strides, cache_k, cache_v, k_scale, v_scale, num_slots, capacity, start,
+                        num, slots, batch, seq, num_kv_heads, head_dim, &a);
+}
+
+int32_t vx_kv_write_rope_fwd(const void* k, const void* v, const int64_t* k_strides, const int64_t* v_strides,
+                             void* cache_k, void* cache_v, uint8_t* k_scale, uint8_t* v_scale, int32_t num_slots,
+                             int32_t capacity, const int32_t* start, const int32_t* num, const int32_t* slots,
+                             const int32_t* positions, const int64_t* position_strides, int32_t num_axes,
+                             const uint64_t* turns, const int32_t* axis, int32_t halves, int32_t batch, int32_t seq,
+                             int32_t num_kv_heads, int32_t head_dim, void* stream) {
+  vx::KvWriteArgs a;
+  vx::AxisRope r;
+  int32_t rc;
+  if ((rc = axis_rope_check(positions, position_strides, num_axes, turns, axis, halves, &r)) != VX_OK ||
+      (rc = kv_write_check(k, v, k_strides, v_strides, cache_k, cache_v, k_scale, v_scale, num_slots, capacity, start,
+                           num, slots, batch, seq, num_kv_heads, head_dim, &a)) != VX_OK)
+    return rc;
+  if ((rc = injected()) != VX_OK) return rc;
+  const char* launched = "";
+  const int err = vx::launch_kv_write_rope(a, r, stream, &launched);
+  if (err != 0) return fail(VX_ERR_LAUNCH, "cache write launch failed (hipError_t %d)", err);
+  g_last_launch = launched;
+  return ok();
+}
+
+int32_t vx_window_attn_check(const void* q, const void* out, const int64_t* q_strides, const int64_t* out_strides,
+                             const void* cache_k, const void* cache_v, const uint8_t* k_scale,
+                             const uint8_t* v_scale, int32_t num_slots, int32_t capacity, const int32_t* kv_len,
+                             const int32_t* q_len, const int32_t* slots, int32_t batch, int32_t seq_q,
+                             int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t window,
+                             int32_t sinks, int32_t causal, float scale) {
+  vx::MaskedAttnArgs a;
+  return window_attn_check(q, out, q_strides, out_strides, cache_k, cache_v, k_scale, v_scale, num_slots, capacity,
+                           kv_len, q_len, slots, batch, seq_q, num_heads, num_kv_heads, head_dim, window, sinks, causal,
+                           scale, &a);
+}
+
+int32_t vx_window_attn_fwd(const void* q, void* out, const int64_t* q_strides, const int64_t* out_strides,
+                           const void* cache_k, const void* cache_v, const uint8_t* k_scale, const uint8_t* v_scale,
+                           int32_t num_slots, int32_t capacity, const int32_t* kv_len, const int32_t* q_len,
+                           const int32_t* slots, int32_t batch, int32_t seq_q, int32_t num_heads,
+                           int32_t num_kv_heads, int32_t head_dim, int32_t window, int32_t sinks, int32_t causal,
+                           float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+  vx::MaskedAttnArgs a;
+  int32_t rc = window_attn_check(q, out, q_strides, out_strides, cache_k, cache_v, k_scale, v_scale, num_slots,
+                                 capacity, kv_len, q_len, slots, batch, seq_q, num_heads, num_kv_heads, head_dim,
+                                 window, sinks, causal, scale, &a);
+  if (rc != VX_OK) return rc;
+  if ((rc = injected()) != VX_OK) return rc;
+  return masked_launch(a, masked_workspace(capacity, batch, seq_q, num_heads, num_kv_heads, head_dim, window, sinks,
+                                           causal != 0), workspace, workspace_bytes, stream);
+}
+
+int64_t vx_window_attn_workspace_size(int32_t capacity, int32_t batch, int32_t seq_q, int32_t num_heads,
+                                      int32_t num_kv_heads, int32_t head_dim, int32_t window, int32_t sinks,
+                                      int32_t causal) {
+  if (window_check(window, sinks) != VX_OK) return -1;
+  return masked_workspace(capacity, batch, seq_q, num_heads, num_kv_heads, head_dim, window, sinks, causal != 0);
+}
+
+int32_t vx_tree_attn_check(const void* q, const void* out, const int64_t* q_strides, const int64_t* out_strides,
+                           const void* cache_k, const void* cache_v, const uint8_t* k_scale, const uint8_t* v_scale,
+                           int32_t num_slots, int32_t capacity, const int32_t* kv_len, const int32_t* q_len,
+                           const int32_t* slots, const int32_t* parents, int64_t parents_stride, int32_t batch,
+                           int32_t seq_q, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale) {
+  vx::MaskedAttnArgs a;
+  return tree_attn_check(q, out, q_strides, out_strides, cache_k, cache_v, k_scale, v_scale, num_slots, capacity,
+                         kv_len, q_len, slots, parents, parents_stride, batch, seq_q, num_heads, num_kv_heads, head_dim,
+                         scale, &a);
+}
+
+int32_t vx_tree_attn_fwd(const void* q, void* out, const int64_t* q_strides, const int64_t* out_strides,
+                         const void* cache_k, const void* cache_v, const uint8_t* k_scale, const uint8_t* v_scale,
+                         int32_t num_slots, int32_t capacity, const int32_t* kv_len, const int32_t* q_len,
+                         const int32_t* slots, const int32_t* parents, int64_t parents_stride, int32_t batch,
+                         int32_t seq_q, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+                         void* workspace, int64_t workspace_bytes, void* stream) {
+  vx::MaskedAttnArgs a;
+  int32_t rc = tree_attn_check(q, out, q_strides, out_strides, cache_k, cache_v, k_scale, v_scale, num_slots, capacity,
+                               kv_len, q_len, slots, parents, parents_stride, batch, seq_q, num_heads, num_kv_heads,
+                               head_dim, scale, &a);
+  if (rc != VX_OK) return rc;
+  if ((rc = injected()) != VX_OK) return rc;
+  return masked_launch(a, masked_workspace(capacity, batch, seq_q, num_heads, num_kv_heads, head_dim, 0, 0, true),
+                       workspace, workspace_bytes, stream);
+}
+
+int64_t vx_tree_attn_workspace_size(int32_t capacity, int32_t batch, int32_t seq_q, int32_t num_heads,
+                                    int32_t num_kv_heads, int32_t head_dim) {
+  if (tree_check(seq_q) != VX_OK) return -1;
+  return masked_workspace(capacity, batch, seq_q, num_heads, num_kv_heads, head_dim, 0, 0, true);
 }
 
 }  // extern "C"

@@ -189,6 +189,28 @@ struct KvWriteArgs {
   int32_t B, S;
 };
 
+// How a token's pairs of channels turn: pair j by positions[b * ps[0] + t * ps[1] +
+// axis[j] * ps[2]] times turns[j], in units of 2^-64 turns.
+struct AxisRope {
+  const int32_t* positions;
+  int64_t ps[3];          // elements: {batch, token, axis}
+  int32_t axes;           // 1 .. kRopeAxes
+  const uint64_t* turns;  // [D / 2], as axis
+  const int32_t* axis;
+  int32_t halves;         // pairs (j, j + D / 2), else (2 j, 2 j + 1)
+};
+constexpr int kRopeAxes = 4;
+
+// Rows (B, S, H, D), turned or (inverse) turned back, to contiguous ones.
+struct AxisRopeArgs {
+  const void* x;
+  void* o;
+  int64_t xs[3];  // elements: {batch, seq, head}
+  AxisRope rope;
+  int32_t inverse;
+  int32_t B, S, H, D;
+};
+
 // Positions start[b] + t, t < S, of slot slots[b] to contiguous (B, S, Hk, D), or
 // (launch_kv_expand) the first limit[b] to (B, Hk, cap, D).
 struct KvReadArgs {
@@ -221,6 +243,19 @@ struct CachedAttnArgs {
   float* ws;
 };
 
+// Attention whose causal or whole view of an item's keys is narrowed: to `window`
+// keys up to the query's and the first `sinks` (parents null), or, of the last
+// q_len[b] keys, to those of the query's ancestors and its own (parents: of item b's
+// query i at parents[b * parents_stride + i], -1 or below i).
+struct MaskedAttnArgs : CachedAttnArgs {
+  int32_t window, sinks;
+  const int32_t* parents;
+  int64_t parents_stride;
+};
+
+// Most drafted tokens of an item.
+constexpr int kTreeMost = 512;
+
 // Compute units of the current device (0 if unknown), cached per device.
 int device_cu_count();
 
@@ -232,6 +267,10 @@ int noalloc_scratch(void** ptr, int64_t* bytes);
 int64_t cached_attn_workspace(int32_t cap, int32_t n_prefix, int32_t p_cap, int32_t B, int32_t Sq, int32_t H,
                               int32_t Hk, int32_t D);
 
+// The same for launch_masked_attn (window 0: a tree).
+int64_t masked_attn_workspace(int32_t cap, int32_t B, int32_t Sq, int32_t H, int32_t Hk, int32_t D, int32_t window,
+                              int32_t sinks, bool causal);
+
 // All return a hipError_t value (0 on success) and store the name of the kernel they launched in *launched (a string with
 // static storage, built from the launched instantiation's template
 // arguments).
@@ -241,9 +280,12 @@ int launch_qk_prologue(const PrologueArgs& a, void* stream, const char** launche
 int launch_key_masks(const KeyMaskArgs& a, void* stream, const char** launched);
 int launch_full_bias(const FullBiasArgs& a, void* stream, const char** launched);
 int launch_kv_write(const KvWriteArgs& a, void* stream, const char** launched);
+int launch_kv_write_rope(const KvWriteArgs& a, const AxisRope& rope, void* stream, const char** launched);
+int launch_axis_rope(const AxisRopeArgs& a, void* stream, const char** launched);
 int launch_kv_read(const KvReadArgs& a, void* stream, const char** launched);
 int launch_kv_expand(const KvReadArgs& a, void* stream, const char** launched);
 int launch_cached_attn(const CachedAttnArgs& a, void* stream, const char** launched);
+int launch_masked_attn(const MaskedAttnArgs& a, void* stream, const char** launched);
 
 // Measurement only: n_groups one-wave workgroups each store (XCD id, HW_ID,
 // shader clock counter, real-time counter) as four uint64 at out + 4 * group;

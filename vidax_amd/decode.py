@@ -1,0 +1,261 @@
+"""The steps of a rollout or a decoding loop over the 8-bit key/value cache.
+
+A rollout that makes a video block by block, or a text pathway that makes it token
+by token, turns its new queries and keys by their positions, writes the keys and
+values to the cache, and attends over what the cache holds. (The reference's rotary
+tables cover a whole grid from position 0, `src/vidax/core/rope3d.py:45-111`, and
+its causal text pathway recomputes all tokens, `src/vidax/models/cosmos3/
+dit_layers.py:114-135`.)
+
+`apply_axis_rope` turns rows by integer positions per token and axis (time, height,
+width), `kv_cache_write_rope` does so to keys on their way into the cache,
+`windowed_attention` attends over a sliding window behind a few first tokens, and
+`tree_attention` lets drafted tokens see their ancestors only. As in the cache's
+other calls, each launches HIP kernels on torch's current stream and never waits for
+the GPU; positions, lengths, parents and slots are device tensors, so a captured
+graph may be replayed while they change.
+"""
+from __future__ import annotations
+
+import functools
+import math
+from typing import NamedTuple, Optional, Sequence
+
+import torch
+
+from . import _lib
+from .kv_cache import KVCache, _check_cache, _check_rows, _ints, _out_for, _rows
+
+__all__ = ["AxisRope", "create_axis_rope", "apply_axis_rope", "kv_cache_write_rope", "windowed_attention",
+           "tree_attention"]
+
+
+class AxisRope(NamedTuple):
+    """How the pairs of a head's channels turn. turns (head_dim / 2,) int64: turns
+    per position in units of 2^-64 turns, modulo 2^64 (the tensor's values as
+    unsigned ones; 0: the pair stays as it is). axis (head_dim / 2,) int32: the axis
+    whose position turns the pair. axes: their number, 1 to 4. halves: pair j is
+    channels (j, j + head_dim / 2) rather than (2 j, 2 j + 1)."""
+    turns: torch.Tensor
+    axis: torch.Tensor
+    axes: int
+    halves: bool
+
+
+def create_axis_rope(head_dim: int, split: Sequence[int], base: float = 10000.0, *, shared: bool = False,
+                     halves: bool = False, axis_scale: Optional[Sequence[float]] = None, device=None) -> AxisRope:
+    """The turns of a head whose channels are split over axes: split[a] channels
+    (an even number) to axis a, in order; channels past their sum do not turn.
+
+    Pair i of an axis's own ones turns by position * base^(-2 i / split[a]) radians
+    (the ladder of create_rope3d_freqs and create_abs_rope3d_freqs); shared: pair j
+    of the head by position * base^(-2 j / head_dim). axis_scale: a factor of each
+    axis's positions (frames per second, a coarser grid). halves as in AxisRope
+    (default: adjacent channels, as in apply_rope3d).
+    """
+    if head_dim not in (64, 128):
+        raise NotImplementedError(f"head_dim {head_dim} is not supported (64 and 128 are)")
+    split = [int(d) for d in split]
+    if not 1 <= len(split) <= 4:
+        raise NotImplementedError(f"{len(split)} axes are not supported (1 to 4 are)")
+    if any(d < 0 or d % 2 for d in split) or sum(split) > head_dim:
+        raise ValueError(f"split {split} must be even numbers of at most head_dim {head_dim} together")
+    scales = [1.0] * len(split) if axis_scale is None else [float(x) for x in axis_scale]
+    if len(scales) != len(split) or not all(math.isfinite(x) for x in scales):
+        raise ValueError(f"axis_scale must hold {len(split)} finite numbers")
+    base = float(base)
+    if not (base > 0 and math.isfinite(base)):
+        raise ValueError(f"base must be positive and finite; got {base}")
+    turns, axis = [], []
+    for a, (channels, scale) in enumerate(zip(split, scales)):
+        for i in range(channels // 2):
+            exponent = 2 * len(turns) / head_dim if shared else 2 * i / channels
+            turns.append(round(scale * base ** -exponent / (2 * math.pi) * 2.0 ** 64) % 2 ** 64)
+            axis.append(a)
+    still = head_dim // 2 - len(turns)
+    turns = [t - 2 ** 64 if t >= 2 ** 63 else t for t in turns] + [0] * still
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+    return AxisRope(torch.tensor(turns, dtype=torch.int64, device=device),
+                    torch.tensor(axis + [0] * still, dtype=torch.int32, device=device), len(split), bool(halves))
+
+
+def _check_rope(rope: AxisRope, head_dim: int, index: int):
+    """(turns' address, axis's address, number of axes, halves) of a rope that goes
+    with rows of this head dim on this device."""
+    if not isinstance(rope, AxisRope):
+        raise TypeError("rope must be an AxisRope")
+    turns, axis, axes, halves = rope
+    for name, t, dtype in (("turns", turns, torch.int64), ("axis", axis, torch.int32)):
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+            raise TypeError(f"rope.{name} must be a tensor of {dtype}")
+        if t.shape != (head_dim // 2,):
+            raise ValueError(f"rope.{name} has shape {tuple(t.shape)}, a head of {head_dim} channels has "
+                             f"{head_dim // 2} pairs")
+        if t.get_device() != index or not t.is_contiguous():
+            raise ValueError(f"rope.{name} must be contiguous and on the rows' device")
+    return turns.data_ptr(), axis.data_ptr(), int(axes), int(bool(halves))
+
+
+def _positions(positions, batch: int, seq: int, axes: int, index: int):
+    """(positions as the kernels read them, their address, their strides)."""
+    shape = positions.shape if isinstance(positions, torch.Tensor) else None
+    if not (shape == (batch, seq, axes) and positions.dtype is torch.int32 and positions.get_device() == index and
+            min(positions.stride(), default=0) >= 0):
+        if not isinstance(positions, torch.Tensor):
+            positions = torch.as_tensor(positions)
+            shape = positions.shape
+        if shape not in ((batch, seq, axes), (seq, axes)):
+            raise ValueError(f"positions must be ({batch}, {seq}, {axes}) or ({seq}, {axes}); got {tuple(shape)}")
+        if not (positions.dtype is torch.int32 and positions.get_device() == index):
+            positions = _ints(positions, positions.numel(), index, "positions")[0].reshape(shape)
+        positions = positions.expand(batch, seq, axes)
+    return positions, positions.data_ptr(), _lib.strides3(positions.stride())
+
+
+def apply_axis_rope(x: torch.Tensor, positions, rope: AxisRope, *, inverse: bool = False) -> torch.Tensor:
+    """Turns every head's pairs of x (B, S, H, D) bf16 by their tokens' positions
+    (B, S, axes) int32 (or (S, axes), shared by the batch; any strides): pair j,
+    (u, w), becomes (u cos a - w sin a, u sin a + w cos a) with a the pair's turns
+    times position[axis[j]]. Returns a new contiguous tensor, turned in fp32 and
+    rounded once. D is 64 or 128.
+
+    inverse: by as much the other way. That undoes a turn (cached keys that move to
+    other positions), and is its gradient: of x, from that of the output.
+    Angles are formed modulo a turn in integers, so far positions turn as exactly as
+    near ones; positions past 32 bits are held at its ends.
+    """
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a torch.Tensor")
+    if not x.is_cuda:
+        raise ValueError("x must be a GPU tensor")
+    index = x.get_device()
+    B, S, H, D = shape = _check_rows(x, "x", index, x.shape[-1] if x.dim() else 0)
+    if D not in (64, 128):
+        raise NotImplementedError(f"head_dim {D} is not supported (64 and 128 are)")
+    turns_at, axis_at, axes, halves = _check_rope(rope, D, index)
+    positions, positions_at, strides = _positions(positions, B, S, axes, index)
+    out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    if B == 0 or S == 0 or H == 0:
+        return out
+    x, x_at, x_strides = _rows(x)
+    _lib.launch(out.device, _lib.lib().vx_axis_rope_fwd, x_at, out.data_ptr(), x_strides, positions_at, strides, axes,
+                turns_at, axis_at, halves, int(bool(inverse)), B, S, H, D)
+    return out
+
+
+def kv_cache_write_rope(cache: KVCache, k: torch.Tensor, v: torch.Tensor, positions, rope: AxisRope, start=None, *,
+                        num=None, slots=None) -> None:
+    """kv_cache_write of keys turned as by apply_axis_rope (one pass; turned in fp32
+    and rounded once, to the cache's 8 bits) and of values as they are. positions
+    (B, S, axes) or (S, axes) are those of the tokens of k, wherever in the cache
+    they go; the other arguments as in kv_cache_write."""
+    n_slots, Hk, cap, D, index = _check_cache(cache, "cache")
+    shape = _check_rows(k, "k", index, D)
+    vshape = _check_rows(v, "v", index, D)
+    B, S, heads, _ = shape
+    if heads != Hk or vshape[2] != Hk:
+        raise ValueError(f"k and v have {heads} and {vshape[2]} heads, the cache {Hk}")
+    if shape != vshape:
+        raise ValueError(f"k and v shapes differ: {tuple(shape)} vs {tuple(vshape)}")
+    turns_at, axis_at, axes, halves = _check_rope(rope, D, index)
+    positions, positions_at, strides = _positions(positions, B, S, axes, index)
+    start, start_at = _ints(start, B, index, "start")
+    num, num_at = _ints(num, B, index, "num")
+    slots, slots_at = _ints(slots, B, index, "slots")
+    if B == 0 or S == 0:
+        return
+    k, k_at, k_strides = _rows(k)
+    v, v_at, v_strides = _rows(v)
+    _lib.launch(cache.k.device, _lib.lib().vx_kv_write_rope_fwd, k_at, v_at, k_strides, v_strides,
+                cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n_slots,
+                cap, start_at, num_at, slots_at, positions_at, strides, axes, turns_at, axis_at, halves, B, S, Hk, D)
+
+
+@functools.lru_cache(maxsize=1024)
+def _window_bytes(device_index: int, *sizes: int) -> int:
+    with torch.cuda.device(device_index):
+        return max(int(_lib.lib().vx_window_attn_workspace_size(*sizes)), 0)  # (what it refuses: the launch says why)
+
+
+@functools.lru_cache(maxsize=1024)
+def _tree_bytes(device_index: int, *sizes: int) -> int:
+    with torch.cuda.device(device_index):
+        return max(int(_lib.lib().vx_tree_attn_workspace_size(*sizes)), 0)
+
+
+def _masked(entry, workspace_bytes, q, cache, kv_len, q_len, slots, scale, out, before, after):
+    """The part that windowed_attention and tree_attention share: the entry's
+    arguments around the sizes are before(...) and after."""
+    n_slots, Hk, cap, D, index = _check_cache(cache, "cache")
+    B, Sq, H, _ = shape = _check_rows(q, "q", index, D)
+    kv_len, kv_len_at = _ints(kv_len, B, index, "kv_len")
+    q_len, q_len_at = _ints(q_len, B, index, "q_len")
+    slots, slots_at = _ints(slots, B, index, "slots")
+    held, before = before(B, Sq, index)
+    dev = q.device
+    empty = B == 0 or Sq == 0 or H == 0
+    if not empty:
+        q, q_at, q_strides = _rows(q)
+    out, out_strides = _out_for(out, shape, dev, q if not empty and q_strides is None else None)
+    if empty:
+        return out
+    ws_bytes = workspace_bytes(index, cap, B, Sq, H, Hk, D, *after)
+    ws = ws_at = None
+    if ws_bytes > 0:
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        ws_at = ws.data_ptr()
+    _lib.launch(dev, entry, q_at, out.data_ptr(), q_strides, out_strides, cache.k.data_ptr(), cache.v.data_ptr(),
+                cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n_slots, cap, kv_len_at, q_len_at, slots_at,
+                *before, B, Sq, H, Hk, D, *after, D ** -0.5 if scale is None else float(scale), ws_at, ws_bytes)
+    return out
+
+
+def _none(B: int, Sq: int, index: int):
+    return None, ()
+
+
+def windowed_attention(q: torch.Tensor, cache: KVCache, kv_len=None, *, window: int, sinks: int = 0, q_len=None,
+                       slots=None, causal: bool = True, scale: Optional[float] = None,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """cached_attention whose queries see the last `window` tokens up to theirs and
+    the first `sinks` ones; returns (B, Sq, H, D) bf16.
+
+    causal: query i of q_len sits at position p = kv_len - q_len + i and sees
+    positions p - window + 1 .. p and, of 0 .. sinks - 1, those up to p (single
+    tokens, prompts in chunks). False: the queries are one block whose tokens see
+    each other: all of them see the last `window` of the kv_len tokens, their own
+    among them, and the first `sinks` (a block of a rollout over the frames before
+    it). Positions that no query sees are not read. The other arguments, lengths
+    outside their range, queries without a visible key and rows of scale NaN are as
+    in cached_attention.
+    """
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window ({window}) must be >= 1 and sinks ({sinks}) >= 0")
+    most = (1 << 31) - 1  # (more than any cache holds)
+    return _masked(_lib.lib().vx_window_attn_fwd, _window_bytes, q, cache, kv_len, q_len, slots, scale, out, _none,
+                   (min(window, most), min(sinks, most), 1 if causal else 0))
+
+
+def tree_attention(q: torch.Tensor, cache: KVCache, parents, kv_len=None, *, q_len=None, slots=None,
+                   scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """cached_attention of drafted tokens that form a tree; returns (B, Sq, H, D) bf16.
+
+    The last q_len of an item's kv_len cached tokens are drafted (write them first),
+    and the queries are theirs, in the same order. parents (B, Sq) int32 (or (Sq,),
+    one tree for all items): the drafted token that a drafted token follows, an
+    earlier one; any value that is not 0 .. i - 1 stands for none: such a token
+    follows the last one in front of the drafted ones. Query i sees all tokens in
+    front of the drafted ones, its ancestors and itself. Sq is at most 512; with
+    parents i - 1 this is cached_attention. The other arguments, lengths outside
+    their range, queries without a visible key and rows of scale NaN are as there.
+    """
+    def arguments(B: int, Sq: int, index: int):
+        shape = parents.shape if isinstance(parents, torch.Tensor) else torch.as_tensor(parents).shape
+        if shape != (B, Sq) and shape != (Sq,):
+            raise ValueError(f"parents must be ({B}, {Sq}) or ({Sq},); got {tuple(shape)}")
+        held, at = _ints(parents, Sq if len(shape) == 1 else B * Sq, index, "parents")
+        return held, (at, 0 if len(shape) == 1 else Sq)
+    if parents is None:
+        raise TypeError("parents must hold integers")
+    return _masked(_lib.lib().vx_tree_attn_fwd, _tree_bytes, q, cache, kv_len, q_len, slots, scale, out, arguments, ())

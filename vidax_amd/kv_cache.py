@@ -238,6 +238,18 @@ def _workspace_bytes(device_index: int, *sizes: int) -> int:
         return max(int(_lib.lib().vx_cached_attn_workspace_size(*sizes)), 0)  # (sizes it refuses: the launch says why)
 
 
+def _out_for(out: Optional[torch.Tensor], shape, dev: torch.device, like: Optional[torch.Tensor]):
+    """(output tensor, its C ABI strides): the caller's, checked, or a new one (as
+    `like`, contiguous queries, which is quicker)."""
+    if out is None:
+        return torch.empty(shape, dtype=torch.bfloat16, device=dev) if like is None else torch.empty_like(like), None
+    if out.shape != shape or out.dtype != torch.bfloat16 or out.stride(-1) != 1 or out.device != dev:
+        raise ValueError("out must be a (B, Sq, H, D) bf16 tensor with a contiguous head dim, on q's device")
+    if out.is_neg() or any(st == 0 and n > 1 for st, n in zip(out.stride(), shape)):
+        raise ValueError("out must be a tensor that holds its values as they are, each in memory of its own")
+    return out, _strides3(out)
+
+
 def _attend(q: torch.Tensor, cache: KVCache, prefix: Optional[KVCache], kv_len, prefix_len, q_len, slots,
             causal: bool, scale: Optional[float], out: Optional[torch.Tensor]) -> torch.Tensor:
     n_slots, Hk, cap, D, index = _check_cache(cache, "cache")
@@ -258,15 +270,7 @@ def _attend(q: torch.Tensor, cache: KVCache, prefix: Optional[KVCache], kv_len, 
     empty = B == 0 or Sq == 0 or H == 0
     if not empty:
         q, q_at, q_strides = _rows(q)
-    out_strides = None
-    if out is None:
-        out = torch.empty_like(q) if not empty and q_strides is None else torch.empty(shape, dtype=q.dtype, device=dev)
-    elif out.shape != shape or out.dtype != q.dtype or out.stride(-1) != 1 or out.device != dev:
-        raise ValueError("out must be a (B, Sq, H, D) bf16 tensor with a contiguous head dim, on q's device")
-    elif out.is_neg() or any(st == 0 and n > 1 for st, n in zip(out.stride(), shape)):
-        raise ValueError("out must be a tensor that holds its values as they are, each in memory of its own")
-    else:
-        out_strides = _strides3(out)
+    out, out_strides = _out_for(out, shape, dev, q if not empty and q_strides is None else None)
     if empty:
         return out
     ws_bytes = _workspace_bytes(index, cap, n_prefix, p_cap, B, Sq, H, Hk, D,
