@@ -26,10 +26,40 @@ int seen_most(int cap, int Sq, int G, int window, int sinks, bool causal) {
   return (int)std::min<int64_t>(cap, most);
 }
 
+// Ranges of few rows go over streams, with a launch that merges; a window makes the
+// streams' lengths alike, so often each is one workgroup's (us a call; 32 heads on 8,
+// lengths 150 to 8192, streams whole / in ranges):
+//   window       1100         2048         4096         8192
+//   8 items      16 / 22      20 / 25      31 / 28      53 / 30
+//   32           21 / 30      28 / 37      52 / 64      75 / 77
+//   64           32 / 43      55 / 66      91 / 97      118 / 119
+//   100          56 / 62      82 / 92      139 / 138    201 / 180
+// A 32-key tile takes a wave 1.65 us, and ranges cost 11 more.
+bool whole_streams(int64_t groups, int64_t tiles, int D, int64_t cus) {
+  const int64_t slots = 2 * cus, rounds = (groups + slots - 1) / slots, waves = groups <= cus ? 8 : 4;
+  const double t = 1.65 * (double)tiles * D / 128;
+  return t * (double)rounds / (double)waves <= t * (double)groups / (double)(slots * kWaves) + 11;
+}
+
+Plan masked_plan(int cap, int B, int Sq, int H, int Hk, int D, int window, int sinks, bool causal) {
+  const int seen = seen_most(cap, Sq, H / Hk, window, sinks, causal);
+  Plan p = plan_of(seen, 0, 0, B, Sq, H, Hk, D);
+  Part& own = p.own.p;
+  const int64_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
+  if (window > 0 && own.few && own.rows <= 32 && own.budget > 0 &&
+      whole_streams((int64_t)B * Hk, (seen + kFewTile - 1) / kFewTile, D, cus)) {
+    own.budget = 0;
+    own.items = B;
+    p.own.blocks = (int64_t)B * Hk;
+    p.own.floats = 0;
+    p.wide = p.own.blocks <= cus;
+  }
+  return p;
+}
+
 template <int D, int MASK>
 int launch(const MaskedAttnArgs& a, hipStream_t st, const char** launched) {
-  const int seen = seen_most(a.c.cap, a.Sq, a.H / a.c.Hk, a.window, a.sinks, a.causal != 0);
-  Plan pl = plan_of(seen, 0, 0, a.B, a.Sq, a.H, a.c.Hk, D);
+  Plan pl = masked_plan(a.c.cap, a.B, a.Sq, a.H, a.c.Hk, D, a.window, a.sinks, a.causal != 0);
   Part& own = pl.own.p;
   own.s = Streams{a.c, a.kv_len, a.slots, a.B};
   own.ws = a.ws;
@@ -65,7 +95,7 @@ int launch(const MaskedAttnArgs& a, hipStream_t st, const char** launched) {
 
 int64_t masked_attn_workspace(int32_t cap, int32_t B, int32_t Sq, int32_t H, int32_t Hk, int32_t D, int32_t window,
                               int32_t sinks, bool causal) {
-  const Plan p = plan_of(seen_most(cap, Sq, H / Hk, window, sinks, causal), 0, 0, B, Sq, H, Hk, D);
+  const Plan p = masked_plan(cap, B, Sq, H, Hk, D, window, sinks, causal);
   return p.own.floats * (int64_t)sizeof(float);
 }
 
