@@ -29,7 +29,8 @@ int32_t vx_decode_abi_version(void);
  *              {batch, seq, head} in elements, multiples of 8 (NULL: contiguous)
  *   out        bf16, the same shape, contiguous, 16-byte aligned; x itself or no
  *              part of it
- *   positions  int32 at strides {batch, token, axis} in elements (>= 0; 0: shared)
+ *   positions  int32 at strides {batch, token, axis} in elements (>= 0; 0: shared;
+ *              NULL: contiguous (batch, seq, num_axes))
  *   num_axes   1 to 4
  *   turns      uint64[head_dim / 2], turns per position in units of 2^-64 turns
  *              (whole turns left out); 0: the pair stays as it is

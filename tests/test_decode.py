@@ -82,7 +82,8 @@ def _tree_check(**kw):
 
 
 def test_checks_accept_valid_arguments():
-    assert _rope_check() == _rope_check(pst=(0, 1, 0), axes=4, D=64, xst=(8, 8, 8), halves=1, inverse=1) == _lib.VX_OK
+    assert _rope_check() == _rope_check(pst=None) == _lib.VX_OK
+    assert _rope_check(pst=(0, 1, 0), axes=4, D=64, xst=(8, 8, 8), halves=1, inverse=1) == _lib.VX_OK
     assert _write_check() == _write_check(slots=A, B=9, pst=(0, 0, 0), halves=1) == _lib.VX_OK
     assert _window_check() == _window_check(window=2 ** 31 - 1, sinks=2 ** 31 - 1, causal=0) == _lib.VX_OK
     assert _tree_check() == _tree_check(S=512, pstride=0) == _lib.VX_OK
@@ -91,7 +92,6 @@ def test_checks_accept_valid_arguments():
 
 ROPE = [
     (dict(pos=None), INVALID, "non-NULL"),
-    (dict(pst=None), INVALID, "non-NULL"),
     (dict(turns=None), INVALID, "non-NULL"),
     (dict(axis=None), INVALID, "non-NULL"),
     (dict(pos=A + 2), INVALID, "aligned"),

@@ -296,40 +296,39 @@ struct Part {
 };
 
 // ---- trees: of the last q_len keys of an item, its drafted tokens, a row sees its
-// ancestors and itself. Per row one bit for each of them in LDS, between a word of
+// ancestors and itself: per row one bit for each of them in LDS, between a word of
 // ones (the keys in front, which all see) and words of zeros, so that the 32 bits
 // from any drafted token on, or up to 32 before the first, are two words shifted.
 constexpr int kTreeWords = kTreeMost / 32 + 3;  // (odd: rows lie in different banks)
 constexpr int tree_bytes(int rows) { return rows * kTreeWords * 4 + kTreeMost * 4; }
 
-// Fills the words of rows 0 .. n - 1, row r the query of map.place(row0 + r). A
-// parent that is not below its child counts as none, so every walk ends.
-template <int THREADS>
-__device__ __forceinline__ void fill_tree(const MaskedAttnArgs& a, const RowMap& map, int row0, int n, lds_u8* at) {
+// A wave fills the words of up to 32 rows for itself, row r the query of map.place(row0
+// + r), and needs no barrier: waves that fill the same rows write the same. A parent
+// that is not below its child counts as none, so every walk ends.
+__device__ __forceinline__ void fill_tree(const MaskedAttnArgs& a, const RowMap& map, int row0, int n, lds_u8* at,
+                                          int lds_row0) {
+  const int lane = threadIdx.x & 63, m = clamp_len(a.q_len, map.stream, a.Sq);
   VX_LDS int* const parents = (VX_LDS int*)at;
-  VX_LDS uint32_t* const words = (VX_LDS uint32_t*)(at + kTreeMost * 4);
-  const int m = clamp_len(a.q_len, map.stream, a.Sq);
-  for (int i = threadIdx.x; i < m; i += THREADS) parents[i] = a.parents[map.stream * a.parents_stride + i];
-  __syncthreads();
-  for (int r = threadIdx.x; r < n; r += THREADS) {
+  for (int i = lane; i < m; i += 64) parents[i] = a.parents[map.stream * a.parents_stride + i];
+  if (lane < n) {
     int b, i, h;
-    map.place(row0 + r, b, i, h);
-    VX_LDS uint32_t* const w = words + r * kTreeWords;
-    w[0] = ~0u;
-#pragma unroll
-    for (int x = 1; x < kTreeWords; ++x) w[x] = 0u;
-    uint32_t bits = 0;
+    map.place(row0 + lane, b, i, h);
+    VX_LDS uint32_t* const w = (VX_LDS uint32_t*)(at + kTreeMost * 4) + (lds_row0 + lane) * kTreeWords;
+    int x = kTreeWords - 1;  // the words from the last to the first, each written once
     for (int j = min(i, m - 1); j >= 0;) {
-      bits |= 1u << (j & 31);
-      const int p = parents[j], next = p < j ? max(p, -1) : -1;
-      if ((next >> 5) != (j >> 5)) {
-        w[1 + (j >> 5)] = bits;
-        bits = 0;
-      }
-      j = next;
+      const int word = 1 + (j >> 5);
+      for (; x > word; --x) w[x] = 0u;
+      uint32_t bits = 0;
+      do {
+        bits |= 1u << (j & 31);
+        const int p = parents[j];
+        j = p < j ? max(p, -1) : -1;
+      } while (1 + (j >> 5) == word);
+      w[x--] = bits;
     }
+    for (; x > 0; --x) w[x] = 0u;
+    w[0] = ~0u;
   }
-  __syncthreads();
 }
 
 // Bits of 32 keys of row r, the first of them `from` keys behind the first drafted one.
@@ -482,8 +481,6 @@ __device__ __forceinline__ void few_part(const Args<MASK>& a, const Part& pt, co
     if constexpr (MASK == kTree) {
       base = len - __builtin_amdgcn_readfirstlane(clamp_len(a.q_len, stream, a.Sq));
       own.all = min(own.all, base);
-      if (rounded || min(first + take, tiles_in<kFewTile>(any)) * kFewTile > own.all)
-        fill_tree<W * 64>(a, map, row0, rows, (lds_u8*)smem + C::kSmem);
     }
     if (rounded) own.all = shared.all = 0;
 
@@ -585,6 +582,10 @@ __device__ __forceinline__ void few_part(const Args<MASK>& a, const Part& pt, co
     const int n = here > wave ? (here - wave + W - 1) / W : 0;  // this wave's tiles
     if (n > 0) stage_at(wave, 0);
     if (n > 1) stage_at(wave + W, 1);
+    if constexpr (MASK == kTree) {  // (the wave's last tile is masked by its bits)
+      if (n > 0 && (first + wave + (n - 1) * W + 1) * kFewTile > own.all)
+        fill_tree(a, map, row0, rows, (lds_u8*)smem + C::kSmem, 0);
+    }
     for (int it = 0; it < n; ++it) {
       if (it + 1 < n)
         wait_copies<C::kPerTile>();
@@ -753,7 +754,8 @@ __device__ __forceinline__ bool many_one(const Args<MASK>& a, const Part& pt, co
   if constexpr (MASK == kTree) {
     all = min(all, base);
     if (rounded || (t0 + n) * kManyTile > base)  // (some tile is masked by its bits)
-      fill_tree<kThreads>(a, map, rt * C::kRows, min(rows - rt * C::kRows, C::kRows), (lds_u8*)smem + C::kSmem);
+      fill_tree(a, map, rt * C::kRows + wave * 32, min(rows - rt * C::kRows - wave * 32, 32),
+                (lds_u8*)smem + C::kSmem, wave * 32);
   }
   f32x16 O[kDB];
 #pragma unroll

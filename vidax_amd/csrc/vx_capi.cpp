@@ -801,18 +801,19 @@ int32_t cached_attn_check(const void* q, const void* out, const int64_t* qs, con
 }
 
 // ---- rotary positions, and attention of less than all keys
-int32_t axis_rope_check(const int32_t* positions, const int64_t* strides, int32_t axes, const uint64_t* turns,
-                        const int32_t* axis, int32_t halves, vx::AxisRope* r) {
-  if (positions == nullptr || strides == nullptr || turns == nullptr || axis == nullptr)
-    return fail(VX_ERR_INVALID_ARGUMENT, "positions, position_strides, turns and axis must be non-NULL");
+int32_t axis_rope_check(const int32_t* positions, const int64_t* strides, int32_t S, int32_t axes,
+                        const uint64_t* turns, const int32_t* axis, int32_t halves, vx::AxisRope* r) {
+  if (positions == nullptr || turns == nullptr || axis == nullptr)
+    return fail(VX_ERR_INVALID_ARGUMENT, "positions, turns and axis must be non-NULL");
   if (!aligned4(positions) || !aligned4(axis) || (reinterpret_cast<uintptr_t>(turns) & 7u) != 0)
     return fail(VX_ERR_INVALID_ARGUMENT, "positions and axis must be 4-byte, turns 8-byte aligned");
   if (axes < 1 || axes > vx::kRopeAxes)
     return fail(VX_ERR_UNSUPPORTED, "num_axes (%d) must be in 1..%d", axes, vx::kRopeAxes);
   if (halves != 0 && halves != 1) return fail(VX_ERR_INVALID_ARGUMENT, "halves must be 0 or 1");
   for (int i = 0; i < 3; ++i) {
-    if (strides[i] < 0) return fail(VX_ERR_INVALID_ARGUMENT, "position_strides must be >= 0");
-    r->ps[i] = strides[i];
+    if (strides != nullptr && strides[i] < 0)
+      return fail(VX_ERR_INVALID_ARGUMENT, "position_strides must be >= 0");
+    r->ps[i] = strides != nullptr ? strides[i] : i == 0 ? (int64_t)S * axes : i == 1 ? axes : 1;
   }
   r->positions = positions;
   r->axes = axes;
@@ -834,7 +835,7 @@ int32_t axis_rope_args(const void* x, const void* out, const int64_t* xs, const 
     return fail(VX_ERR_UNSUPPORTED, "head_dim %d is not supported (this build handles 64 and 128)", D);
   if (inverse != 0 && inverse != 1) return fail(VX_ERR_INVALID_ARGUMENT, "inverse must be 0 or 1");
   int32_t rc;
-  if ((rc = axis_rope_check(positions, ps, axes, turns, axis, halves, &a->rope)) != VX_OK) return rc;
+  if ((rc = axis_rope_check(positions, ps, S, axes, turns, axis, halves, &a->rope)) != VX_OK) return rc;
   strides_or_default(xs, S, H, D, a->xs);
   if ((rc = check_strides("x", a->xs, S)) != VX_OK) return rc;
   // (a grid's threads, 64 for 32 heads of a token at most, are counted in 32 bits)
@@ -1524,7 +1525,7 @@ int32_t vx_kv_write_rope_check(const void* k, const void* v, const int64_t* k_st
   vx::KvWriteArgs a;
   vx::AxisRope r;
   int32_t rc;
-  if ((rc = axis_rope_check(positions, position_strides, num_axes, turns, axis, halves, &r)) != VX_OK) return rc;
+  if ((rc = axis_rope_check(positions, position_strides, seq, num_axes, turns, axis, halves, &r)) != VX_OK) return rc;
   return kv_write_check(k, v, k_strides, v_strides, cache_k, cache_v, k_scale, v_scale, num_slots, capacity, start,
                         num, slots, batch, seq, num_kv_heads, head_dim, &a);
 }
@@ -1538,7 +1539,7 @@ int32_t vx_kv_write_rope_fwd(const void* k, const void* v, const int64_t* k_stri
   vx::KvWriteArgs a;
   vx::AxisRope r;
   int32_t rc;
-  if ((rc = axis_rope_check(positions, position_strides, num_axes, turns, axis, halves, &r)) != VX_OK ||
+  if ((rc = axis_rope_check(positions, position_strides, seq, num_axes, turns, axis, halves, &r)) != VX_OK ||
       (rc = kv_write_check(k, v, k_strides, v_strides, cache_k, cache_v, k_scale, v_scale, num_slots, capacity, start,
                            num, slots, batch, seq, num_kv_heads, head_dim, &a)) != VX_OK)
     return rc;

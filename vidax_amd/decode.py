@@ -24,7 +24,7 @@ from typing import NamedTuple, Optional, Sequence
 import torch
 
 from . import _lib
-from .kv_cache import KVCache, _check_cache, _check_rows, _ints, _out_for, _rows
+from .kv_cache import _MOST, KVCache, _check_cache, _check_rows, _ints, _out_for, _rows
 
 __all__ = ["AxisRope", "create_axis_rope", "apply_axis_rope", "kv_cache_write_rope", "windowed_attention",
            "tree_attention"]
@@ -85,6 +85,14 @@ def _check_rope(rope: AxisRope, head_dim: int, index: int):
     if not isinstance(rope, AxisRope):
         raise TypeError("rope must be an AxisRope")
     turns, axis, axes, halves = rope
+    try:
+        if (turns.dtype is torch.int64 and axis.dtype is torch.int32 and
+                turns.shape == axis.shape == (head_dim // 2,) and turns.get_device() == index and
+                axis.get_device() == index and turns.is_contiguous() and axis.is_contiguous()):
+            return turns.data_ptr(), axis.data_ptr(), int(axes), int(bool(halves))
+    except AttributeError:
+        pass
+    # what is wrong
     for name, t, dtype in (("turns", turns, torch.int64), ("axis", axis, torch.int32)):
         if not isinstance(t, torch.Tensor) or t.dtype != dtype:
             raise TypeError(f"rope.{name} must be a tensor of {dtype}")
@@ -93,17 +101,19 @@ def _check_rope(rope: AxisRope, head_dim: int, index: int):
                              f"{head_dim // 2} pairs")
         if t.get_device() != index or not t.is_contiguous():
             raise ValueError(f"rope.{name} must be contiguous and on the rows' device")
-    return turns.data_ptr(), axis.data_ptr(), int(axes), int(bool(halves))
+    raise ValueError("rope is not an AxisRope that the kernels take")
 
 
 def _positions(positions, batch: int, seq: int, axes: int, index: int):
-    """(positions as the kernels read them, their address, their strides)."""
-    shape = positions.shape if isinstance(positions, torch.Tensor) else None
-    if not (shape == (batch, seq, axes) and positions.dtype is torch.int32 and positions.get_device() == index and
-            min(positions.stride(), default=0) >= 0):
+    """(positions as the kernels read them, their address, their C ABI strides)."""
+    if (isinstance(positions, torch.Tensor) and positions.shape == (batch, seq, axes) and
+            positions.dtype is torch.int32 and positions.get_device() == index):
+        if positions.is_contiguous():
+            return positions, positions.data_ptr(), None
+    else:
         if not isinstance(positions, torch.Tensor):
             positions = torch.as_tensor(positions)
-            shape = positions.shape
+        shape = positions.shape
         if shape not in ((batch, seq, axes), (seq, axes)):
             raise ValueError(f"positions must be ({batch}, {seq}, {axes}) or ({seq}, {axes}); got {tuple(shape)}")
         if not (positions.dtype is torch.int32 and positions.get_device() == index):
@@ -134,10 +144,10 @@ def apply_axis_rope(x: torch.Tensor, positions, rope: AxisRope, *, inverse: bool
         raise NotImplementedError(f"head_dim {D} is not supported (64 and 128 are)")
     turns_at, axis_at, axes, halves = _check_rope(rope, D, index)
     positions, positions_at, strides = _positions(positions, B, S, axes, index)
-    out = torch.empty(shape, dtype=x.dtype, device=x.device)
     if B == 0 or S == 0 or H == 0:
-        return out
+        return torch.empty(shape, dtype=x.dtype, device=x.device)
     x, x_at, x_strides = _rows(x)
+    out = torch.empty_like(x) if x_strides is None else torch.empty(shape, dtype=x.dtype, device=x.device)
     _lib.launch(out.device, _lib.lib().vx_axis_rope_fwd, x_at, out.data_ptr(), x_strides, positions_at, strides, axes,
                 turns_at, axis_at, halves, int(bool(inverse)), B, S, H, D)
     return out
@@ -183,35 +193,33 @@ def _tree_bytes(device_index: int, *sizes: int) -> int:
         return max(int(_lib.lib().vx_tree_attn_workspace_size(*sizes)), 0)
 
 
-def _masked(entry, workspace_bytes, q, cache, kv_len, q_len, slots, scale, out, before, after):
-    """The part that windowed_attention and tree_attention share: the entry's
-    arguments around the sizes are before(...) and after."""
+def _attend_args(q: torch.Tensor, cache: KVCache, kv_len, q_len, slots, out: Optional[torch.Tensor]):
+    """What windowed_attention and tree_attention have alike: (sizes, tensors that
+    the call reads, output, the C ABI's arguments up to slots). Where there is
+    nothing to compute, the arguments are None."""
     n_slots, Hk, cap, D, index = _check_cache(cache, "cache")
     B, Sq, H, _ = shape = _check_rows(q, "q", index, D)
     kv_len, kv_len_at = _ints(kv_len, B, index, "kv_len")
     q_len, q_len_at = _ints(q_len, B, index, "q_len")
     slots, slots_at = _ints(slots, B, index, "slots")
-    held, before = before(B, Sq, index)
     dev = q.device
-    empty = B == 0 or Sq == 0 or H == 0
-    if not empty:
-        q, q_at, q_strides = _rows(q)
-    out, out_strides = _out_for(out, shape, dev, q if not empty and q_strides is None else None)
-    if empty:
-        return out
-    ws_bytes = workspace_bytes(index, cap, B, Sq, H, Hk, D, *after)
-    ws = ws_at = None
-    if ws_bytes > 0:
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        ws_at = ws.data_ptr()
-    _lib.launch(dev, entry, q_at, out.data_ptr(), q_strides, out_strides, cache.k.data_ptr(), cache.v.data_ptr(),
-                cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n_slots, cap, kv_len_at, q_len_at, slots_at,
-                *before, B, Sq, H, Hk, D, *after, D ** -0.5 if scale is None else float(scale), ws_at, ws_bytes)
-    return out
+    sizes = (index, cap, B, Sq, H, Hk, D)
+    if B == 0 or Sq == 0 or H == 0:
+        return sizes, None, _out_for(out, shape, dev, None)[0], None
+    q, q_at, q_strides = _rows(q)
+    out, out_strides = _out_for(out, shape, dev, q if q_strides is None else None)
+    k, v, ks, vs = cache
+    return sizes, (q, kv_len, q_len, slots), out, (q_at, out.data_ptr(), q_strides, out_strides, k.data_ptr(),
+                                                   v.data_ptr(), ks.data_ptr(), vs.data_ptr(), n_slots, cap,
+                                                   kv_len_at, q_len_at, slots_at)
 
 
-def _none(B: int, Sq: int, index: int):
-    return None, ()
+def _workspace(nbytes: int, dev: torch.device):
+    """(a workspace, its address), or (None, None)."""
+    if nbytes == 0:
+        return None, None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return ws, ws.data_ptr()
 
 
 def windowed_attention(q: torch.Tensor, cache: KVCache, kv_len=None, *, window: int, sinks: int = 0, q_len=None,
@@ -232,9 +240,15 @@ def windowed_attention(q: torch.Tensor, cache: KVCache, kv_len=None, *, window: 
     window, sinks = int(window), int(sinks)
     if window < 1 or sinks < 0:
         raise ValueError(f"window ({window}) must be >= 1 and sinks ({sinks}) >= 0")
-    most = (1 << 31) - 1  # (more than any cache holds)
-    return _masked(_lib.lib().vx_window_attn_fwd, _window_bytes, q, cache, kv_len, q_len, slots, scale, out, _none,
-                   (min(window, most), min(sinks, most), 1 if causal else 0))
+    window, sinks, causal = min(window, _MOST), min(sinks, _MOST), 1 if causal else 0  # (more than any cache holds)
+    sizes, held, out, args = _attend_args(q, cache, kv_len, q_len, slots, out)
+    if args is not None:
+        index, cap, B, Sq, H, Hk, D = sizes
+        nbytes = _window_bytes(index, cap, B, Sq, H, Hk, D, window, sinks, causal)
+        ws, ws_at = _workspace(nbytes, out.device)
+        _lib.launch(out.device, _lib.lib().vx_window_attn_fwd, *args, B, Sq, H, Hk, D, window, sinks, causal,
+                    D ** -0.5 if scale is None else float(scale), ws_at, nbytes)
+    return out
 
 
 def tree_attention(q: torch.Tensor, cache: KVCache, parents, kv_len=None, *, q_len=None, slots=None,
@@ -250,12 +264,18 @@ def tree_attention(q: torch.Tensor, cache: KVCache, parents, kv_len=None, *, q_l
     parents i - 1 this is cached_attention. The other arguments, lengths outside
     their range, queries without a visible key and rows of scale NaN are as there.
     """
-    def arguments(B: int, Sq: int, index: int):
-        shape = parents.shape if isinstance(parents, torch.Tensor) else torch.as_tensor(parents).shape
-        if shape != (B, Sq) and shape != (Sq,):
-            raise ValueError(f"parents must be ({B}, {Sq}) or ({Sq},); got {tuple(shape)}")
-        held, at = _ints(parents, Sq if len(shape) == 1 else B * Sq, index, "parents")
-        return held, (at, 0 if len(shape) == 1 else Sq)
     if parents is None:
         raise TypeError("parents must hold integers")
-    return _masked(_lib.lib().vx_tree_attn_fwd, _tree_bytes, q, cache, kv_len, q_len, slots, scale, out, arguments, ())
+    sizes, held, out, args = _attend_args(q, cache, kv_len, q_len, slots, out)
+    index, cap, B, Sq, H, Hk, D = sizes
+    shape = parents.shape if isinstance(parents, torch.Tensor) else torch.as_tensor(parents).shape
+    if shape != (B, Sq) and shape != (Sq,):
+        raise ValueError(f"parents must be ({B}, {Sq}) or ({Sq},); got {tuple(shape)}")
+    one = len(shape) == 1
+    parents, parents_at = _ints(parents, Sq if one else B * Sq, index, "parents")
+    if args is not None:
+        nbytes = _tree_bytes(index, cap, B, Sq, H, Hk, D)
+        ws, ws_at = _workspace(nbytes, out.device)
+        _lib.launch(out.device, _lib.lib().vx_tree_attn_fwd, *args, parents_at, 0 if one else Sq, B, Sq, H, Hk, D,
+                    D ** -0.5 if scale is None else float(scale), ws_at, nbytes)
+    return out
