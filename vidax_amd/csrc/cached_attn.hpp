@@ -338,6 +338,24 @@ __device__ __forceinline__ uint32_t tree_bits(const lds_u8* at, int r, int from)
   return __builtin_amdgcn_alignbit(w[(x >> 5) + 1], w[x >> 5], x & 31);
 }
 
+// Bits below n of 32 (n of any size).
+__device__ __forceinline__ uint32_t bits_below(int n) {
+  return n >= 32 ? ~0u : (1u << max(n, 0)) - 1u;
+}
+
+// The same of a window: bits of 32 keys from key0 on that a row with this bound sees.
+__device__ __forceinline__ uint32_t window_bits(const MaskedAttnArgs& a, int bound, int key0) {
+  const uint32_t hidden = bits_below(bound - a.window - key0) & ~bits_below(a.sinks - key0);
+  return bits_below(bound - key0) & ~hidden;
+}
+
+// x where bit i is set, else minus infinity: two instructions, none of them a compare
+// whose result a branch or a select has to wait for.
+__device__ __forceinline__ float masked_by(uint32_t bits, int i, float x) {
+  const uint32_t all = (uint32_t)((int32_t)(bits << (31 - i)) >> 31);
+  return __uint_as_float((__float_as_uint(x) & all) | (0xff800000u & ~all));
+}
+
 // Partial results in the workspace, one block per (part, kv head): rows x D
 // unnormalised fp32 outputs, then (reference point, sum) per row.
 __device__ __forceinline__ int64_t part_floats(int64_t rows, int D) { return (rows * (D + 2) + 3) & ~(int64_t)3; }
@@ -507,21 +525,23 @@ __device__ __forceinline__ void few_part(const Args<MASK>& a, const Part& pt, co
       }
       bool slow = key0 + kFewTile > all;  // some row does not see some key (or the products are rounded)
       if constexpr (MASK == kWindow) slow = slow || (key0 < from && key0 + kFewTile > a.sinks);
-      uint32_t bits = 0;
+      uint32_t bits = ~0u;  // (a mask's) of the lane's keys, key i at 16 (i / 8) + i % 8
       if constexpr (MASK == kTree) {
         if (slow) bits = tree_bits((lds_u8*)smem + C::kSmem, min(col, rows - 1), key0 - base) >> (8 * hf);
       }
-      auto seen = [&](int key, int i) {  // key, number i of the lane's 16
-        if constexpr (MASK == kTree) return (bits & (1u << (16 * (i >> 3) + (i & 7)))) != 0;
-        if constexpr (MASK == kWindow) return key < bound && (key >= bound - a.window || key < a.sinks);
-        return key < bound;
-      };
+      if constexpr (MASK == kWindow) {
+        if (slow) bits = window_bits(a, bound, key0) >> (8 * hf);
+      }
       float cc = c;
       if (slow) {
         cc = 1.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          S[i] = seen(key0 + 16 * (i >> 3) + 8 * hf + (i & 7), i) ? S[i] * c : -__builtin_inff();
+        for (int i = 0; i < 16; ++i) {
+          if constexpr (MASK == kPlain)
+            S[i] = key0 + 16 * (i >> 3) + 8 * hf + (i & 7) < bound ? S[i] * c : -__builtin_inff();
+          else
+            S[i] = masked_by(bits, 16 * (i >> 3) + (i & 7), S[i] * c);
+        }
       }
       float mx = S[0];
 #pragma unroll
@@ -550,7 +570,11 @@ __device__ __forceinline__ void few_part(const Args<MASK>& a, const Part& pt, co
             p[i] = fast_exp2(__builtin_fmaf(S[8 * j + e + i], cc, mneg));
             float w = p[i] * __uint_as_float(((vsc[j][e >> 2] >> (8 * ((e & 3) + i))) & 0xffu) << 23);
             // (its scale may be anything)
-            if (slow && !seen(key0 + 16 * j + 8 * hf + e + i, 8 * j + e + i)) w = 0.f;
+            if constexpr (MASK == kPlain) {
+              if (slow && !(key0 + 16 * j + 8 * hf + e + i < bound)) w = 0.f;
+            } else {
+              if (slow && !(bits & (1u << (16 * j + e + i)))) w = 0.f;
+            }
             P[j][e + i] = (bf16)w;
           }
           l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{(bf16)p[0], (bf16)p[1]}, one2, l, false);
@@ -890,14 +914,15 @@ __device__ __forceinline__ bool many_one(const Args<MASK>& a, const Part& pt, co
           if constexpr (MASK == kTree)
             bits = tree_bits((lds_u8*)smem + C::kSmem, min(wave * 32 + col, rows - 1 - rt * C::kRows),
                              key0 + k2 * 32 - base) >> (4 * hf);
-          auto seen = [&](int i) {
-            const int key = key0 + k2 * 32 + (i >> 2) * 8 + hf * 4 + (i & 3);
-            if constexpr (MASK == kTree) return (bits & (1u << ((i >> 2) * 8 + (i & 3)))) != 0;
-            if constexpr (MASK == kWindow) return key < bound && (key >= bound - a.window || key < a.sinks);
-            return key < bound;
-          };
+          if constexpr (MASK == kWindow) bits = window_bits(a, bound, key0 + k2 * 32) >> (4 * hf);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) S[k2][i] = seen(i) ? S[k2][i] * c : -__builtin_inff();
+          for (int i = 0; i < 16; ++i) {
+            const int key = key0 + k2 * 32 + (i >> 2) * 8 + hf * 4 + (i & 3);
+            if constexpr (MASK == kPlain)
+              S[k2][i] = key < bound ? S[k2][i] * c : -__builtin_inff();
+            else
+              S[k2][i] = masked_by(bits, (i >> 2) * 8 + (i & 3), S[k2][i] * c);
+          }
         }
       }
       // The reference point of the weights moves up when a tile's maximum is
