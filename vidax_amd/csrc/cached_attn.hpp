@@ -282,6 +282,17 @@ __device__ __forceinline__ int real_query(const CachedAttnArgs& a, int b, int i)
   return min(i, max(clamp_len(a.q_len, b, a.Sq) - 1, 0));
 }
 
+// The bounds of rows r0 .. r1 under a mask are those of their queries, which only
+// grow: the first row's and the last one's are the least and the most. (Scalar work;
+// over the lanes each would be five dependent LDS exchanges, half a microsecond.)
+struct Bounds {
+  int least, most;
+};
+__device__ __forceinline__ Bounds bounds_of(const CachedAttnArgs& a, int stream, int G, int r0, int r1, int len) {
+  return Bounds{__builtin_amdgcn_readfirstlane(own_bound(a, stream, real_query(a, stream, r0 / G), len)),
+                __builtin_amdgcn_readfirstlane(own_bound(a, stream, real_query(a, stream, r1 / G), len))};
+}
+
 // One launch's work on one kind of streams.
 struct Part {
   Streams s;
@@ -302,19 +313,34 @@ struct Part {
 constexpr int kTreeWords = kTreeMost / 32 + 3;  // (odd: rows lie in different banks)
 constexpr int tree_bytes(int rows) { return rows * kTreeWords * 4 + kTreeMost * 4; }
 
+// An item's parents, a lane's 64 apart: loaded ahead of what a part loads besides them.
+struct Parents {
+  int x[kTreeMost / 64];
+};
+__device__ __forceinline__ Parents load_parents(const MaskedAttnArgs& a, int stream) {
+  const int lane = threadIdx.x & 63, m = __builtin_amdgcn_readfirstlane(clamp_len(a.q_len, stream, a.Sq));
+  Parents p;
+#pragma unroll
+  for (int i = 0; i < kTreeMost / 64; ++i)
+    p.x[i] = 64 * i < m ? a.parents[stream * a.parents_stride + min(64 * i + lane, m - 1)] : -1;
+  return p;
+}
+
 // A wave fills the words of up to 32 rows for itself, row r the query of map.place(row0
 // + r), and needs no barrier: waves that fill the same rows write the same. A parent
 // that is not below its child counts as none, so every walk ends.
 __device__ __forceinline__ void fill_tree(const MaskedAttnArgs& a, const RowMap& map, int row0, int n, lds_u8* at,
-                                          int lds_row0) {
-  const int lane = threadIdx.x & 63, m = clamp_len(a.q_len, map.stream, a.Sq);
+                                          int lds_row0, const Parents& p) {
+  const int lane = threadIdx.x & 63, m = __builtin_amdgcn_readfirstlane(clamp_len(a.q_len, map.stream, a.Sq));
   VX_LDS int* const parents = (VX_LDS int*)at;
-  for (int i = lane; i < m; i += 64) parents[i] = a.parents[map.stream * a.parents_stride + i];
+#pragma unroll
+  for (int i = 0; i < kTreeMost / 64; ++i)
+    if (64 * i < m) parents[64 * i + lane] = p.x[i];
   if (lane < n) {
     int b, i, h;
     map.place(row0 + lane, b, i, h);
     VX_LDS uint32_t* const w = (VX_LDS uint32_t*)(at + kTreeMost * 4) + (lds_row0 + lane) * kTreeWords;
-    int x = kTreeWords - 1;  // the words from the last to the first, each written once
+    int x = ((m + 63) >> 5) + 1;  // the words that are read, from the last to the first, each written once
     for (int j = min(i, m - 1); j >= 0;) {
       const int word = 1 + (j >> 5);
       for (; x > word; --x) w[x] = 0u;
@@ -461,14 +487,15 @@ __device__ __forceinline__ void few_part(const Args<MASK>& a, const Part& pt, co
     map.place(row0 + min(col, rows - 1), rb, ri, rh);
     if constexpr (MASK != kPlain) ri = real_query(a, rb, ri);
     bf16x8 q[D / 16];
-    {
+    auto load_q = [&]() {
       const bf16* p = (const bf16*)a.q + rb * a.qs[0] + ri * a.qs[1] + rh * a.qs[2] + hf * 16;
 #pragma unroll
       for (int x = 0; x < D / 32; ++x) {
         q[2 * x] = *(const bf16x8*)(p + 32 * x);
         q[2 * x + 1] = *(const bf16x8*)(p + 32 * x + 8);
       }
-    }
+    };
+    if (MASK == kPlain) load_q();
     FewKeys own = keys(s, stream, len), shared = own;
     int pre_tiles = 0;
     if (BOTH) {
@@ -483,16 +510,23 @@ __device__ __forceinline__ void few_part(const Args<MASK>& a, const Part& pt, co
       for (int off = 16; off >= 1; off >>= 1) x = min(x, __shfl_xor(x, off, 64));
       return __builtin_amdgcn_readfirstlane(x);
     };
-    own.all = least(own.bound);
-    const int any = -least(-own.bound);  // keys that some row sees
+    int any;  // keys that some row sees
+    if constexpr (MASK == kPlain) {
+      own.all = least(own.bound);
+      any = -least(-own.bound);
+    } else {
+      const Bounds x = bounds_of(a, stream, map.G, row0, row0 + rows - 1, len);
+      own.all = x.least;
+      any = x.most;
+    }
     if (BOTH) shared.all = least(shared.bound);
     // The part's tiles that some row sees, and where all rows see all keys of one:
     // before own.all and, of a window, from `from` on or among the sinks.
     Pieces pieces{};
     int from = 0, base = 0;
     if constexpr (MASK == kWindow) {
-      const int low = least(own.bound > 0 ? own.bound : len);
-      from = -least(a.window - own.bound);
+      const int low = max(own.all, 1);  // (bounds grow one by one: the least that sees anything)
+      from = any - a.window;
       const int m = __builtin_amdgcn_readfirstlane(clamp_len(a.q_len, stream, a.Sq));
       pieces = pieces_of(stream_window<kFewTile>(a, len, m), window_of<kFewTile>(a, low, any), first, take);
     }
@@ -604,11 +638,17 @@ __device__ __forceinline__ void few_part(const Args<MASK>& a, const Part& pt, co
         stage(own, MASK == kWindow ? pieces.tile(t) : first + t - pre_tiles, buf);
     };
     const int n = here > wave ? (here - wave + W - 1) / W : 0;  // this wave's tiles
+    Parents parents;
+    bool masked = false;  // (the wave's last tile is, by its rows' bits)
+    if constexpr (MASK == kTree) {
+      masked = n > 0 && (first + wave + (n - 1) * W + 1) * kFewTile > own.all;
+      if (masked) parents = load_parents(a, stream);
+    }
     if (n > 0) stage_at(wave, 0);
     if (n > 1) stage_at(wave + W, 1);
-    if constexpr (MASK == kTree) {  // (the wave's last tile is masked by its bits)
-      if (n > 0 && (first + wave + (n - 1) * W + 1) * kFewTile > own.all)
-        fill_tree(a, map, row0, rows, (lds_u8*)smem + C::kSmem, 0);
+    if (MASK != kPlain) load_q();  // (behind the copies, which take longer)
+    if constexpr (MASK == kTree) {
+      if (masked) fill_tree(a, map, row0, rows, (lds_u8*)smem + C::kSmem, 0, parents);
     }
     for (int it = 0; it < n; ++it) {
       if (it + 1 < n)
@@ -748,8 +788,16 @@ __device__ __forceinline__ bool many_one(const Args<MASK>& a, const Part& pt, co
     for (int ds = 0; ds < kDS; ++ds) q[ds] = *(const bf16x8*)(p + ds * 16);
   }
   int all = bound;  // keys that every row of the wave sees
+  int from = 0;     // (window) the first that every row sees, the sinks apart
+  if constexpr (MASK == kPlain) {
 #pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) all = min(all, __shfl_xor(all, off, 64));
+    for (int off = 16; off >= 1; off >>= 1) all = min(all, __shfl_xor(all, off, 64));
+  } else {
+    const int r0 = min(rt * C::kRows + wave * 32, rows - 1);
+    const Bounds x = bounds_of(a, stream, map.G, r0, min(r0 + 31, rows - 1), len);
+    all = x.least;
+    if (MASK == kWindow) from = x.most - a.window;
+  }
   all = rounded ? 0 : __builtin_amdgcn_readfirstlane(all);
   // keys that any row of the workgroup sees
   int end = len, base = 0;
@@ -768,18 +816,11 @@ __device__ __forceinline__ bool many_one(const Args<MASK>& a, const Part& pt, co
   const int tiles = (end + kManyTile - 1) / kManyTile;
   const int t0 = first, n = MASK == kWindow ? pieces.count() : min(take, tiles - first);
   auto tile_at = [&](int u) { return MASK == kWindow ? pieces.tile(u) : t0 + u; };
-  int from = 0;  // (window) the first key that every row of the wave sees, the sinks apart
-  if constexpr (MASK == kWindow) {
-    int high = bound;
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) high = max(high, __shfl_xor(high, off, 64));
-    from = __builtin_amdgcn_readfirstlane(high) - a.window;
-  }
   if constexpr (MASK == kTree) {
     all = min(all, base);
     if (rounded || (t0 + n) * kManyTile > base)  // (some tile is masked by its bits)
       fill_tree(a, map, rt * C::kRows + wave * 32, min(rows - rt * C::kRows - wave * 32, 32),
-                (lds_u8*)smem + C::kSmem, wave * 32);
+                (lds_u8*)smem + C::kSmem, wave * 32, load_parents(a, stream));
   }
   f32x16 O[kDB];
 #pragma unroll
