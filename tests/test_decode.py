@@ -202,8 +202,9 @@ def test_a_missing_workspace_is_refused():
 
 
 # ------------------------------------------------------------------ the turns
-@pytest.mark.parametrize("D,split,shared", [(128, (44, 42, 42), False), (128, (32, 48, 48), True), (64, (16, 16, 16), False),
-                                            (64, (64,), False), (64, (8, 0, 24, 32), True)])
+@pytest.mark.parametrize("D,split,shared", [(128, (44, 42, 42), False), (128, (32, 48, 48), True),
+                                            (64, (16, 16, 16), False), (64, (64,), False),
+                                            (64, (8, 0, 24, 32), True)])
 @pytest.mark.parametrize("base,scale", [(10000.0, None), (5e6, (0.25, 1.0, 3.0, 1e6))])
 def test_turns_are_the_ladders(D, split, shared, base, scale):
     """turns / 2^64 is scale * base^-e / 2 pi modulo 1, as far as 64 bits tell."""
@@ -363,7 +364,8 @@ def test_positions_and_rows_of_any_layout(gpu):
     p = torch.randint(0, 900, (2, 21, 3), generator=g, device=gpu, dtype=torch.int32)
     want = vx.apply_axis_rope(x.contiguous(), p, rope)
     odd = torch.zeros(x.numel() + 1, dtype=torch.bfloat16, device=gpu)[1:].reshape(x.shape).copy_(x)
-    for rows in (x, odd, x.transpose(1, 2).contiguous().transpose(1, 2), x.transpose(2, 3).contiguous().transpose(2, 3)):
+    for rows in (x, odd, x.transpose(1, 2).contiguous().transpose(1, 2),
+                 x.transpose(2, 3).contiguous().transpose(2, 3)):
         assert torch.equal(vx.apply_axis_rope(rows, p, rope), want)
     for q in (p.permute(2, 0, 1).contiguous().permute(1, 2, 0), p.long(), p.cpu(), p.to(torch.int16), p.tolist()):
         assert torch.equal(vx.apply_axis_rope(x, q, rope), want)
@@ -465,7 +467,8 @@ def test_kv_cache_write_rope(gpu, case, halves):
     rng = np.random.default_rng(B * S + D)
     raw = [rng.integers(0, 256, (4, Hk, cap, D), np.uint8) for _ in range(2)]
     raw += [rng.integers(0, 256, (4, Hk, cap), np.uint8) for _ in range(2)]
-    make = lambda: vx.KVCache(*(torch.from_numpy(x.copy()).to(gpu).view(t) for x, t in zip(raw, (E4M3, E4M3, E8M0, E8M0))))
+    types = (E4M3, E4M3, E8M0, E8M0)
+    make = lambda: vx.KVCache(*(torch.from_numpy(x.copy()).to(gpu).view(t) for x, t in zip(raw, types)))
     rope = vx.create_axis_rope(D, split, halves=halves, device=gpu)
     k, v = (_bf16(rng.standard_normal((B, S, Hk, D)) * np.exp(3 * rng.standard_normal((B, S, Hk, 1))), gpu)
             for _ in range(2))
@@ -494,7 +497,8 @@ def test_kv_cache_write_rope(gpu, case, halves):
         untouched[slot, pos] = False
         for h in range(Hk):
             top = np.abs(y[b, t, h]).max()
-            fits = {int(CO.quantise(np.array([[m]]))[1][0]) for m in (top - slack[b, t, h].max(), top + slack[b, t, h].max())}
+            most = slack[b, t, h].max()
+            fits = {int(CO.quantise(np.array([[m]]))[1][0]) for m in (top - most, top + most)}
             s = int(got[2][slot, h, pos])
             assert s in fits, (slot, pos, h, s, fits)
             tol = np.maximum(2.0 ** -4 * np.abs(y[b, t, h]), 2.0 ** (s - 127 - 10)) + (1 + 2.0 ** -4) * slack[b, t, h]
@@ -722,8 +726,8 @@ def test_tree_attention(gpu, case):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,Sq,H,Hk,D,cap", [(70, 5, 8, 2, 128, 1536), (9, 30, 4, 1, 64, 4096), (3, 100, 8, 2, 128, 2048),
-                                             (130, 9, 2, 1, 64, 192)])
+@pytest.mark.parametrize("B,Sq,H,Hk,D,cap", [(70, 5, 8, 2, 128, 1536), (9, 30, 4, 1, 64, 4096),
+                                             (3, 100, 8, 2, 128, 2048), (130, 9, 2, 1, 64, 192)])
 def test_trees_over_many_lengths(gpu, B, Sq, H, Hk, D, cap):
     print(f"[case] trees B={B} Sq={Sq} H={H}/{Hk} D={D} cap={cap}", flush=True)
     rng = np.random.default_rng(B + cap)
@@ -753,7 +757,8 @@ def _plan_call(mask, gpu, rng, q, cache, kv_len, **kw):
         return sees, lambda: vx.windowed_attention(q, cache, _ints(kv_len, gpu), window=window, sinks=sinks, **kw)
     parents = _tree(rng, B, Sq, "any")
     on = _ints(parents.tolist(), gpu)
-    return (lambda b, n, m: O.tree_sees(n, m, parents[b])), lambda: vx.tree_attention(q, cache, on, _ints(kv_len, gpu), **kw)
+    lens = _ints(kv_len, gpu)
+    return (lambda b, n, m: O.tree_sees(n, m, parents[b])), lambda: vx.tree_attention(q, cache, on, lens, **kw)
 
 
 @pytest.mark.gpu
@@ -831,6 +836,33 @@ def test_logits_of_any_size(gpu, plan, mask, size):
             ref, spread = w @ x, w @ np.abs(x)
             tol = 2 * 2.0 ** -8 * np.abs(ref) + spread * (2.0 ** -8 + 2 * (cap + 64) * 2.0 ** -24)
             assert (np.abs(got[b, :, h] - ref) <= tol).all(), (b, h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mask", ["window", "tree"])
+@pytest.mark.parametrize("plan", PLANS, ids=[f"{p[0]} {p[5]}" for p in PLANS])
+def test_queries_that_are_not_finite(gpu, plan, mask):
+    """A NaN in a query makes NaN that query's output alone; in padding rows it is
+    not looked at, and they give zeros."""
+    name, B, Sq, H, Hk, cap, kv_len = plan
+    rng = np.random.default_rng(cap)
+    cap = (cap + 63) // 64 * 64
+    cache = _cache_of(rng, B, Hk, cap, 128, gpu, np.array(kv_len))
+    q = _bf16(rng.standard_normal((B, Sq, H, 128)), gpu)
+    q_len = [Sq - min(b, Sq - 1) * (Sq // 3 + 1) if Sq > 2 else Sq for b in range(B)]
+    q_len = [max(m, 1) for m in q_len]
+    sees, call = _plan_call(mask, gpu, rng, q, cache, kv_len, q_len=_ints(q_len, gpu))
+    want = call()
+    for b in range(B):
+        q[b, q_len[b]:] = float("nan")
+    assert torch.equal(call(), want) and _lib.last_launch() == name.format(D=128, mask=mask)
+    assert all((want[b, q_len[b]:] == 0).all() for b in range(B))
+    q[0, Sq // 2, H - 1, 5] = float("nan")
+    q[B - 1, 0, 0, 127] = float("nan")
+    got = call()
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[0, Sq // 2, H - 1] = hit[B - 1, 0, 0] = True
+    assert got[hit].isnan().all() and torch.equal(got[~hit], want[~hit])
 
 
 @pytest.mark.gpu
@@ -926,8 +958,10 @@ def _rollout(gpu, on_stream=None):
     q, k, v = new(9, H), new(9, Hk), new(9, Hk)
     turned = vx.apply_axis_rope(q, p, rope)
     vx.kv_cache_write_rope(cache, k, v, p, rope, _ints([n, n], gpu), slots=_ints(slots, gpu))
-    drafted = vx.tree_attention(turned, cache, _ints(parents.tolist(), gpu), _ints([n + 9] * 2, gpu), slots=_ints(slots, gpu))
-    _assert_close(drafted, turned, _held(cache), lambda b, n, m: O.tree_sees(n, m, parents), kv_len=[n + 9] * 2, slots=slots)
+    drafted = vx.tree_attention(turned, cache, _ints(parents.tolist(), gpu), _ints([n + 9] * 2, gpu),
+                                slots=_ints(slots, gpu))
+    _assert_close(drafted, turned, _held(cache), lambda b, n, m: O.tree_sees(n, m, parents), kv_len=[n + 9] * 2,
+                  slots=slots)
     # the path 0 - 1 - 3 - 6 - 8 is accepted: written as the sequence's next tokens, its queries see what they saw
     path = [0, 1, 3, 6, 8]
     vx.kv_cache_write_rope(cache, k[:, path], v[:, path], p[path], rope, _ints([n, n], gpu), slots=_ints(slots, gpu))
@@ -945,7 +979,8 @@ def _rollout(gpu, on_stream=None):
         vx.kv_cache_write_rope(cache, k, v, p, rope, _ints([n, n], gpu), slots=_ints(slots, gpu))
         n += 1
         got = vx.windowed_attention(turned, cache, _ints([n, n], gpu), window=50, sinks=4, slots=_ints(slots, gpu))
-        _assert_close(got, turned, _held(cache), lambda b, n, m: O.window_sees(n, m, 50, 4, True), kv_len=[n, n], slots=slots)
+        _assert_close(got, turned, _held(cache), lambda b, n, m: O.window_sees(n, m, 50, 4, True), kv_len=[n, n],
+                      slots=slots)
 
 
 @pytest.mark.gpu
@@ -985,7 +1020,8 @@ def test_graph_replays(gpu, Sq, cap):
         r = np.random.default_rng(seed)
         for t in (q, k, v):
             t.copy_(torch.from_numpy(r.standard_normal(t.shape).astype(np.float32)))
-        n, used = [int(cap * share) // (i + 1) for i in range(B)], [max(int(Sq * share), 1) if i else Sq for i in range(B)]
+        n = [int(cap * share) // (i + 1) for i in range(B)]
+        used = [max(int(Sq * share), 1) if i else Sq for i in range(B)]
         kv_len.copy_(torch.tensor(n))
         m.copy_(torch.tensor(used))
         start.copy_(torch.tensor([a - b for a, b in zip(n, used)]))
@@ -1020,7 +1056,8 @@ def test_two_streams_at_once(gpu):
     cache = _cache_of(rng, 4, 4, 8192, 128, gpu)
     q = [_bf16(rng.standard_normal((4, 3, 8, 128)), gpu) for _ in range(2)]
     parents = _ints([-1, 0, 0], gpu)
-    calls = [lambda: vx.windowed_attention(q[0], cache, window=6000, sinks=8), lambda: vx.tree_attention(q[1], cache, parents)]
+    calls = [lambda: vx.windowed_attention(q[0], cache, window=6000, sinks=8),
+             lambda: vx.tree_attention(q[1], cache, parents)]
     want = [c() for c in calls]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
@@ -1042,7 +1079,8 @@ def test_host_integers_and_captures(gpu):
     q = torch.randn((2, 3, 4, 64), device=gpu).bfloat16()
     par = [[-1, 0, 0], [-1, -1, 1]]
     want = vx.tree_attention(q, cache, _ints(par, gpu), _ints([50, 60], gpu))
-    for x in (par, np.array(par), torch.tensor(par), torch.tensor(par, device=gpu), torch.tensor(par, dtype=torch.int8)):
+    for x in (par, np.array(par), torch.tensor(par), torch.tensor(par, device=gpu),
+              torch.tensor(par, dtype=torch.int8)):
         assert torch.equal(vx.tree_attention(q, cache, x, [50, 60]), want)
     want = vx.tree_attention(q, cache, _ints([par[0]] * 2, gpu))
     assert torch.equal(vx.tree_attention(q, cache, par[0]), want)

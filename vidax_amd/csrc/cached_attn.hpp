@@ -328,20 +328,46 @@ __device__ __forceinline__ Parents load_parents(const MaskedAttnArgs& a, int str
 
 // A wave fills the words of up to 32 rows for itself, row r the query of map.place(row0
 // + r), and needs no barrier: waves that fill the same rows write the same. A parent
-// that is not below its child counts as none, so every walk ends.
+// that is not below its child counts as none, so every walk ends. Up to 64 drafted
+// tokens are a lane each, whose part of its chain doubles from round to round; rows of
+// more walk their chains out in LDS (a step is as long as a round).
 __device__ __forceinline__ void fill_tree(const MaskedAttnArgs& a, const RowMap& map, int row0, int n, lds_u8* at,
                                           int lds_row0, const Parents& p) {
   const int lane = threadIdx.x & 63, m = __builtin_amdgcn_readfirstlane(clamp_len(a.q_len, map.stream, a.Sq));
+  int b, query, h;
+  map.place(row0 + lane, b, query, h);
+  query = min(query, m - 1);
+  VX_LDS uint32_t* const w = (VX_LDS uint32_t*)(at + kTreeMost * 4) + (lds_row0 + lane) * kTreeWords;
+  if (m <= 64) {
+    // the lane's token and its nearest 2^r - 1 ancestors, and the 2^r-th (none: -1)
+    uint32_t lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
+    int up = p.x[0] >= 0 && p.x[0] < lane && lane < m ? p.x[0] : -1;
+    while (__builtin_amdgcn_ballot_w64(up >= 0) != 0) {
+      const uint32_t l = __shfl((int)lo, max(up, 0), 64), g = __shfl((int)hi, max(up, 0), 64);
+      const int next = __shfl(up, max(up, 0), 64);
+      if (up >= 0) {
+        lo |= l;
+        hi |= g;
+        up = next;
+      }
+    }
+    lo = __shfl((int)lo, max(query, 0), 64);
+    hi = __shfl((int)hi, max(query, 0), 64);
+    if (lane < n) {
+      w[0] = ~0u;
+      w[1] = lo;
+      w[2] = hi;
+      w[3] = w[4] = 0u;
+    }
+    return;
+  }
   VX_LDS int* const parents = (VX_LDS int*)at;
 #pragma unroll
   for (int i = 0; i < kTreeMost / 64; ++i)
     if (64 * i < m) parents[64 * i + lane] = p.x[i];
   if (lane < n) {
-    int b, i, h;
-    map.place(row0 + lane, b, i, h);
-    VX_LDS uint32_t* const w = (VX_LDS uint32_t*)(at + kTreeMost * 4) + (lds_row0 + lane) * kTreeWords;
     int x = ((m + 63) >> 5) + 1;  // the words that are read, from the last to the first, each written once
-    for (int j = min(i, m - 1); j >= 0;) {
+    for (int j = query; j >= 0;) {
       const int word = 1 + (j >> 5);
       for (; x > word; --x) w[x] = 0u;
       uint32_t bits = 0;
@@ -371,7 +397,7 @@ __device__ __forceinline__ uint32_t bits_below(int n) {
 
 // The same of a window: bits of 32 keys from key0 on that a row with this bound sees.
 __device__ __forceinline__ uint32_t window_bits(const MaskedAttnArgs& a, int bound, int key0) {
-  const uint32_t hidden = bits_below(bound - a.window - key0) & ~bits_below(a.sinks - key0);
+  const uint32_t hidden = bits_below(max(bound - a.window, 0) - key0) & ~bits_below(a.sinks - key0);
   return bits_below(bound - key0) & ~hidden;
 }
 
@@ -540,7 +566,7 @@ __device__ __forceinline__ void few_part(const Args<MASK>& a, const Part& pt, co
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) O[db] = f32x16{};
     float m = kNone, l = 0.f;
-    auto step = [&](const int key0, const int bound, const int all, const int buf) {
+    auto step = [&](const int key0, const int bound, const int all, const int buf, const bool start) {
       const lds_u8* kb = ring + buf * C::kBuf;
       const lds_u8* vb = kb + C::kTileBytes;
       const lds_u8* sc = vb + C::kTileBytes;
@@ -584,9 +610,11 @@ __device__ __forceinline__ void few_part(const Args<MASK>& a, const Part& pt, co
       if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
         const float mn = fmaxf(m, mx), alpha = fast_exp2(m - mn);
         m = mn;
-        l *= alpha;
+        if (MASK == kPlain || !start) {  // (there is nothing yet)
+          l *= alpha;
 #pragma unroll
-        for (int db = 0; db < D / 32; ++db) O[db] *= alpha;
+          for (int db = 0; db < D / 32; ++db) O[db] *= alpha;
+        }
       }
       // The weights times their value rows' scales, rounded to bf16 (a power of two changes
       // no rounding), and the sum of the rounded weights, so that those that multiply V
@@ -657,8 +685,9 @@ __device__ __forceinline__ void few_part(const Args<MASK>& a, const Part& pt, co
         wait_copies<0>();
       const int t = wave + it * W;
       const bool of_prefix = BOTH && t < pre_tiles;
-      step((of_prefix ? t : MASK == kWindow ? pieces.tile(t) : first + t - pre_tiles) * kFewTile, of_prefix ? shared.bound : own.bound,
-           of_prefix ? shared.all : own.all, it & 1);
+      step((of_prefix ? t : MASK == kWindow ? pieces.tile(t) : first + t - pre_tiles) * kFewTile,
+           of_prefix ? shared.bound : own.bound,
+           of_prefix ? shared.all : own.all, it & 1, it == 0);
       if (it + 2 < n) {
         wait_lds_reads();
         stage_at(t + 2 * W, it & 1);
@@ -1151,8 +1180,8 @@ __device__ __forceinline__ void many_part(const Args<MASK>& a, const Part& pt, c
   while (left > 0) {
     const int tiles = tiles_of<kManyTile, MASK>(a, stream, len);
     const int take = pt.budget == 0 ? tiles : min(left, tiles - first);
-    if (!many_one<D, MASK>(a, pt, kvh, rt, stream, len, first, take, take == tiles, pt.budget == 0 ? item : item + stream,
-                     rounded, smem)) {
+    if (!many_one<D, MASK>(a, pt, kvh, rt, stream, len, first, take, take == tiles,
+                           pt.budget == 0 ? item : item + stream, rounded, smem)) {
       rounded = true;
       __syncthreads();  // (the tiles' buffers take the part again)
       continue;
@@ -1184,7 +1213,8 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const CachedAttnArgs 
 
 template <int D, int W, int MASK>
 __global__ __launch_bounds__(W * 64, 2) void few_masked_kernel(const Args<MASK> a, const Part own) {
-  __shared__ __attribute__((aligned(256))) unsigned char smem[FewCfg<D, W>::kSmem + (MASK == kTree ? tree_bytes(32) : 0)];
+  constexpr int kTreeBytes = MASK == kTree ? tree_bytes(32) : 0;
+  __shared__ __attribute__((aligned(256))) unsigned char smem[FewCfg<D, W>::kSmem + kTreeBytes];
   few_part<D, W, false, MASK>(a, own, nullptr, blockIdx.x, smem);
 }
 
@@ -1335,8 +1365,8 @@ inline bool runs_few(int64_t heads, int64_t rows, int64_t cap, int D, int64_t cu
   return 0.4125 * (double)((rows + 31) / 32) * x < 1.05 * (double)((rows + kManyRows - 1) / kManyRows) * x + 5;
 }
 
-inline Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, int D, int64_t slots, int64_t cus, bool prefix,
-                  bool with_prefix) {
+inline Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, int D, int64_t slots, int64_t cus,
+                         bool prefix, bool with_prefix) {
   Planned h;
   Part& p = h.p;
   p.rows = (int)rows;
