@@ -453,6 +453,11 @@ WRITES = [
     (3, 9, 2, 128, 128, [4, 4, 4], [9, 9, 12], [5, -1, 1], (32, 48, 48)),
     (3, 20, 2, 64, 64, [0, 10, 5], None, [1, 1, 1], (32, 32)),       # the same slot and positions twice
     (1, 700, 5, 128, 1024, [123], [651], None, (44, 42, 42)),
+    # heads in fours: a workgroup's waves share their tokens' angles
+    (1, 1, 4, 64, 64, [63], None, None, (64,)),
+    (2, 33, 4, 128, 128, [1, 95], [33, 20], None, (44, 42, 42)),
+    (3, 17, 8, 64, 64, [0, 5, 47], [17, 0, 9], [5, 2, 1], (16, 24, 24)),
+    (2, 100, 12, 128, 128, [0, 30], [100, 65], [1, 1], (32, 48, 48)),
 ]
 
 

@@ -38,7 +38,7 @@ __global__ __launch_bounds__(kWaves * 64) void axis_rope_kernel(const AxisRopeAr
     }
   }
   float s[8], co[8];
-  rope_angles(rope_table<D>(a.rope, c), rope_place(a.rope, b * a.rope.ps[0] + (int64_t)t * a.rope.ps[1]),
+  rope_angles(rope_table<8>(a.rope, 8 * c), rope_place(a.rope, b * a.rope.ps[0] + (int64_t)t * a.rope.ps[1]),
               a.inverse != 0, s, co);
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {

@@ -102,8 +102,10 @@ __device__ __forceinline__ u32x4 quantise(const float (&x)[2][8], uint32_t s) {
 }
 
 // PAIRS: keys are turned (kNoRope: as they are) on the way, in fp32, and rounded once.
-// Then lanes take their channels as the pairs lie (see vx_axis_rope.hpp).
-template <int D, int PAIRS>
+// Then lanes take their channels as the pairs lie (see vx_axis_rope.hpp). SHARED: the
+// workgroup's waves have four heads of the same tokens, and form a quarter of a token's
+// angles each for all four, by way of LDS.
+template <int D, int PAIRS, bool SHARED = false>
 __device__ __forceinline__ void write_rows(const KvWriteArgs& a, const AxisRope& rope) {
   using R = Rows<D>;
   const int lane = threadIdx.x & 63;
@@ -167,6 +169,23 @@ __device__ __forceinline__ void write_rows(const KvWriteArgs& a, const AxisRope&
     }
   }
   const int64_t row0 = ((int64_t)slot * hk + head) * a.c.cap;
+  __shared__ f32x4 angles[SHARED ? R::kPasses : 1][SHARED ? 64 : 1][4];  // a lane's eight sines, then cosines
+  if constexpr (SHARED) {
+    static_assert(kWaves == 4, "two of a lane's pairs each");
+    const int mine = 2 * (threadIdx.x >> 6);
+    const RopeTable<2> table = rope_table<2>(rope, 8 * c + mine);
+#pragma unroll
+    for (int p = 0; p < R::kPasses; ++p) {
+      float s[2], co[2];
+      rope_angles(table, place[p], false, s, co);
+      float* const at = (float*)angles[p][lane] + mine;
+      at[0] = s[0];
+      at[1] = s[1];
+      at[8] = co[0];
+      at[9] = co[1];
+    }
+    __syncthreads();  // (whole workgroups are here: their waves' tokens are the same)
+  }
 #pragma unroll
   for (int p = 0; p < R::kPasses; ++p) {
     uint32_t sk;
@@ -175,7 +194,12 @@ __device__ __forceinline__ void write_rows(const KvWriteArgs& a, const AxisRope&
       sk = scale_byte(row_amax<D>(xk[p]));
     } else {
       float s[8], co[8];
-      rope_angles(rope_table<D>(rope, c), place[p], false, s, co);
+      if constexpr (SHARED) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = angles[p][lane][e >> 2][e & 3], co[e] = angles[p][lane][2 + (e >> 2)][e & 3];
+      } else {
+        rope_angles(rope_table<8>(rope, 8 * c), place[p], false, s, co);
+      }
       rope_turn<PAIRS>(xk[p], s, co, y);
       sk = scale_byte32(row_amax<D>(y));
     }
@@ -210,9 +234,9 @@ __global__ __launch_bounds__(kWaves * 64) void kv_write_kernel(const KvWriteArgs
   write_rows<D, kNoRope>(a, AxisRope{});
 }
 
-template <int D, int PAIRS>
+template <int D, int PAIRS, bool SHARED>
 __global__ __launch_bounds__(kWaves * 64) void kv_write_rope_kernel(const KvWriteArgs a, const AxisRope rope) {
-  write_rows<D, PAIRS>(a, rope);
+  write_rows<D, PAIRS, SHARED>(a, rope);
 }
 
 template <int D>
@@ -309,6 +333,16 @@ dim3 grid_of(int B, int S, int Hk) {
   return dim3((unsigned)((waves + kWaves - 1) / kWaves), (unsigned)B);
 }
 
+// (Waves go by head, then by tokens: with heads in fours a workgroup has whole tokens.)
+template <int D, int PAIRS>
+void write_rope(const KvWriteArgs& a, const AxisRope& rope, hipStream_t st) {
+  const dim3 grid = grid_of(a.B, a.S, a.c.Hk), threads(kWaves * 64);
+  if (a.c.Hk % kWaves == 0)
+    hipLaunchKernelGGL((kv_write_rope_kernel<D, PAIRS, true>), grid, threads, 0, st, a, rope);
+  else
+    hipLaunchKernelGGL((kv_write_rope_kernel<D, PAIRS, false>), grid, threads, 0, st, a, rope);
+}
+
 }  // namespace
 
 int launch_kv_write(const KvWriteArgs& a, void* stream, const char** launched) {
@@ -322,16 +356,11 @@ int launch_kv_write(const KvWriteArgs& a, void* stream, const char** launched) {
 }
 
 int launch_kv_write_rope(const KvWriteArgs& a, const AxisRope& rope, void* stream, const char** launched) {
-  const dim3 grid = grid_of(a.B, a.S, a.c.Hk), threads(kWaves * 64);
   const hipStream_t st = (hipStream_t)stream;
-  if (a.c.D == 128 && rope.halves)
-    hipLaunchKernelGGL((kv_write_rope_kernel<128, kHalves>), grid, threads, 0, st, a, rope);
-  else if (a.c.D == 128)
-    hipLaunchKernelGGL((kv_write_rope_kernel<128, kAdjacent>), grid, threads, 0, st, a, rope);
-  else if (rope.halves)
-    hipLaunchKernelGGL((kv_write_rope_kernel<64, kHalves>), grid, threads, 0, st, a, rope);
+  if (a.c.D == 128)
+    rope.halves ? write_rope<128, kHalves>(a, rope, st) : write_rope<128, kAdjacent>(a, rope, st);
   else
-    hipLaunchKernelGGL((kv_write_rope_kernel<64, kAdjacent>), grid, threads, 0, st, a, rope);
+    rope.halves ? write_rope<64, kHalves>(a, rope, st) : write_rope<64, kAdjacent>(a, rope, st);
   *launched = a.c.D == 128 ? (rope.halves ? "kv_write_rope_kernel<128, halves>" : "kv_write_rope_kernel<128, adjacent>")
                            : (rope.halves ? "kv_write_rope_kernel<64, halves>" : "kv_write_rope_kernel<64, adjacent>");
   return (int)hipGetLastError();

@@ -46,19 +46,20 @@ __device__ __forceinline__ void sincos_turns(uint32_t a, float& s, float& c) {
   c = __uint_as_float(__float_as_uint(y) ^ (((q + 1) & 2) << 30));
 }
 
-// The lane's eight pairs of a token: their sines and cosines.
+// N pairs, from `first` on.
+template <int N>
 struct RopeTable {
-  uint64_t turns[8];
-  int32_t axis[8];
+  uint64_t turns[N];
+  int32_t axis[N];
 };
 
-template <int D>
-__device__ __forceinline__ RopeTable rope_table(const AxisRope& r, int c) {
-  RopeTable t;
+template <int N>
+__device__ __forceinline__ RopeTable<N> rope_table(const AxisRope& r, int first) {
+  RopeTable<N> t;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    t.turns[e] = r.turns[8 * c + e];
-    t.axis[e] = r.axis[8 * c + e];
+  for (int e = 0; e < N; ++e) {
+    t.turns[e] = r.turns[first + e];
+    t.axis[e] = r.axis[first + e];
   }
   return t;
 }
@@ -74,10 +75,12 @@ __device__ __forceinline__ RopePlace rope_place(const AxisRope& r, int64_t at) {
   return p;
 }
 
-__device__ __forceinline__ void rope_angles(const RopeTable& t, const RopePlace& at, bool back, float (&s)[8],
-                                            float (&c)[8]) {
+// Their sines and cosines at a token's positions.
+template <int N>
+__device__ __forceinline__ void rope_angles(const RopeTable<N>& t, const RopePlace& at, bool back, float (&s)[N],
+                                            float (&c)[N]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < N; ++e) {
     int32_t p = 0;  // (a pair of an axis that there is not does not turn)
 #pragma unroll
     for (int x = 0; x < kRopeAxes; ++x) p = t.axis[e] == x ? at.p[x] : p;
