@@ -444,6 +444,32 @@ def test_the_grid_tables_are_a_case_of_it():
     assert np.abs(np.sin(a) - sin[0, :, 0].double().numpy()).max() <= 4 * 4 * 2.0 ** -23
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("halves", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+def test_pairs_that_do_not_turn_keep_their_values(gpu, D, halves):
+    """Bit for bit, with infinities, NaN and zeros of either sign beside them: pairs past
+    the split at any position, and all pairs at position 0."""
+    rope = vx.create_axis_rope(D, (D // 4,), halves=halves, device=gpu)
+    x = np.random.default_rng(D).standard_normal((1, 2, 3, D))
+    special = np.array([np.inf, -np.inf, np.nan, 0.0, -0.0, 3.0])
+    u, w = np.meshgrid(special, special)
+    still = [j for j in range(D // 2) if rope.turns[j] == 0]
+    assert len(still) == D // 2 - D // 8
+    at = lambda j: (j, j + D // 2) if halves else (2 * j, 2 * j + 1)
+    for i, (p, q) in enumerate(zip(u.ravel(), w.ravel())):
+        x[:, :, i % 3, list(at(still[i // 3]))] = p, q
+        x[:, 1, i % 3, list(at(i // 3 % (D // 8)))] = p, q
+    x = _bf16(x, gpu)
+    for inverse in (False, True):
+        y = vx.apply_axis_rope(x, _ints([[123457], [0]], gpu), rope, inverse=inverse)
+        assert (x.isnan() == y.isnan()).all(), inverse
+        same = (x.view(torch.int16) == y.view(torch.int16)) | x.isnan()
+        assert same[:, 1].all(), inverse
+        for j in still:
+            assert same[:, 0, :, list(at(j))].all(), (inverse, j)
+
+
 WRITES = [
     # B, S, Hk, D, cap, start, num, slots, split
     (1, 1, 1, 64, 64, None, None, None, (16, 24, 24)),

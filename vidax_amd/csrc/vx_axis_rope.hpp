@@ -7,8 +7,9 @@
 // turn (and by half a unit of turns[j], 2^-65, times the position). The nearest
 // quarter turn is the top bits' own; what is left, r in [-pi/4, pi/4), goes through
 // the Taylor polynomials of sine and cosine to r^9 and r^8, whose remainders,
-// r^11 / 11! and r^10 / 10!, are below 1.8e-9 and 2.5e-8. With their roundings a sine
-// or cosine is off by at most 2^-22. A pair that does not turn keeps its values.
+// r^11 / 11! and r^10 / 10!, are below 1.8e-9 and 2.5e-8. With their roundings (three
+// half steps in r, one in the result) a sine or cosine is off by less than 2^-21. A pair
+// that does not turn keeps its values.
 //
 // Lanes: D / 16 to a head's row, each with eight pairs: channels 16 c .. 16 c + 15
 // (adjacent pairs) or 8 c .. 8 c + 7 of both halves (pairs (j, j + D / 2)).
@@ -102,8 +103,11 @@ __device__ __forceinline__ void rope_turn(const u32x4 (&x)[2], const float (&s)[
       return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
     };
     const float a = value(g0, i0), b = value(g1, i1);
-    y[g0][i0] = __builtin_fmaf(a, c[e], -(b * s[e]));
-    y[g1][i1] = __builtin_fmaf(a, s[e], b * c[e]);
+    // (without a turn neither channel takes the other's infinity or NaN, nor loses the
+    // sign of a zero)
+    const bool still = s[e] == 0.0f && c[e] > 0.0f;
+    y[g0][i0] = still ? a : __builtin_fmaf(a, c[e], -(b * s[e]));
+    y[g1][i1] = still ? b : __builtin_fmaf(a, s[e], b * c[e]);
   }
 }
 
