@@ -770,12 +770,12 @@ __device__ __forceinline__ void few_part(const Args<MASK>& a, const Part& pt, co
 // ------------------------------------------------------------------ many rows
 constexpr int kManyTile = 64;  // keys per tile of many_part
 
-// A workgroup of kWaves waves of 32 rows. LDS: two K tiles, two V tiles of bf16; a
+// A workgroup of W waves of 32 rows. LDS: two K tiles, two V tiles of bf16; a
 // tile is D / 64 half planes of 64 keys x 128 bytes, a row's 16-byte chunks XOR
 // half_swizzle (as in flash_fwd.hip).
-template <int D>
+template <int D, int W = kWaves>
 struct ManyCfg {
-  static constexpr int kRows = 32 * kWaves;
+  static constexpr int kThreads = W * 64, kRows = 32 * W;
   static constexpr int kHalf = kManyTile * 128;         // 64 keys x 64 dims
   static constexpr int kTileBytes = kManyTile * D * 2;  // of K, and of V
   static constexpr int kVBuf = 0, kKBuf = 2 * kTileBytes;
@@ -790,12 +790,12 @@ struct ManyCfg {
 // kRows + 0 .. kRows - 1 of kv head kvh; part_no: the number of its partial result.
 // False, with nothing written, if a reference point is far and the products are not
 // `rounded`. (kTree: smem holds tree_bytes(kRows) more.)
-template <int D, int MASK>
+template <int D, int MASK, int W>
 __device__ __forceinline__ bool many_one(const Args<MASK>& a, const Part& pt, const int kvh, const int rt,
                                          const int stream, const int len, const int first, const int take,
                                          const bool whole, const int part_no, const bool rounded,
                                          unsigned char* smem) {
-  using C = ManyCfg<D>;
+  using C = ManyCfg<D, W>;
   const Streams& s = pt.s;
   const int rows = pt.rows, Hk = s.c.Hk;
   constexpr int kDB = C::kDB, kDS = C::kDS, kPV = C::kPV, kSlots = C::kSlots, kAhead = C::kAhead;
@@ -947,9 +947,9 @@ __device__ __forceinline__ bool many_one(const Args<MASK>& a, const Part& pt, co
     Raw w0;
     load(kg, 0, w0);
     load(kg, min(1, n - 1), wk);
-    const int kZero = kThreads * 16;
+    const int kZero = C::kThreads * 16;
 #pragma unroll
-    for (int p = 0; p < C::kTileBytes / (kThreads * 16); ++p)
+    for (int p = 0; p < C::kTileBytes / (C::kThreads * 16); ++p)
       *(VX_LDS u32x4*)((lds_u8*)smem + C::kVBuf + C::kTileBytes + p * kZero + tid * 16) = u32x4{0, 0, 0, 0};
     store_all(w0, true, C::kKBuf);
     store_all(wk, true, C::kKBuf + C::kTileBytes);
@@ -1111,7 +1111,7 @@ __device__ __forceinline__ bool many_one(const Args<MASK>& a, const Part& pt, co
       __syncthreads();
       int any_far = 0;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) any_far |= far[w];
+      for (int w = 0; w < W; ++w) any_far |= far[w];
       if (__builtin_amdgcn_readfirstlane(any_far) != 0) return false;
     }
   }
@@ -1156,11 +1156,11 @@ __device__ __forceinline__ bool many_one(const Args<MASK>& a, const Part& pt, co
 }
 
 // A range of tiles of streams of more rows, for one tile of rows of one kv head.
-template <int D, int MASK = kPlain>
+template <int D, int MASK = kPlain, int W = kWaves>
 __device__ __forceinline__ void many_part(const Args<MASK>& a, const Part& pt, const int block,
                                           unsigned char* smem) {
   const int Hk = pt.s.c.Hk;
-  const int n_rt = (pt.rows + ManyCfg<D>::kRows - 1) / ManyCfg<D>::kRows;
+  const int n_rt = (pt.rows + ManyCfg<D, W>::kRows - 1) / ManyCfg<D, W>::kRows;
   // Order: a prompt's last row tiles, which see the most keys, first; kv heads
   // side by side, so that with 8 of them each XCD keeps one head's keys in its L2.
   // Where all workgroups find a place at once (two per CU), the second half runs
@@ -1180,7 +1180,7 @@ __device__ __forceinline__ void many_part(const Args<MASK>& a, const Part& pt, c
   while (left > 0) {
     const int tiles = tiles_of<kManyTile, MASK>(a, stream, len);
     const int take = pt.budget == 0 ? tiles : min(left, tiles - first);
-    if (!many_one<D, MASK>(a, pt, kvh, rt, stream, len, first, take, take == tiles,
+    if (!many_one<D, MASK, W>(a, pt, kvh, rt, stream, len, first, take, take == tiles,
                            pt.budget == 0 ? item : item + stream, rounded, smem)) {
       rounded = true;
       __syncthreads();  // (the tiles' buffers take the part again)
@@ -1218,11 +1218,11 @@ __global__ __launch_bounds__(W * 64, 2) void few_masked_kernel(const Args<MASK> 
   few_part<D, W, false, MASK>(a, own, nullptr, blockIdx.x, smem);
 }
 
-template <int D, int MASK>
-__global__ __launch_bounds__(kThreads, 2) void many_masked_kernel(const Args<MASK> a, const Part own) {
-  using C = ManyCfg<D>;
+template <int D, int MASK, int W>
+__global__ __launch_bounds__(W * 64, 2) void many_masked_kernel(const Args<MASK> a, const Part own) {
+  using C = ManyCfg<D, W>;
   __shared__ __attribute__((aligned(256))) unsigned char smem[C::kSmem + (MASK == kTree ? tree_bytes(C::kRows) : 0)];
-  many_part<D, MASK>(a, own, blockIdx.x, smem);
+  many_part<D, MASK, W>(a, own, blockIdx.x, smem);
 }
 
 // A prefix's chunks (the first pre_blocks workgroups) and the items' own, side by
@@ -1366,7 +1366,7 @@ inline bool runs_few(int64_t heads, int64_t rows, int64_t cap, int D, int64_t cu
 }
 
 inline Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, int D, int64_t slots, int64_t cus,
-                         bool prefix, bool with_prefix) {
+                         bool prefix, bool with_prefix, int many_rows = kManyRows) {
   Planned h;
   Part& p = h.p;
   p.rows = (int)rows;
@@ -1374,7 +1374,7 @@ inline Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, in
   p.few = runs_few(streams * (int64_t)Hk, rows, cap, D, cus);
   p.prefix = prefix;
   p.direct = !with_prefix;
-  const int64_t row_tiles = p.few ? (rows + 31) / 32 : (rows + kManyRows - 1) / kManyRows;
+  const int64_t row_tiles = p.few ? (rows + 31) / 32 : (rows + many_rows - 1) / many_rows;
   const int64_t tile = p.few ? kFewTile : kManyTile;
   const int64_t tiles = (cap + tile - 1) / tile, groups = streams * row_tiles * Hk;
   p.min_chunk = p.few ? 4 : 2;
@@ -1385,7 +1385,7 @@ inline Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, in
                                         streams * ((tiles + p.min_chunk - 1) / p.min_chunk));
   } else {
     const int64_t k = p.few ? best_ranges(groups, (tiles + kWaves - 1) / kWaves, 0.9, 1.65, 32, D, slots, cus)
-                            : best_ranges(groups, tiles, 1.3, 2.1, kManyRows, D, slots, cus);
+                            : best_ranges(groups, tiles, many_rows > kManyRows ? 1.7 : 1.3, 2.1, many_rows, D, slots, cus);
     if (k > 1) p.budget = (int)(k * streams);
   }
   p.items = p.budget != 0 ? p.budget : streams;
@@ -1401,7 +1401,7 @@ inline Planned plan_part(int streams, int64_t rows, int per, int cap, int Hk, in
 struct Plan {
   Planned own, pre;
   bool both = false;  // few_kernel<D, W, true>
-  bool wide = false;  // few_kernel's W: 8, else 4
+  bool wide = false;  // W of few_kernel (of many_masked_kernel) is 8, else 4
 };
 
 inline Plan plan_of(int cap, int n_prefix, int p_cap, int B, int Sq, int H, int Hk, int D) {

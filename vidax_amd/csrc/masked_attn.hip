@@ -48,6 +48,26 @@ bool whole_streams(int64_t groups, int64_t tiles, int D, int64_t cus) {
   return t * (double)rounds / (double)waves <= t * (double)groups / (double)(slots * kWaves) + 11;
 }
 
+// us that many_part takes about (head dim 128). Two workgroups of four waves on a CU take
+// 1.83 a tile, one alone 1.3; one of eight, which converts a tile's keys and values once
+// for 256 rows, takes 1.7, but leaves less to fill an uneven round with. Measured, 4 / 8
+// waves:
+//   4680 rows of 12 heads on 20280 keys, one block       570 / 543 us
+//   9360                                                 1159 / 1071
+//   7800 on 17160 (372 workgroups of eight waves)        826 / 897 (not taken)
+//   2 x 1000 queries of 32 heads on 8, window 1500       66 / 62
+//   1 x 1000                                             46.3 / 54.5 (not taken)
+//   trees: 16 x 61 on 150 .. 8192 keys                   118 / 111
+// Whole streams whose lengths differ (queries on 3000 to 8192 keys: 189 / 211) stay with
+// two workgroups, a long one beside a short one.
+double many_time(const Planned& h, int streams, int64_t tiles, bool wide, int64_t cus) {
+  const int64_t k = h.p.budget > 0 ? h.p.budget / streams : 1, full = h.blocks / (2 * cus), rest = h.blocks % (2 * cus);
+  const double rounds = wide ? 1.7 * (double)((h.blocks + cus - 1) / cus)
+                             : 1.83 * (double)full + (rest == 0 ? 0 : rest <= cus ? 1.3 : 1.83);
+  const double rows = (double)h.blocks * (wide ? 2 * kManyRows : kManyRows);
+  return rounds * (double)((tiles + k - 1) / k) + (k > 1 ? 6 + 2 * rows * (128 + 2) * 4 / 4e6 : 0);
+}
+
 Plan masked_plan(int cap, int B, int Sq, int H, int Hk, int D, int window, int sinks, bool causal) {
   const int seen = seen_most(cap, Sq, H / Hk, window, sinks, causal);
   Plan p = plan_of(seen, 0, 0, B, Sq, H, Hk, D);
@@ -60,6 +80,15 @@ Plan masked_plan(int cap, int B, int Sq, int H, int Hk, int D, int window, int s
     p.own.blocks = (int64_t)B * Hk;
     p.own.floats = 0;
     p.wide = p.own.blocks <= cus;
+  }
+  if (!own.few && D == 128 && (B == 1 || own.budget > 0 || seen < cap)) {
+    Planned wide = plan_part(B, own.rows, 1, seen, Hk, D, cus, cus, false, false, 2 * kManyRows);
+    wide.p.one_round = false;
+    const int64_t tiles = (seen + kManyTile - 1) / kManyTile;
+    if (many_time(wide, B, tiles, true, cus) < many_time(p.own, B, tiles, false, cus)) {
+      p.own = wide;
+      p.wide = true;
+    }
   }
   return p;
 }
@@ -79,8 +108,11 @@ int launch(const MaskedAttnArgs& a, hipStream_t st, const char** launched) {
     hipLaunchKernelGGL((few_masked_kernel<D, 4, MASK>), grid, threads, 0, st, a, own);
     *launched = MASK == kTree ? (D == 128 ? "few_masked_kernel<128, 4, tree>" : "few_masked_kernel<64, 4, tree>")
                               : (D == 128 ? "few_masked_kernel<128, 4, window>" : "few_masked_kernel<64, 4, window>");
+  } else if (D == 128 && pl.wide) {
+    hipLaunchKernelGGL((many_masked_kernel<128, MASK, 8>), grid, dim3(512), 0, st, a, own);
+    *launched = MASK == kTree ? "many_masked_kernel<128, 8, tree>" : "many_masked_kernel<128, 8, window>";
   } else {
-    hipLaunchKernelGGL((many_masked_kernel<D, MASK>), grid, threads, 0, st, a, own);
+    hipLaunchKernelGGL((many_masked_kernel<D, MASK, 4>), grid, threads, 0, st, a, own);
     *launched = MASK == kTree ? (D == 128 ? "many_masked_kernel<128, tree>" : "many_masked_kernel<64, tree>")
                               : (D == 128 ? "many_masked_kernel<128, window>" : "many_masked_kernel<64, window>");
   }
