@@ -83,7 +83,9 @@ int32_t vx_kv_write_rope_check(const void* k, const void* v, const int64_t* k_st
  *   window  >= 1, the query's own position (not causal: the last one) among it
  *   sinks   >= 0
  * The other arguments, the numerics, and rows without a visible key, as there.
- * Positions that no query of a call sees are not read.
+ * What the cache holds at positions that no query of a call sees may be anything:
+ * never written, codes and scales of NaN. (Tiles of it are not read; what shares a
+ * tile of 64 positions with seen ones has no effect.)
  */
 int32_t vx_window_attn_fwd(const void* q, void* out, const int64_t* q_strides, const int64_t* out_strides,
                            const void* cache_k, const void* cache_v, const uint8_t* k_scale, const uint8_t* v_scale,

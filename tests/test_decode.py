@@ -939,6 +939,56 @@ def test_unseen_positions_are_not_read(gpu):
         assert torch.equal(vx.windowed_attention(q, junk, [n], window=window, sinks=sinks), want)
 
 
+UNSEEN = [
+    # kernels with heads of 64 and of 128, B, Sq, H, Hk, cap, kv_len, window, sinks, causal
+    ("few 8, few 8", 1, 1, 12, 12, 704, [690], 500, 10, True),            # both borders inside tiles
+    ("few 8, few 8", 1, 1, 12, 12, 704, [690], 640, 35, True),            # ... of the same tile: 35 .. 49
+    ("few 4, few 4", 1, 1, 4, 4, 704, [690], 1, 0, True),                 # one key of a tile
+    ("few 8, few 8", 1, 1, 4, 4, 704, [690], 34, 1, True),
+    ("few 4, few 4", 40, 1, 8, 8, 128, [100] * 39 + [33], 30, 2, True),
+    ("few 4, few 4", 2, 3, 8, 8, 8192, [8190, 5000], 4000, 70, True),     # in parts
+    ("few 8, few 8", 2, 40, 4, 1, 512, [500, 300], 100, 31, True),        # tiles of rows with windows of their own
+    ("few 8, few 8", 2, 20, 4, 1, 512, [500, 300], 77, 5, False),
+    ("many 4, many 4", 2, 256, 64, 16, 2048, [2000, 1400], 1000, 70, True),
+    ("many 4, many 4", 2, 600, 64, 32, 1024, [1000, 960], 300, 33, True),  # (the second item's: 33 .. 60)
+    ("few 4, many 8", 1, 600, 64, 32, 1024, [999], 300, 33, True),
+    ("many 4, many 4", 2, 700, 64, 32, 1024, [1000, 701], 500, 5, False),
+    ("many 4, many 8", 2, 256, 32, 8, 4096, [4000, 3001], 2500, 100, True),  # in parts
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("case", UNSEEN, ids=[str(c) for c in UNSEEN])
+def test_what_unseen_positions_hold_is_nothing(gpu, case, D):
+    """Whatever lies at positions that no query sees, up to the borders of the sinks and
+    of the window and behind the last token, changes no bit: NaN codes under scales of
+    NaN, the largest values under the largest scale, any bytes."""
+    kernels, B, Sq, H, Hk, cap, kv_len, window, sinks, causal = case
+    print(f"[case] unseen {case} D={D}", flush=True)
+    rng = np.random.default_rng(Sq + window)
+    cache = _cache_of(rng, B, Hk, cap, D, gpu)
+    q = _bf16(2 * rng.standard_normal((B, Sq, H, D)), gpu)
+    call = lambda c: vx.windowed_attention(q, c, _ints(kv_len, gpu), window=window, sinks=sinks, causal=causal)
+    want = call(cache)
+    print(f"  launched {_lib.last_launch()}", flush=True)
+    kind, waves = kernels.split(", ")[D // 128].split()
+    assert _lib.last_launch() == f"{kind}_masked_kernel<{D}, {waves}, window>".replace(", 4" * (kind == "many"), "")
+    assert not want.isnan().any()
+    seen = torch.zeros((B, cap), dtype=torch.bool)
+    for b, n in enumerate(kv_len):
+        seen[b, :n] = torch.from_numpy(O.window_sees(n, Sq, window, sinks, causal).any(0))
+        assert not seen[b, sinks:n].all()
+    hidden = (~seen).to(gpu)[:, None].expand(B, Hk, cap)
+    for code, scale in ((0xff, 255), (0x7e, 254), (None, None)):
+        junk = vx.KVCache(*(t.clone() for t in cache))
+        for t, x in zip(junk, (code, code, scale, scale)):
+            held = t.view(torch.uint8)
+            at = hidden[..., None].expand_as(held) if held.dim() == 4 else hidden
+            held[at] = x if x is not None else torch.from_numpy(rng.integers(0, 256, int(at.sum()), np.uint8)).to(gpu)
+        assert torch.equal(call(junk), want), code
+
+
 @pytest.mark.gpu
 def test_offsets_past_32_bits(gpu):
     """Positions of a slot that lies more than 2^32 bytes into the cache, written

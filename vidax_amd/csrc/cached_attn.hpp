@@ -130,7 +130,18 @@ __device__ __forceinline__ Window window_of(const MaskedAttnArgs& a, int low, in
   return w;
 }
 
-// Those of all rows of a stream of `keys` keys and m queries.
+// Keys from `first` on and before `end` are seen by none of the rows whose bounds begin
+// at `low`: they lie between the sinks and the rows' first window. (Tiles at its ends hold
+// seen keys too. A masked weight is zero, but what it multiplies has to be finite, and
+// what lies in the cache at such keys may be anything.)
+struct Unseen {
+  int first, end;
+};
+__device__ __forceinline__ Unseen unseen_of(const MaskedAttnArgs& a, int low) {
+  return Unseen{a.sinks, max(low - a.window, 0)};
+}
+
+// The window's tiles of all rows of a stream of `keys` keys and m queries.
 template <int TILE>
 __device__ __forceinline__ Window stream_window(const MaskedAttnArgs& a, int keys, int m) {
   return window_of<TILE>(a, a.causal ? max(keys - m + 1, 0) : keys, keys);
@@ -447,6 +458,7 @@ struct FewKeys {
   const uint8_t* scales;  // this lane's 16 bytes of a tile's scales (lanes 0-1 K, 2-3 V)
   int len;                // keys
   int bound, all;         // those that this lane's row sees, those that every row does
+  Unseen unseen;          // (a window's) that no row sees
 };
 
 // A range of tiles of streams, for 32 rows of one kv head (BOTH: stream `block`, the
@@ -480,7 +492,7 @@ __device__ __forceinline__ void few_part(const Args<MASK>& a, const Part& pt, co
     const int64_t at = ((int64_t)slot_of(from, stream) * Hk + kvh) * from.c.cap;
     return FewKeys{uniform_u64((uint64_t)(uintptr_t)(from.c.k + at * D)),
                    uniform_u64((uint64_t)(uintptr_t)(from.c.v + at * D)),
-                   (lane & 2 ? from.c.vs : from.c.ks) + at + 16 * (lane & 1), len, len, len};
+                   (lane & 2 ? from.c.vs : from.c.ks) + at + 16 * (lane & 1), len, len, len, Unseen{}};
   };
   // ---- staging: copy p of a tile fills 1024 / D rows; lane L takes row L / (D / 16),
   // LDS chunk L % (D / 16), which holds the row's chunk with that number XOR the swizzle
@@ -492,8 +504,14 @@ __device__ __forceinline__ void few_part(const Args<MASK>& a, const Part& pt, co
 #pragma unroll
     for (int p = 0; p < C::kCopies; ++p) {
       const int r = p * (1024 / D) + lane / T::kChunks;
-      // (rows past the last key repeat it: what lies there may be anything)
-      const uint32_t off = (uint32_t)(min(r, last) * D + ((lane % T::kChunks) ^ T::swizzle(r)) * 16);
+      // (rows past the last key repeat it: what lies there may be anything; and rows that no
+      // row of queries sees the key behind them or, where that is another tile's, in front)
+      int row = min(r, last);
+      if constexpr (MASK == kWindow) {
+        const int u0 = x.unseen.first - t * kFewTile, u1 = x.unseen.end - t * kFewTile;
+        if (u0 < kFewTile && u1 > 0) row = r >= u0 && r < u1 ? (u1 < kFewTile ? u1 : u0 - 1) : row;
+      }
+      const uint32_t off = (uint32_t)(row * D + ((lane % T::kChunks) ^ T::swizzle(r)) * 16);
       lds_dma16_buf(rk, off, dst + p * 1024);
       lds_dma16_buf(rv, off, dst + C::kTileBytes + p * 1024);
     }
@@ -555,6 +573,7 @@ __device__ __forceinline__ void few_part(const Args<MASK>& a, const Part& pt, co
       from = any - a.window;
       const int m = __builtin_amdgcn_readfirstlane(clamp_len(a.q_len, stream, a.Sq));
       pieces = pieces_of(stream_window<kFewTile>(a, len, m), window_of<kFewTile>(a, low, any), first, take);
+      own.unseen = unseen_of(a, low);
     }
     if constexpr (MASK == kTree) {
       base = len - __builtin_amdgcn_readfirstlane(clamp_len(a.q_len, stream, a.Sq));
@@ -831,6 +850,7 @@ __device__ __forceinline__ bool many_one(const Args<MASK>& a, const Part& pt, co
   // keys that any row of the workgroup sees
   int end = len, base = 0;
   Pieces pieces{};
+  Unseen unseen{};
   if (!pt.prefix) {
     const int m = clamp_len(a.q_len, stream, a.Sq);
     const int i0 = rt * C::kRows / map.G, i1 = min(rt * C::kRows + C::kRows - 1, rows - 1) / map.G;
@@ -839,6 +859,7 @@ __device__ __forceinline__ bool many_one(const Args<MASK>& a, const Part& pt, co
     if constexpr (MASK == kWindow) {
       const int low = __builtin_amdgcn_readfirstlane(i0 < m ? own_bound(a, stream, i0, len) : 0);
       pieces = pieces_of(stream_window<kManyTile>(a, len, m), window_of<kManyTile>(a, low, end), first, take);
+      unseen = unseen_of(a, low);
     }
     if constexpr (MASK == kTree) base = __builtin_amdgcn_readfirstlane(len - m);
   }
@@ -992,6 +1013,16 @@ __device__ __forceinline__ bool many_one(const Args<MASK>& a, const Part& pt, co
               S[k2][i] = key < bound ? S[k2][i] * c : -__builtin_inff();
             else
               S[k2][i] = masked_by(bits, (i >> 2) * 8 + (i & 3), S[k2][i] * c);
+          }
+        }
+        if constexpr (MASK == kWindow) {
+          // (values that no row sees, on their way to LDS; such a tile is slow for every wave)
+          if (key0 < unseen.end && key0 + kManyTile > unseen.first) {
+#pragma unroll
+            for (int p = 0; p < C::kLoads; ++p) {
+              const int key = key0 + p * kKeysPerPass + skey;
+              if (key >= unseen.first && key < unseen.end) wv.x[p] = u32x4{0, 0, 0, 0};
+            }
           }
         }
       }

@@ -8,7 +8,9 @@
 //           of its sinks and of the union of its rows' windows, so the ranges that
 //           workgroups take hold no tile that nobody sees, and each tile of rows
 //           skips what its own rows do not see; only tiles at a row's border, at
-//           either end, are masked key by key.
+//           either end, are masked key by key. What lies in such a tile at keys that none
+//           of its rows sees (Unseen) is kept out of the products: another key's bytes
+//           are copied in their place, or zeros stored.
 //   tree    keys in front of the drafted ones as ever; of those, the query's
 //           ancestors and itself, as bits in LDS that each row walks out from the
 //           parents once per part (fill_tree): a tile takes 32 of a row's bits from

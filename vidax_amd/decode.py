@@ -233,9 +233,9 @@ def windowed_attention(q: torch.Tensor, cache: KVCache, kv_len=None, *, window: 
     tokens, prompts in chunks). False: the queries are one block whose tokens see
     each other: all of them see the last `window` of the kv_len tokens, their own
     among them, and the first `sinks` (a block of a rollout over the frames before
-    it). Positions that no query sees are not read. The other arguments, lengths
-    outside their range, queries without a visible key and rows of scale NaN are as
-    in cached_attention.
+    it). What the cache holds at positions that no query sees may be anything, as
+    past kv_len. The other arguments, lengths outside their range, queries without a
+    visible key and rows of scale NaN are as in cached_attention.
     """
     window, sinks = int(window), int(sinks)
     if window < 1 or sinks < 0:
