@@ -27,8 +27,8 @@ int32_t vx_decode_abi_version(void);
  * turn's input, from that of its output.
  *   x          bf16 (batch, seq, num_heads, head_dim), 16-byte aligned; strides
  *              {batch, seq, head} in elements, multiples of 8 (NULL: contiguous)
- *   out        bf16, the same shape, contiguous, 16-byte aligned; x itself or no
- *              part of it
+ *   out        bf16, the same shape, contiguous, 16-byte aligned; x itself, if that is
+ *              contiguous (refused if not), or no part of it
  *   positions  int32 at strides {batch, token, axis} in elements (>= 0; 0: shared;
  *              NULL: contiguous (batch, seq, num_axes))
  *   num_axes   1 to 4
@@ -47,7 +47,7 @@ int32_t vx_axis_rope_fwd(const void* x, void* out, const int64_t* x_strides, con
                          const int32_t* axis, int32_t halves, int32_t inverse, int32_t batch, int32_t seq,
                          int32_t num_heads, int32_t head_dim, void* stream);
 
-/* Host-only argument check for vx_axis_rope_fwd (no GPU needed). */
+/* Host-only argument check for vx_axis_rope_fwd (no GPU needed; whether out is x is not looked at). */
 int32_t vx_axis_rope_check(const void* x, const void* out, const int64_t* x_strides, const int32_t* positions,
                            const int64_t* position_strides, int32_t num_axes, const uint64_t* turns,
                            const int32_t* axis, int32_t halves, int32_t inverse, int32_t batch, int32_t seq,

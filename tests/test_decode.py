@@ -190,6 +190,27 @@ def test_injected_error_is_reported():
         L.vx_debug_inject_error(0)
 
 
+def test_turning_in_place_needs_contiguous_rows():
+    """out is written contiguously: where x is the same memory at other strides, rows
+    would be overwritten before they are read. (Strides of a single item, token or head
+    say nothing.) Refused before anything is launched."""
+    L, positions = _lib.lib(), _lib.strides3((6, 3, 1))
+    call = lambda x, o, st, B=2, S=3, H=4: L.vx_axis_rope_fwd(x, o, _s3(st), A, positions, 3, A, A, 0, 0, B, S, H, 64,
+                                                              None)
+    L.vx_debug_inject_error(_lib.VX_ERR_LAUNCH)  # (what is not refused)
+    try:
+        for st in ((0, 256, 64), (768, 0, 64), (768, 256, 0), (768, 64, 192), (2304, 768, 64), (256, 512, 64)):
+            assert call(A, A, st) == INVALID, st
+            assert "in-place" in _lib.last_error()
+            assert call(A, A + (1 << 20), st) == _lib.VX_ERR_LAUNCH
+        for sizes, st in ((dict(), None), (dict(), (768, 256, 64)), (dict(B=1), (8, 256, 64)),
+                          (dict(B=1, S=1), (8, 16, 64)), (dict(S=1), (256, 8, 64)), (dict(H=1), (192, 64, 8)),
+                          (dict(B=1, S=1, H=1), (0, 0, 0))):
+            assert call(A, A, st, **sizes) == _lib.VX_ERR_LAUNCH, (sizes, st)
+    finally:
+        L.vx_debug_inject_error(0)
+
+
 def test_a_missing_workspace_is_refused():
     L, f = _lib.lib(), ctypes.c_float(0.1)
     for ws, n in ((None, 1 << 40), (A + 4, 1 << 40), (A, 16)):
@@ -381,6 +402,22 @@ def test_positions_and_rows_of_any_layout(gpu):
     assert vx.apply_axis_rope(x[:0], p[:0], rope).shape == (0, 21, 4, 64)
     assert vx.apply_axis_rope(x[:, :0], p[:, :0], rope).shape == (2, 0, 4, 64)
     assert vx.apply_axis_rope(x[:, :, :0], p, rope).shape == (2, 21, 0, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("halves", [0, 1])
+@pytest.mark.parametrize("B,S,H,D", [(1, 1, 1, 64), (3, 37, 71, 64), (2, 130, 40, 128)])
+def test_turning_in_place(gpu, B, S, H, D, halves):
+    """The C entry with out = x gives what it gives elsewhere, bit for bit."""
+    print(f"[case] in place B={B} S={S} H={H} D={D} halves={halves}", flush=True)
+    rope = vx.create_axis_rope(D, (D // 4, D // 4, D // 4), halves=bool(halves), device=gpu)
+    g = torch.Generator(device=gpu).manual_seed(S)
+    x = torch.randn((B, S, H, D), generator=g, device=gpu).bfloat16()
+    p = torch.randint(0, 5000, (B, S, 3), generator=g, device=gpu, dtype=torch.int32)
+    want = vx.apply_axis_rope(x, p, rope)
+    _lib.launch(x.device, _lib.lib().vx_axis_rope_fwd, x.data_ptr(), x.data_ptr(), None, p.data_ptr(), None, 3,
+                rope.turns.data_ptr(), rope.axis.data_ptr(), halves, 0, B, S, H, D)
+    assert torch.equal(x, want)
 
 
 @pytest.mark.gpu

@@ -1507,6 +1507,11 @@ int32_t vx_axis_rope_fwd(const void* x, void* out, const int64_t* x_strides, con
   int32_t rc = axis_rope_args(x, out, x_strides, positions, position_strides, num_axes, turns, axis, halves, inverse,
                               batch, seq, num_heads, head_dim, &a);
   if (rc != VX_OK) return rc;
+  // (rows that lie elsewhere in x than in out would be overwritten before they are read)
+  const int64_t row = (int64_t)num_heads * head_dim;
+  if (x == out && ((batch > 1 && a.xs[0] != seq * row) || (seq > 1 && a.xs[1] != row) ||
+                   (num_heads > 1 && a.xs[2] != head_dim)))
+    return fail(VX_ERR_INVALID_ARGUMENT, "in-place use (out == x) needs contiguous rows");
   if ((rc = injected()) != VX_OK) return rc;
   const char* launched = "";
   const int err = vx::launch_axis_rope(a, stream, &launched);
