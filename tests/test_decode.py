@@ -9,9 +9,11 @@ y = u c - w s is off by at most
 before it is stored in 8 bits: half a step of e4m3 and the first of these.
 """
 import ctypes
+import decimal
 import math
 import os
 import re
+from decimal import Decimal as D_
 
 import numpy as np
 import pytest
@@ -241,6 +243,37 @@ def test_turns_are_the_ladders(D, split, shared, base, scale):
             off = (got - want) % 1.0
             assert min(off, 1 - off) <= 2.0 ** -51 * max(1.0, want) and int(rope.axis[at]) == a
             at += 1
+    assert (rope.turns[at:] == 0).all()
+
+
+def _pi(digits):
+    """By the arithmetic-geometric mean (Gauss and Legendre), in a context of that precision."""
+    a, b, t, p = D_(1), 1 / D_(2).sqrt(), D_(1) / 4, D_(1)
+    for _ in range(digits.bit_length() + 2):
+        a, b, t, p = (a + b) / 2, (a * b).sqrt(), t - p * ((a - b) / 2) ** 2, 2 * p
+    return (a + b) ** 2 / (4 * t)
+
+
+@pytest.mark.parametrize("D,split,shared", [(128, (44, 42, 42), False), (64, (64,), False), (64, (8, 0, 24, 32), True)])
+@pytest.mark.parametrize("base,scale", [(10000.0, None), (5e6, (24.0, 1.0, 0.1, 1e6)), (500000.0, (-1 / 3, 24, 1e-9, 7)),
+                                        (1e-300, (1.0, 2.0, 3.0, 4.0)), (1.5e308, (1e300, -1e308, 5e-324, 2.0 ** 80))])
+def test_turns_are_rounded_once(D, split, shared, base, scale):
+    """turns is scale * base^-e / 2 pi modulo 1 to the nearest of 2^64 steps: base and
+    scale are taken as the numbers they are, so positions of 2^31 are off by 2^-34 of a
+    turn at most whatever the scale."""
+    scale = (1.0,) * len(split) if scale is None else scale[:len(split)]
+    rope = vx.create_axis_rope(D, split, base, shared=shared, axis_scale=scale, device="cpu")
+    digits = 120 if 1 < base < 1e9 else 800
+    with decimal.localcontext(decimal.Context(prec=digits, traps=[])):
+        two_pi, at = 2 * _pi(digits), 0
+        for a, channels in enumerate(split):
+            for i in range(channels // 2):
+                e = D_(2 * at) / D if shared else D_(2 * i) / channels
+                want = D_(scale[a]) * D_(base) ** -e / two_pi * 2 ** 64
+                off = (int(rope.turns[at]) - want) % 2 ** 64  # (Decimal's remainder keeps the sign)
+                off = min(abs(off), 2 ** 64 - abs(off))
+                assert off <= D_("0.5000001"), (at, off)
+                at += 1
     assert (rope.turns[at:] == 0).all()
 
 

@@ -17,8 +17,10 @@ graph may be replayed while they change.
 """
 from __future__ import annotations
 
+import decimal
 import functools
 import math
+from decimal import Decimal
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -42,6 +44,35 @@ class AxisRope(NamedTuple):
     halves: bool
 
 
+@functools.lru_cache(maxsize=8)
+def _two_pi(digits: int) -> Decimal:
+    """2 pi to that many digits: pi / 4 = 4 arctan(1/5) - arctan(1/239) (Machin)."""
+    one = 10 ** (digits + 10)
+
+    def arctan_of_inverse(n: int) -> int:
+        total, power, k = 0, one // n, 1
+        while power:
+            total += power // k if k % 4 == 1 else -(power // k)
+            power, k = power // (n * n), k + 2
+        return total
+
+    return Decimal(8 * (4 * arctan_of_inverse(5) - arctan_of_inverse(239))) / one
+
+
+def _turns_of(base: float, ladder: Sequence[tuple]) -> list:
+    """scale * base^-(n / d) / 2 pi for each (scale, n, d), in units of 2^-64, whole turns
+    left out, rounded once: 53 bits of a float would leave position * 2^-56 of a turn, and
+    as much times the scale. (n < d, so what is largest are the scale and 1 / base.)"""
+    largest = max((abs(scale) for scale, _, _ in ladder), default=0.0)
+    # (those of the whole turns, and 20 behind the point, with room for roundings)
+    digits = 60 + sum(int(math.log10(x)) + 1 for x in (largest, 1 / max(base, 1e-308)) if x > 1)
+    with decimal.localcontext(decimal.Context(prec=digits, rounding=decimal.ROUND_HALF_EVEN, Emin=-99999, Emax=99999,
+                                              traps=[])):
+        unit, log = Decimal(2 ** 64) / _two_pi(digits), Decimal(base).ln()
+        return [int((Decimal(scale) * (log * -n / d).exp() * unit).to_integral_value()) % 2 ** 64
+                for scale, n, d in ladder]
+
+
 def create_axis_rope(head_dim: int, split: Sequence[int], base: float = 10000.0, *, shared: bool = False,
                      halves: bool = False, axis_scale: Optional[Sequence[float]] = None, device=None) -> AxisRope:
     """The turns of a head whose channels are split over axes: split[a] channels
@@ -51,7 +82,9 @@ def create_axis_rope(head_dim: int, split: Sequence[int], base: float = 10000.0,
     (the ladder of create_rope3d_freqs and create_abs_rope3d_freqs); shared: pair j
     of the head by position * base^(-2 j / head_dim). axis_scale: a factor of each
     axis's positions (frames per second, a coarser grid). halves as in AxisRope
-    (default: adjacent channels, as in apply_rope3d).
+    (default: adjacent channels, as in apply_rope3d). The turns are rounded once, to
+    the nearest 2^-64 of a turn: at any position the angle is that of base and
+    axis_scale, as the numbers they are, to within 2^-34 of a turn.
     """
     if head_dim not in (64, 128):
         raise NotImplementedError(f"head_dim {head_dim} is not supported (64 and 128 are)")
@@ -66,12 +99,12 @@ def create_axis_rope(head_dim: int, split: Sequence[int], base: float = 10000.0,
     base = float(base)
     if not (base > 0 and math.isfinite(base)):
         raise ValueError(f"base must be positive and finite; got {base}")
-    turns, axis = [], []
+    ladder, axis = [], []
     for a, (channels, scale) in enumerate(zip(split, scales)):
         for i in range(channels // 2):
-            exponent = 2 * len(turns) / head_dim if shared else 2 * i / channels
-            turns.append(round(scale * base ** -exponent / (2 * math.pi) * 2.0 ** 64) % 2 ** 64)
+            ladder.append((scale, 2 * len(ladder), head_dim) if shared else (scale, 2 * i, channels))
             axis.append(a)
+    turns = _turns_of(base, ladder)
     still = head_dim // 2 - len(turns)
     turns = [t - 2 ** 64 if t >= 2 ** 63 else t for t in turns] + [0] * still
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
