@@ -8,7 +8,8 @@
 //   few_part   32 rows: four (or eight) waves, each on every fourth 32-key tile of
 //              the range (single tokens, short prompts, small prefixes)
 //   many_part  128 rows: four waves of 32 rows each on the same 64-key tiles
-//              (prompts in chunks, cross-attention, a long prefix under a batch)
+//              (prompts in chunks, cross-attention, a long prefix under a batch); under
+//              a mask also 256 rows and eight waves (see masked_attn.hip)
 //   merge      joins the parts of a stream, and a prefix's with the items' own
 //
 // All compute S^T = K Q^T and O^T = V^T P^T with v_mfma_f32_32x32x16_bf16, so that a
@@ -27,7 +28,7 @@
 // the transposed read gives a lane eight keys of one dim. It is bound by memory for
 // single tokens: 64 sequences of 227 to 8192 keys, 8 kv heads, 562 MB in 105 us (5.4
 // TB/s); two of 131000 and 105009 keys 488 MB in 90 us (5.4 TB/s).
-// many_part converts each 64-key tile once for its four waves, on the way to LDS,
+// many_part converts each 64-key tile once for its waves, on the way to LDS,
 // and runs the matrix cores of a tile beside the next one's softmax and conversions:
 // 1000 and 943 queries of 32 heads on 5003 and 4324 keys 138 us (0.96 PFLOP/s; 150 to
 // 175 us in the first calls after an idle time). The matrix cores are busy 44 % of that

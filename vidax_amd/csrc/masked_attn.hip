@@ -35,14 +35,21 @@ int seen_most(int cap, int Sq, int G, int window, int sinks, bool causal) {
   return (int)std::min<int64_t>(cap, most);
 }
 
-// Ranges of few rows go over streams, with a launch that merges; a window makes the
-// streams' lengths alike, so often each is one workgroup's (us a call; 32 heads on 8,
-// lengths 150 to 8192, streams whole / in ranges):
-//   window       1100         2048         4096         8192
-//   8 items      16 / 22      20 / 25      31 / 28      53 / 30
-//   32           21 / 30      28 / 37      52 / 64      75 / 77
-//   64           32 / 43      55 / 66      91 / 97      118 / 119
-//   100          56 / 62      82 / 92      139 / 138    201 / 180
+// Ranges of few rows go over streams, with a launch that merges. Where most streams are
+// longer than the window it makes them alike, so often each is one workgroup's. Measured,
+// streams whole / in ranges, where the rule takes them whole (us a call; 32 heads on 8,
+// capacity 8192, lengths spread evenly over 150 to 8192):
+//   window       1100           2048           4096           8192
+//   8 items      12.9 / 17.1    19.6 / 18.7
+//   32           17.3 / 24.8    24.9 / 31.8    39.1 / 46.2    74.0 / 57.6
+//   64           28.2 / 38.2    48.8 / 57.8    77.7 / 83.6    131 / 121
+//   100          42.6 / 50.4
+// The rule has the capacity, not the lengths, which are on the device. A stream of 8192
+// among ones of 200 takes its time alone, and a window of the capacity bounds nothing:
+//   8            12.9 / 16.1    19.2 / 15.4
+//   32           13.1 / 17.6    19.7 / 18.6    33.1 / 21.3    60.2 / 22.7
+//   64           17.0 / 19.4    26.3 / 19.6    48.2 / 24.6    92.2 / 27.1
+//   100          19.1 / 25.5
 // A 32-key tile takes a wave 1.65 us, and ranges cost 11 more.
 bool whole_streams(int64_t groups, int64_t tiles, int D, int64_t cus) {
   const int64_t slots = 2 * cus, rounds = (groups + slots - 1) / slots, waves = groups <= cus ? 8 : 4;
@@ -60,8 +67,12 @@ bool whole_streams(int64_t groups, int64_t tiles, int D, int64_t cus) {
 //   2 x 1000 queries of 32 heads on 8, window 1500       66 / 62
 //   1 x 1000                                             46.3 / 54.5 (not taken)
 //   trees: 16 x 61 on 150 .. 8192 keys                   118 / 111
-// Whole streams whose lengths differ (queries on 3000 to 8192 keys: 189 / 211) stay with
-// two workgroups, a long one beside a short one.
+// Whole streams that no window bounds (of a tree, or seen to the capacity) stay with two
+// workgroups, a long one beside a short one (queries on 3000 to 8192 keys: 189 / 211).
+// Those of a window count as alike, though a wide one leaves them their lengths: window
+// 8000 of 8192, 256 queries of 32 heads on 8, lengths of 3000 to 8192, 4 items 117 / 114,
+// 8 items 193 / 210, 16 items 418 / 419; 8 items of which one has 8192 keys and the
+// others 1100, 160 / 196.
 double many_time(const Planned& h, int streams, int64_t tiles, bool wide, int64_t cus) {
   const int64_t k = h.p.budget > 0 ? h.p.budget / streams : 1, full = h.blocks / (2 * cus), rest = h.blocks % (2 * cus);
   const double rounds = wide ? 1.7 * (double)((h.blocks + cus - 1) / cus)

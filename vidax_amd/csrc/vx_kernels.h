@@ -273,7 +273,8 @@ int64_t masked_attn_workspace(int32_t cap, int32_t B, int32_t Sq, int32_t H, int
 
 // All return a hipError_t value (0 on success) and store the name of the kernel they launched in *launched (a string with
 // static storage, built from the launched instantiation's template
-// arguments).
+// arguments). Two go unnamed: that kv_write_rope_kernel's waves share their angles (heads
+// in fours), and that many_masked_kernel has its usual four waves.
 int launch_flash_fwd(const FlashArgs& a, void* stream, const char** launched);
 int launch_na3d_fwd(const Na3dArgs& a, void* stream, const char** launched);
 int launch_qk_prologue(const PrologueArgs& a, void* stream, const char** launched);
