@@ -5,7 +5,7 @@
 // heads a pass, whole lines on both sides, in up to kPasses passes whose loads are
 // all in flight before the angles are formed: they are formed once for all of the
 // wave's heads, and their cost hides behind the loads. Measured: 32760 tokens of 40
-// heads of 128 in 119 us (5.6 TB/s; a copy of 1 GiB 5.2), 2 x 5003 of 16 heads of 64 in
+// heads of 128 in 119 us (5.6 TB/s; a copy of 1 GiB 5.1), 2 x 5003 of 16 heads of 64 in
 // 12, eight single tokens of 32 heads in 4.2. Not kept: several tokens of few heads per
 // wave (11.5 -> 12.5).
 #include "vx_axis_rope.hpp"

@@ -16,12 +16,12 @@
 //           parents once per part (fill_tree): a tile takes 32 of a row's bits from
 //           two words of them, one VALU instruction.
 //
-// Measured (kernels): one query of 12 heads in a window of 256 of 700 tokens 8.0 us,
+// Measured (kernels): one query of 12 heads in a window of 256 of 700 tokens 8.1 us,
 // latency of 9 tiles on eight waves; 64 sequences of 150 to 8192 tokens, 32 heads on 8,
 // window 2048, 53 us (245 MB, 4.6 TB/s); 1000 and 777 queries of 32 heads, window 1500,
-// 65 us (51 GFLOP), and 4680 of 12 heads on 20280 keys 543 us (583 GFLOP, 1.07 PFLOP/s),
+// 65 us (51 GFLOP), and 4680 of 12 heads on 20280 keys 544 us (583 GFLOP, 1.07 PFLOP/s),
 // both bound by many_part's loop; trees of 30 to 61 tokens of 32 heads on 150 to 8192
-// keys, 16 items, 99 us and the merge of 48 MB of partial rows 15.
+// keys, 16 items, 95 us and the merge of 48 MB of partial rows 15.
 #include "cached_attn.hpp"
 
 namespace vx {
